@@ -7,7 +7,8 @@ SRCS  := $(CSRC)/vita_api.hip $(CSRC)/vita_gemm_f32.hip $(CSRC)/vita_gemm_f32_dm
 HDRS  := $(CSRC)/vita_common.h $(CSRC)/vita_host.h $(CSRC)/vita_gemm_epilogue.h $(CSRC)/vita_gemm_dma_tile.h $(CSRC)/vita_ode_sync.h $(CSRC)/vita_splitk_fused.h include/vita_hip.h
 OBJS  := $(SRCS:.hip=.o)
 LIB   := vita_amd/libvita_hip.so
-HIPFLAGS := --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -ffp-contract=off -Wall -Wno-unused-function
+# packed fp32 arithmetic off: hipcc forms v_pk_{add,mul,fma}_f32 from ordinary float code, and some of their forms have given wrong results
+HIPFLAGS := --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -ffp-contract=off -Wall -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops
 
 all: $(LIB)
 

@@ -657,6 +657,106 @@ int vita_compute_loss_meanflow_f32(const vita_meanflow_policy_weights* w, const 
                                    float* d_obs_features, int64_t ld_dobs, void* const* grad_ready, void* workspace,
                                    size_t workspace_bytes, vita_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Operators of the transformer blocks (flare/models/attention.py, models/transformer/blocks.py; the modules are
+ * vita_amd/encoders.py).  dtype is that of the activations (and, where said, of a table or weight); strides are in elements; the last
+ * dimension of every tensor is contiguous.  Statistics, softmax and sums are fp32, each result is rounded once.
+ * --------------------------------------------------------------------------------------- */
+enum { VITA_DT_F32 = 0, VITA_DT_BF16 = 1 };
+enum { VITA_NORM_LAYER = 0, /* (x - mean) / sqrt(var + eps): nn.LayerNorm(head_dim), attention.py:38-39 */
+       VITA_NORM_RMS = 1    /* x / sqrt(mean(x^2) + eps) */ };
+
+/* ---------------------------------------------------------------------------------------
+ * vita_qk_norm_rope — `rope(q_norm(q)), rope(k_norm(k))` (attention.py:50-57) in one launch: a norm over each head's D elements with
+ * weight and bias, then the rotation of neighbouring pairs by the token's position (pos_embed.py:103-125).
+ *   x (B, S, H, D) -> y (B, S, H, D) for queries and keys, each with its own head count; y may be x itself.
+ *   rope (rope_rows, rope_heads, D / 2, 2) fp32 = (cos, sin) of a position; rope_heads = 1: one table for every head, = H: the
+ *   reference's RotaryPosEmbed cache (rope_rows, dim / 2, 2), whose frequencies are dealt to the heads in order.
+ *   positions: int64 (B, S) with row stride ld_positions (0: one row for the batch), or NULL = 0 .. S - 1.  A position outside
+ *   [0, rope_rows) never leaves the table: its row (and, in the backward pass, the weights' gradients) becomes NaN.
+ *   D even, 2 .. 256.  weight / bias: fp32 (D) or NULL (1 / 0).
+ * Backward (dy given, y receives dx; dx may be dy or x itself): dx for queries and keys, dweight / dbias (fp32, written; NULL = not
+ * wanted), summed in a fixed order.
+ * --------------------------------------------------------------------------------------- */
+typedef struct vita_norm_rope_side {
+    const void* x; int64_t x_sb, x_ss, x_sh;      /* strides of batch, token, head */
+    void* y; int64_t y_sb, y_ss, y_sh;
+    const void* dy; int64_t dy_sb, dy_ss, dy_sh;  /* backward only */
+    const float *weight, *bias;
+    float *dweight, *dbias;                       /* backward only */
+    int32_t H;
+} vita_norm_rope_side;
+typedef struct vita_norm_rope_args {
+    int32_t dtype, norm, B, S, D;
+    float eps;
+    const float* rope; int64_t rope_rows; int32_t rope_heads;
+    const int64_t* positions; int64_t ld_positions;
+    vita_norm_rope_side q, k;
+} vita_norm_rope_args;
+int vita_qk_norm_rope(const vita_norm_rope_args* args, vita_stream_t stream);
+size_t vita_qk_norm_rope_bwd_workspace_bytes(const vita_norm_rope_args* args);
+int vita_qk_norm_rope_bwd(const vita_norm_rope_args* args, void* workspace, size_t workspace_bytes, vita_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
+ * vita_attention — softmax attention (F.scaled_dot_product_attention, attention.py:58) with a learned relative position bias:
+ *   s[i, j] = scale * q_i . k_j + table[buckets[clamp(j - (i + Sk - Sq), -radius, radius) + radius], h],   o_i = sum_j softmax_j(s) v_j
+ *   q, o (B, Sq, H, D), k, v (B, Sk, Hk, D): head h reads key head h / (H / Hk).  The queries are the LAST Sq of the Sk positions.
+ *   causal: key j is seen by query i when j <= i + Sk - Sq.  key_pad (B, Sk) bytes, row stride ld_pad: nonzero = the key does not
+ *   exist (is_pad of the dataset's batches); whatever its k and v hold is not used.  A query that sees no key gives zeros.
+ *   table (num_buckets, H) of the call's dtype, buckets int32 (2 radius + 1), radius <= 1024; table NULL = no bias.  An id outside
+ *   [0, num_buckets) makes its scores NaN.
+ *   D a multiple of 8, <= 128; tensors and their strides 16-byte aligned.  lse (B, H, Sq) or NULL: log sum exp of each row's scores
+ *   (-inf for a query without keys), what the backward pass needs.
+ * Backward: dq, dk, dv (written), dtable (num_buckets, H) of the call's dtype (NULL = not wanted), from dout, o and lse; every sum
+ * in a fixed order.
+ * --------------------------------------------------------------------------------------- */
+typedef struct vita_attention_args {
+    int32_t dtype, B, H, Hk, Sq, Sk, D, causal;
+    float scale;
+    const void* q; int64_t q_sb, q_ss, q_sh;
+    const void* k; int64_t k_sb, k_ss, k_sh;
+    const void* v; int64_t v_sb, v_ss, v_sh;
+    void* o; int64_t o_sb, o_ss, o_sh;            /* backward: read */
+    float* lse;                                   /* backward: read */
+    const uint8_t* key_pad; int64_t ld_pad;
+    const void* table; const int32_t* buckets; int32_t radius, num_buckets;
+    const void* dout; int64_t dout_sb, dout_ss, dout_sh;
+    void* dq; int64_t dq_sb, dq_ss, dq_sh;
+    void* dk; int64_t dk_sb, dk_ss, dk_sh;
+    void* dv; int64_t dv_sb, dv_ss, dv_sh;
+    void* dtable;
+} vita_attention_args;
+size_t vita_attention_workspace_bytes(const vita_attention_args* args);
+int vita_attention(const vita_attention_args* args, void* workspace, size_t workspace_bytes, vita_stream_t stream);
+size_t vita_attention_bwd_workspace_bytes(const vita_attention_args* args);
+int vita_attention_bwd(const vita_attention_args* args, void* workspace, size_t workspace_bytes, vita_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
+ * vita_gated_linear — the gated feed-forward product: z = x . w^T + b, h = act(z[:, :F]) * z[:, F:]
+ *   x (M, K), w (2F, K): rows 0 .. F - 1 the gate, F .. 2F - 1 the up projection, b (2F) fp32 or NULL, h (M, F); act VITA_ACT_RELU ..
+ *   VITA_ACT_MISH.  K and F multiples of 8; rows 16-byte aligned.
+ *   z: NULL, or (M, 2F) fp32 that receives the pre-activations.
+ * Backward from dh (M, F):  dz = [dh * z_up * act'(z_gate) | dh * act(z_gate)],  dx = dz . w,  dw = dz^T . x,  db = column sums of dz
+ *   (dx (M, K) and dw (2F, K) of the call's dtype, db fp32; each may be NULL).  z: the forward call's, or NULL = formed again from x and w.
+ *   Every sum is in a fixed order.
+ * --------------------------------------------------------------------------------------- */
+typedef struct vita_gated_args {
+    int32_t dtype, act, M, F, K;
+    const void* x; int64_t ldx;
+    const void* w; int64_t ldw;
+    const float* b;
+    void* h; int64_t ldh;                         /* forward */
+    float* z; int64_t ldz;
+    const void* dh; int64_t ld_dh;                /* backward */
+    void* dx; int64_t ld_dx;
+    void* dw; int64_t ld_dw;
+    float* db;
+} vita_gated_args;
+size_t vita_gated_linear_workspace_bytes(const vita_gated_args* args);
+int vita_gated_linear(const vita_gated_args* args, void* workspace, size_t workspace_bytes, vita_stream_t stream);
+size_t vita_gated_linear_bwd_workspace_bytes(const vita_gated_args* args);
+int vita_gated_linear_bwd(const vita_gated_args* args, void* workspace, size_t workspace_bytes, vita_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -140,6 +140,37 @@ class Bf16Weights(C.Structure):
     ]
 
 
+class NormRopeSide(C.Structure):
+    _fields_ = [("x", c_fp), ("x_sb", C.c_int64), ("x_ss", C.c_int64), ("x_sh", C.c_int64),
+                ("y", c_fp), ("y_sb", C.c_int64), ("y_ss", C.c_int64), ("y_sh", C.c_int64),
+                ("dy", c_fp), ("dy_sb", C.c_int64), ("dy_ss", C.c_int64), ("dy_sh", C.c_int64),
+                ("weight", c_fp), ("bias", c_fp), ("dweight", c_fp), ("dbias", c_fp), ("H", C.c_int32)]
+
+
+class NormRopeArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("norm", C.c_int32), ("B", C.c_int32), ("S", C.c_int32), ("D", C.c_int32), ("eps", C.c_float),
+                ("rope", c_fp), ("rope_rows", C.c_int64), ("rope_heads", C.c_int32),
+                ("positions", c_fp), ("ld_positions", C.c_int64), ("q", NormRopeSide), ("k", NormRopeSide)]
+
+
+class AttentionArgs(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "B", "H", "Hk", "Sq", "Sk", "D", "causal")] + [("scale", C.c_float)]
+                + [f for n in ("q", "k", "v", "o") for f in ((n, c_fp), (n + "_sb", C.c_int64), (n + "_ss", C.c_int64), (n + "_sh", C.c_int64))]
+                + [("lse", c_fp), ("key_pad", c_fp), ("ld_pad", C.c_int64), ("table", c_fp), ("buckets", c_fp), ("radius", C.c_int32),
+                   ("num_buckets", C.c_int32)]
+                + [f for n in ("dout", "dq", "dk", "dv") for f in ((n, c_fp), (n + "_sb", C.c_int64), (n + "_ss", C.c_int64), (n + "_sh", C.c_int64))]
+                + [("dtable", c_fp)])
+
+
+class GatedArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("act", C.c_int32), ("M", C.c_int32), ("F", C.c_int32), ("K", C.c_int32),
+                ("x", c_fp), ("ldx", C.c_int64), ("w", c_fp), ("ldw", C.c_int64), ("b", c_fp), ("h", c_fp), ("ldh", C.c_int64),
+                ("z", c_fp), ("ldz", C.c_int64), ("dh", c_fp), ("ld_dh", C.c_int64), ("dx", c_fp), ("ld_dx", C.c_int64),
+                ("dw", c_fp), ("ld_dw", C.c_int64), ("db", c_fp)]
+
+
+DT_F32, DT_BF16 = 0, 1
+NORM_LAYER, NORM_RMS = 0, 1
 ENC_CNN, ENC_SIMPLE, ENC_EXTERNAL = 0, 1, 2
 FM_CONDITIONAL, FM_TARGET, FM_SCHRODINGER = 0, 1, 2
 LOSS_NAMES = ("loss", "flow_loss", "consistency_loss", "flow_action_recon_loss", "enc_action_recon_loss", "enc_contrastive_loss",
@@ -249,6 +280,17 @@ SIGNATURES = {
     "vita_compute_loss_meanflow_f32": (C.c_int, [C.POINTER(MeanFlowPolicyWeights), C.POINTER(MeanFlowPolicyWeights),
                                                  C.POINTER(MeanFlowLossConfig), c_fp, C.c_int64, c_fp, c_fp, c_fp, c_fp, C.c_int32, c_fp,
                                                  c_fp, C.c_int64, C.POINTER(c_fp), c_fp, C.c_size_t, c_fp]),
+    "vita_qk_norm_rope": (C.c_int, [C.POINTER(NormRopeArgs), c_fp]),
+    "vita_qk_norm_rope_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(NormRopeArgs)]),
+    "vita_qk_norm_rope_bwd": (C.c_int, [C.POINTER(NormRopeArgs), c_fp, C.c_size_t, c_fp]),
+    "vita_attention_workspace_bytes": (C.c_size_t, [C.POINTER(AttentionArgs)]),
+    "vita_attention": (C.c_int, [C.POINTER(AttentionArgs), c_fp, C.c_size_t, c_fp]),
+    "vita_attention_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(AttentionArgs)]),
+    "vita_attention_bwd": (C.c_int, [C.POINTER(AttentionArgs), c_fp, C.c_size_t, c_fp]),
+    "vita_gated_linear_workspace_bytes": (C.c_size_t, [C.POINTER(GatedArgs)]),
+    "vita_gated_linear": (C.c_int, [C.POINTER(GatedArgs), c_fp, C.c_size_t, c_fp]),
+    "vita_gated_linear_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(GatedArgs)]),
+    "vita_gated_linear_bwd": (C.c_int, [C.POINTER(GatedArgs), c_fp, C.c_size_t, c_fp]),
     "vita_normalize_f32": (C.c_int, [c_fp, c_fp, c_fp, c_fp, C.c_int64, C.c_int32, C.c_int64, c_fp]),
     "vita_unnormalize_f32": (C.c_int, [c_fp, c_fp, c_fp, c_fp, C.c_int64, C.c_int32, C.c_int64, c_fp]),
     "vita_layernorm_modulate_f32": (C.c_int, [c_fp, C.c_int64, c_fp, C.c_int64, C.c_int32, C.c_int32, C.c_float, C.c_int32,

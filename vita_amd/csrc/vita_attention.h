@@ -1,0 +1,221 @@
+// Device code shared by the attention kernels (vita_attention_fwd.hip, vita_attention_bwd.hip).
+//
+// One fragment format for both types: a lane of a 32 x 32 MFMA holds 8 elements of its row (A) or column (B) of a 16-deep step, element
+// j of half-wave h standing for depth 8 h + j.  bf16: one v_mfma_f32_32x32x16_bf16; fp32: eight v_mfma_f32_32x32x2_f32, the j-th
+// multiplying element j of both halves.  A and B only have to agree on what depth an element stands for, which is what lets a product's
+// OUTPUT be the next product's B operand without leaving its registers: accumulator register r of half h is row
+// 8 (r / 4) + 4 h + r % 4, so registers 0 .. 7 are a 16-deep B fragment over those rows, and the A fragment is read in the same order.
+// The scores are therefore formed transposed (rows = keys, columns = queries): a lane owns one query, the softmax statistics are
+// per-lane scalars joined by one exchange between the half-waves, and P^T feeds O^T = V^T P^T directly.
+#pragma once
+#include "vita_host.h"
+
+namespace vita {
+
+typedef __bf16 bf16;
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef short attn_s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kInf = __builtin_inff();
+constexpr int kMaxRadius = 1024;
+
+struct AttnTensor { char* p; int64_t sb, ss, sh; };      // strides in elements
+
+struct AttnParams {
+    AttnTensor q, k, v, o, dout, dq, dk, dv;
+    float* lse;                      // (B, H, Sq)
+    float* delta;                    // backward: (B, H, Sq) in the workspace
+    const uint8_t* pad; int64_t ld_pad;
+    const void* table; const int32_t* buckets; int R, NB;
+    int B, H, Hk, G, Sq, Sk, D, causal;
+    float scale, scale_log2;
+    int pack;                        // forward: query heads of one key head that share a row tile (1 or G)
+    int tiles, splits, tiles_per_split;
+    float* part_o; float* part_ml;   // forward, splits > 1
+    float* dist_part;                // backward: (B * q tiles, H, 2 R + 1)
+    int want_dtable;
+};
+
+template <class T> struct Frag;
+template <> struct Frag<float> { float v[8]; };
+template <> struct Frag<bf16> { bf16x8 v; };
+
+__device__ __forceinline__ void mma(f32x16& acc, const Frag<float>& a, const Frag<float>& b) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[j], b.v[j], acc, 0, 0, 0);
+}
+__device__ __forceinline__ void mma(f32x16& acc, const Frag<bf16>& a, const Frag<bf16>& b) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, acc, 0, 0, 0);
+}
+
+__device__ __forceinline__ int acc_row(int r, int half) { return (r >> 2) * 8 + half * 4 + (r & 3); }
+
+// elements of a tile's row in LDS: padded so that the 16-byte reads of 16 consecutive rows meet 16 different bank groups
+template <class T, int DP> constexpr int lds_stride() { return DP + 16 / (int)sizeof(T); }
+
+template <class T>
+__device__ __forceinline__ Frag<T> load8(const T* p) {      // 16-byte aligned
+    Frag<T> f;
+    if constexpr (sizeof(T) == 2) {
+        f.v = *reinterpret_cast<const bf16x8*>(p);
+    } else {
+        const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { f.v[j] = a[j]; f.v[4 + j] = b[j]; }
+    }
+    return f;
+}
+template <class T>
+__device__ __forceinline__ Frag<T> zero8() {
+    Frag<T> f;
+    if constexpr (sizeof(T) == 2) f.v = bf16x8{};
+    else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f.v[j] = 0.f;
+    }
+    return f;
+}
+
+// fragment whose depth is the transpose of the tile: row = column col0 + lane % 32 of the tile, depth = the tile's rows row0 ..
+// row0 + 15 in accumulator order.  bf16: the hardware's transposed read (a group of 16 lanes gives 4 rows x 16 columns, lane i
+// getting column i); fp32: 8 reads of 32 neighbouring columns.
+template <class T, int KS>
+__device__ __forceinline__ Frag<T> col_frag(const T* tile, int row0, int col0, int lane) {
+    Frag<T> f;
+    if constexpr (sizeof(T) == 2) {
+        const int g = lane >> 4, q = (lane & 15) >> 2, c = lane & 3;
+        const T* a = tile + (row0 + (g >> 1) * 4 + q) * KS + col0 + (g & 1) * 16 + c * 4;
+        typedef __attribute__((address_space(3))) attn_s16x4* lds_ptr;
+        struct { attn_s16x4 lo, hi; } t;
+        t.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)a);
+        t.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(a + 8 * KS));
+        f.v = __builtin_bit_cast(bf16x8, t);
+    } else {
+        const T* a = tile + (row0 + (lane >> 5) * 4) * KS + col0 + (lane & 31);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f.v[j] = a[((j >> 2) * 8 + (j & 3)) * KS];
+    }
+    return f;
+}
+
+template <class T>
+__device__ __forceinline__ Frag<T> pack8(const f32x16& s, int chunk) {
+    Frag<T> f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f.v[j] = (T)s[chunk * 8 + j];
+    return f;
+}
+
+// rows of a tile: global -> registers -> LDS, 16 bytes a thread; rows whose bit is clear and columns from D on become zero
+template <class T, int DP, int ROWS, int NT>
+struct Stage {
+    static constexpr int NV = DP * (int)sizeof(T) / 16, E = 16 / (int)sizeof(T), NLD = ROWS * NV / NT;
+    static_assert(ROWS * NV % NT == 0 && NLD >= 1, "tile and workgroup do not match");
+    uint4 r[NLD];
+    __device__ __forceinline__ void load(const T* base, int64_t stride, uint64_t m0, uint64_t m1, int D, int tid) {
+#pragma unroll
+        for (int j = 0; j < NLD; ++j) {
+            const int i = j * NT + tid, row = i / NV, vec = i - row * NV;
+            const bool in = ((ROWS <= 64 || row < 64 ? m0 >> (row & 63) : m1 >> (row & 63)) & 1) != 0 && vec * E < D;
+            r[j] = in ? *reinterpret_cast<const uint4*>(base + (int64_t)row * stride + vec * E) : make_uint4(0, 0, 0, 0);
+        }
+    }
+    __device__ __forceinline__ void store(T* tile, int tid) const {
+#pragma unroll
+        for (int j = 0; j < NLD; ++j) {
+            const int i = j * NT + tid, row = i / NV, vec = i - row * NV;
+            *reinterpret_cast<uint4*>(tile + row * lds_stride<T, DP>() + vec * E) = r[j];
+        }
+    }
+};
+
+// which keys exist, 64 to a word; a wave holds the words of 4096 keys, one a lane
+struct KeyMask {
+    const uint8_t* pad;      // this batch row's bytes, or null
+    int Sk, base;            // base: first word held
+    uint64_t w;
+    __device__ __forceinline__ void init(const AttnParams& p, int b) {
+        pad = p.pad != nullptr ? p.pad + (int64_t)b * p.ld_pad : nullptr;
+        Sk = p.Sk;
+        base = -(1 << 28);
+    }
+    __device__ __forceinline__ void fill(int first) {
+        base = first;
+        const int64_t k0 = ((int64_t)first + (threadIdx.x & 63)) * 64;
+        const int64_t left = (int64_t)Sk - k0;
+        const int n = left >= 64 ? 64 : (left > 0 ? (int)left : 0);
+        uint64_t m = n == 64 ? ~uint64_t(0) : (uint64_t(1) << n) - 1;
+        if (pad != nullptr) {
+            uint64_t here = 0;
+            if (n == 64) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    uint32_t v;
+                    __builtin_memcpy(&v, pad + k0 + 4 * j, 4);
+                    const uint32_t t = ((((v & 0x7f7f7f7fu) + 0x7f7f7f7fu) | v) & 0x80808080u) >> 7;      // 1 in each byte that is not 0
+                    here |= (uint64_t)((t * 0x01020408u) >> 24 & 15u) << (4 * j);
+                }
+            } else {
+                for (int j = 0; j < n; ++j) here |= (uint64_t)(pad[k0 + j] != 0) << j;
+            }
+            m &= ~here;
+        }
+        w = m;
+    }
+    // word i of the row (uniform i); 0 behind the last key
+    __device__ __forceinline__ uint64_t word(int i) {
+        if (i < base || i >= base + 64) fill(i);
+        const int l = i - base;
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)w, l), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(w >> 32), l);
+        return (uint64_t)hi << 32 | lo;
+    }
+    // bits of the KT keys of tile t
+    template <int KT>
+    __device__ __forceinline__ void tile(int t, uint64_t& m0, uint64_t& m1) {
+        m1 = 0;
+        if constexpr (KT == 32) m0 = (word(t >> 1) >> ((t & 1) * 32)) & 0xffffffffu;
+        else if constexpr (KT == 64) m0 = word(t);
+        else { m0 = word(2 * t); m1 = word(2 * t + 1); }
+    }
+};
+
+// the bias of every distance -R .. R of `heads` heads from `head0`, times log2 e
+template <class T>
+__device__ __forceinline__ void load_bias(const AttnParams& p, float* bias, int head0, int heads, int tid, int nt) {
+    const int n = 2 * p.R + 1;
+    for (int i = tid; i < n * heads; i += nt) {
+        const int g = i / n, id = p.buckets[i - g * n];
+        const bool in = id >= 0 && id < p.NB;
+        const float v = (float)reinterpret_cast<const T*>(p.table)[(int64_t)(in ? id : 0) * p.H + head0 + g];
+        bias[i] = in ? v * kLog2e : __builtin_nanf("");
+    }
+}
+
+// workgroup ids go round the 8 XCDs: give each a contiguous range, so that the workgroups of one (batch row, head) share an L2
+__device__ __forceinline__ int xcd_order(int id, int n) {
+    const int per = n >> 3, rem = n & 7, x = id & 7;
+    return x * per + (x < rem ? x : rem) + (id >> 3);
+}
+
+template <class T> __device__ __forceinline__ const T* at(const AttnTensor& t, int b, int64_t s, int h) {
+    return reinterpret_cast<const T*>(t.p) + b * t.sb + s * t.ss + h * t.sh;
+}
+template <class T> __device__ __forceinline__ T* at_mut(const AttnTensor& t, int b, int64_t s, int h) {
+    return reinterpret_cast<T*>(t.p) + b * t.sb + s * t.ss + h * t.sh;
+}
+// 4 consecutive columns of an output row
+template <class T>
+__device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
+    if constexpr (sizeof(T) == 2) {
+        bf16x4 v = {(bf16)a, (bf16)b, (bf16)c, (bf16)d};
+        *reinterpret_cast<bf16x4*>(p) = v;
+    } else {
+        *reinterpret_cast<f32x4*>(p) = f32x4{a, b, c, d};
+    }
+}
+
+int attention_check(const vita_attention_args* a, bool bwd, const char* who);
+void attention_fill(const vita_attention_args* a, AttnParams& p);
+
+}  // namespace vita

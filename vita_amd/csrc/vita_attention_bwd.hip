@@ -1,0 +1,536 @@
+// Backward pass of the attention with a bucketed relative position bias.  With P from the saved log sum exp and dO the gradient of O:
+//
+//   delta_i = dO_i . O_i,   dP = dO V^T,   dS = P (dP - delta),   dQ = scale dS K,   dK = scale dS^T Q,   dV = P^T dO,
+//   dtable[c, h] = sum over batch rows and pairs (i, j) with bucket c of dS
+//
+// Two kernels, each owning what it sums, so nothing is added by atomics and the bits do not depend on the run:
+//   dq:  a wave owns 32 query rows and walks the keys (scores transposed as in the forward pass; also delta and the bias gradient);
+//   dkv: a wave owns 32 keys and walks the query rows of every query head of its key head (scores untransposed, a lane owns one key).
+// Each forms S and dP again: 7 products of Sq x Sk x D against 5 for one kernel that would have to add dQ or dK, dV across workgroups.
+// In both the second operand of the next product is the score tile's own registers (vita_attention.h), so P and dS never touch LDS.
+//
+// Bias gradient: a tile's dS is summed along its diagonals (one distance each) through 4 KB of LDS a wave, lane t taking diagonal t in
+// row order; tiles wholly outside the radius add to one of two scalars a lane.  A workgroup writes one row of sums by distance, and a
+// second launch adds the rows and gathers distances into buckets, both in index order.
+//
+// bf16 calls round P and dS to bf16 for the products that consume them; delta, statistics and sums are fp32.
+#include "vita_attention.h"
+
+namespace vita {
+namespace {
+
+constexpr int kDiag = 33;                                            // row stride of a wave's score tile in LDS
+__host__ __device__ inline int dist_slots(int R) { return 2 * R + 1 + 124; }      // distances of a tile that touches the radius: -R - 62 .. R + 62
+
+// what a wave's lanes wrote to LDS is read by its other lanes: LDS operations of a wave are served in order, the compiler must keep them so
+__device__ __forceinline__ void wave_lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+template <class T, int DP, int NW, int KT>
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void attention_dq_kernel(AttnParams p) {
+    constexpr int NT = 64 * NW, KS = lds_stride<T, DP>(), NC = DP / 16, ND = DP / 32;
+    constexpr bool AHEAD = NW > 1;      // the next tile is fetched while this one is multiplied; one-wave workgroups mostly have one tile
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    T* kt = reinterpret_cast<T*>(smem);
+    T* vt = kt + KT * KS;
+    float* bias = reinterpret_cast<float*>(vt + KT * KS);
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+    int id = xcd_order(blockIdx.x, gridDim.x);
+    const int qt = p.causal ? p.tiles - 1 - id % p.tiles : id % p.tiles;
+    const int bh = id / p.tiles, h = bh % p.H, b = bh / p.H, kvh = h / p.G;
+
+    const int first_row = (qt * NW + wave) * 32, row = first_row + col;
+    const bool valid = row < p.Sq;
+    const int qi = min(row, p.Sq - 1), qpos = p.Sk - p.Sq + qi;
+    const int pos_lo = p.Sk - p.Sq + min(first_row, p.Sq - 1), pos_hi = p.Sk - p.Sq + min(first_row + 31, p.Sq - 1);
+    const int wg_hi = p.Sk - p.Sq + min((qt + 1) * NW * 32 - 1, p.Sq - 1);
+
+    Frag<T> q[NC], g[NC];
+    float delta = 0.f;
+    {
+        const T* qs = at<T>(p.q, b, qi, h);
+        const T* gs = at<T>(p.dout, b, qi, h);
+        const T* os = at<T>(p.o, b, qi, h);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int d = c * 16 + half * 8;
+            const bool in = valid && d < p.D;
+            q[c] = in ? load8(qs + d) : zero8<T>();
+            g[c] = in ? load8(gs + d) : zero8<T>();
+            const Frag<T> o = in ? load8(os + d) : zero8<T>();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) delta = fmaf((float)g[c].v[j], (float)o.v[j], delta);
+        }
+    }
+    delta += __shfl_xor(delta, 32, 64);
+    const int64_t rec = ((int64_t)b * p.H + h) * p.Sq + qi;
+    if (valid && half == 0) p.delta[rec] = delta;
+    float lse2 = p.lse[rec] * kLog2e;
+    if (!valid || lse2 == -kInf) lse2 = kInf;                         // a row without keys: every probability is 2^-inf
+
+    const bool has_bias = p.table != nullptr, want = p.want_dtable != 0;
+    const int R = p.R, nb = 2 * R + 1;
+    float* diag = bias + (has_bias ? ((nb + 3) & ~3) : 0) + wave * (want ? 32 * kDiag + ((dist_slots(R) + 3) & ~3) : 0);
+    float* dist = diag + 32 * kDiag;
+    float far_lo = 0.f, far_hi = 0.f;
+    if (has_bias) load_bias<T>(p, bias, h, 1, tid, NT);
+    if (want)
+        for (int i = lane; i < dist_slots(R); i += 64) dist[i] = 0.f;
+
+    f32x16 dq[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dq[d][r] = 0.f;
+
+    const int limit = p.causal ? min(p.Sk, wg_hi + 1) : p.Sk;
+    const int t1 = limit > 0 ? (limit + KT - 1) / KT : 0;
+    KeyMask mask;
+    mask.init(p, b);
+    uint64_t m0 = 0, m1 = 0;
+    auto next = [&](int t) {
+        for (; t < t1; ++t) {
+            mask.tile<KT>(t, m0, m1);
+            if (m0 != 0) break;
+        }
+        return t;
+    };
+    Stage<T, DP, KT, NT> sk, sv;
+    const T* kbase = at<T>(p.k, b, 0, kvh);
+    const T* vbase = at<T>(p.v, b, 0, kvh);
+    auto fetch = [&](int t) {
+        sk.load(kbase + (int64_t)t * KT * p.k.ss, p.k.ss, m0, m1, p.D, tid);
+        sv.load(vbase + (int64_t)t * KT * p.v.ss, p.v.ss, m0, m1, p.D, tid);
+    };
+    int t = next(0);
+    if (AHEAD && t < t1) fetch(t);
+    while (t < t1) {
+        const uint64_t c0 = m0;
+        __syncthreads();
+        if (!AHEAD) fetch(t);
+        sk.store(kt, tid);
+        sv.store(vt, tid);
+        __syncthreads();
+        const int tn = next(t + 1);
+        if (AHEAD && tn < t1) fetch(tn);
+#pragma unroll
+        for (int n = 0; n < KT / 32; ++n) {
+            const int key0 = t * KT + n * 32;
+            const uint32_t bits = (uint32_t)(c0 >> (n * 32));
+            if (bits == 0 || first_row >= p.Sq || (p.causal && key0 > pos_hi)) continue;      // (a wave behind the last row has nothing)
+            f32x16 s, dp;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+#pragma unroll
+            for (int c = 0; c < NC; ++c) mma(s, load8(kt + (n * 32 + col) * KS + c * 16 + half * 8), q[c]);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) mma(dp, load8(vt + (n * 32 + col) * KS + c * 16 + half * 8), g[c]);
+            const int dmax = key0 + 31 - pos_lo, dmin = key0 - pos_hi;
+            const bool far = dmax <= -R || dmin >= R;
+            if (has_bias && !far) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int ds = key0 + acc_row(r, half) - qpos;
+                    s[r] = fmaf(s[r], p.scale_log2, bias[max(-R, min(R, ds)) + R]);
+                }
+            } else {
+                const float c = has_bias ? bias[dmax <= -R ? 0 : 2 * R] : 0.f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], p.scale_log2, c);
+            }
+            const bool full = bits == 0xffffffffu && !(p.causal && key0 + 31 > pos_lo);
+            const uint32_t mine = bits >> (half * 4);
+            const int see = p.causal ? qpos - key0 - half * 4 : 1 << 30;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[r] = __builtin_amdgcn_exp2f(s[r] - lse2) * (dp[r] - delta);
+                if (!full) {
+                    const int k = acc_row(r, 0);
+                    s[r] = ((mine >> k) & 1) != 0 && k <= see ? s[r] : 0.f;
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const Frag<T> df = pack8<T>(s, c);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) mma(dq[d], col_frag<T, KS>(kt, n * 32 + c * 16, d * 32, lane), df);
+            }
+            if (want) {
+                if (far) {
+                    float a = 0.f;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) a += s[r];
+                    if (dmax <= -R) far_lo += a;
+                    else far_hi += a;
+                } else {
+                    // rows are queries here: lane t sums the elements (i, i + t - 31)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) diag[col * kDiag + acc_row(r, half)] = valid ? s[r] : 0.f;
+                    wave_lds_order();
+                    float a = 0.f;
+                    const int off = lane - 31;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int j = i + off;
+                        const float v = diag[i * kDiag + (j & 31)];
+                        a += (j & ~31) == 0 ? v : 0.f;
+                    }
+                    wave_lds_order();
+                    if (lane < 63) dist[key0 - (p.Sk - p.Sq + first_row) + off + R + 62] += a;
+                }
+            }
+        }
+        t = tn;
+    }
+    if (valid) {
+        T* dst = at_mut<T>(p.dq, b, qi, h);
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int c = d * 32 + acc_row(r, half);
+                if (c < p.D) store4<T>(dst + c, dq[d][r] * p.scale, dq[d][r + 1] * p.scale, dq[d][r + 2] * p.scale, dq[d][r + 3] * p.scale);
+            }
+    }
+    if (want) {
+        far_lo = wave_sum(valid ? far_lo : 0.f);
+        far_hi = wave_sum(valid ? far_hi : 0.f);
+        wave_lds_order();
+        if (lane == 0) {
+            dist[R + 62 - R] += far_lo;       // distances -R and below, R and above
+            dist[R + 62 + R] += far_hi;
+        }
+        __syncthreads();
+        const int stride = 32 * kDiag + ((dist_slots(R) + 3) & ~3);
+        const float* all = dist - wave * stride;
+        float* out = p.dist_part + ((int64_t)(b * p.tiles + qt) * p.H + h) * nb;
+        for (int i = tid; i < nb; i += NT) {
+            float a = 0.f;
+            for (int w = 0; w < NW; ++w) {
+                const float* s = all + w * stride;
+                a += s[i + 62];
+                if (i == 0)
+                    for (int e = 0; e < 62; ++e) a += s[e];
+                if (i == 2 * R)
+                    for (int e = 2 * R + 63; e < dist_slots(R); ++e) a += s[e];
+            }
+            out[i] = a;
+        }
+    }
+}
+
+template <class T, int DP, int NW, int QT>
+__global__ __launch_bounds__(64 * NW, DP >= 64 ? 1 : 2) void attention_dkv_kernel(AttnParams p) {
+    constexpr int NT = 64 * NW, KS = lds_stride<T, DP>(), NC = DP / 16, ND = DP / 32;
+    constexpr bool AHEAD = NW > 1;      // the next tile is fetched while this one is multiplied; one-wave workgroups mostly have one tile
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    T* qs = reinterpret_cast<T*>(smem);
+    T* gs = qs + QT * KS;
+    float* stat = reinterpret_cast<float*>(gs + QT * KS);            // (2, QT): log sum exp (times log2 e), delta
+    float* bias = stat + 2 * QT;
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+    const int id = xcd_order(blockIdx.x, gridDim.x);
+    const int kt = id % p.tiles, bh = id / p.tiles, kvh = bh % p.Hk, b = bh / p.Hk;
+    const int key0 = (kt * NW + wave) * 32, key = key0 + col;
+    const bool valid = key < p.Sk && (p.pad == nullptr || p.pad[(int64_t)b * p.ld_pad + key] == 0);
+    const int wg_key0 = kt * NW * 32;
+
+    Frag<T> k[NC], v[NC];
+    {
+        const T* ks = at<T>(p.k, b, min(key, p.Sk - 1), kvh);
+        const T* vs = at<T>(p.v, b, min(key, p.Sk - 1), kvh);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int d = c * 16 + half * 8;
+            k[c] = valid && d < p.D ? load8(ks + d) : zero8<T>();
+            v[c] = valid && d < p.D ? load8(vs + d) : zero8<T>();
+        }
+    }
+    f32x16 dk[ND], dv[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) { dk[d][r] = 0.f; dv[d][r] = 0.f; }
+
+    const bool has_bias = p.table != nullptr, alive = __ballot(valid) != 0;
+    const int R = p.R, back = p.Sk - p.Sq;
+    // causal: query i sees the workgroup's first key from i = wg_key0 - back on
+    const int q_first = p.causal ? max(0, wg_key0 - back) / QT : 0, q_tiles = (p.Sq + QT - 1) / QT;
+    const int per = max(0, q_tiles - q_first);
+    const int any = __syncthreads_or(alive);
+    const int total = any ? per * p.G : 0;
+
+    Stage<T, DP, QT, NT> sq, sg;
+    float st_l = 0.f, st_d = 0.f;
+    auto fetch = [&](int i) {
+        const int gi = i / per, h = kvh * p.G + gi, row0 = (q_first + i - gi * per) * QT;
+        const int left = p.Sq - row0;
+        const uint64_t m = left >= 64 ? ~uint64_t(0) : (uint64_t(1) << left) - 1;
+        sq.load(at<T>(p.q, b, row0, h), p.q.ss, m, 0, p.D, tid);
+        sg.load(at<T>(p.dout, b, row0, h), p.dout.ss, m, 0, p.D, tid);
+        if (tid < QT) {
+            const int64_t rec = ((int64_t)b * p.H + h) * p.Sq + row0 + tid;
+            const float l = tid < left ? p.lse[rec] * kLog2e : kInf;
+            st_l = l == -kInf ? kInf : l;
+            st_d = tid < left ? p.delta[rec] : 0.f;
+        }
+    };
+    if (AHEAD && total > 0) fetch(0);
+    int have = -1;
+    for (int i = 0; i < total; ++i) {
+        const int gi = i / per, row0 = (q_first + i - gi * per) * QT;
+        __syncthreads();
+        if (!AHEAD) fetch(i);
+        sq.store(qs, tid);
+        sg.store(gs, tid);
+        if (tid < QT) {
+            stat[tid] = st_l;
+            stat[QT + tid] = st_d;
+        }
+        if (has_bias && gi != have) {
+            load_bias<T>(p, bias, kvh * p.G + gi, 1, tid, NT);
+            have = gi;
+        }
+        __syncthreads();
+        if (AHEAD && i + 1 < total) fetch(i + 1);
+        if (!alive) continue;
+#pragma unroll
+        for (int n = 0; n < QT / 32; ++n) {
+            const int pos0 = back + row0 + n * 32;                     // position of the tile's first query
+            if (row0 + n * 32 >= p.Sq || (p.causal && pos0 + 31 < key0)) continue;
+            f32x16 s, dp;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+#pragma unroll
+            for (int c = 0; c < NC; ++c) mma(s, load8(qs + (n * 32 + col) * KS + c * 16 + half * 8), k[c]);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) mma(dp, load8(gs + (n * 32 + col) * KS + c * 16 + half * 8), v[c]);
+            const int dmax = key0 + 31 - pos0, dmin = key0 - pos0 - 31;
+            if (has_bias && !(dmax <= -R || dmin >= R)) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int ds = key - pos0 - acc_row(r, half);
+                    s[r] = fmaf(s[r], p.scale_log2, bias[max(-R, min(R, ds)) + R]);
+                }
+            } else {
+                const float c = has_bias ? bias[dmax <= -R ? 0 : 2 * R] : 0.f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], p.scale_log2, c);
+            }
+            const bool full = !(p.causal && key0 + 31 > pos0);
+            const int see = p.causal ? key - pos0 - half * 4 : -(1 << 30);       // rows from `see` on see this key
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const f32x4 l4 = *reinterpret_cast<const f32x4*>(stat + n * 32 + acc_row(r, half));
+                const f32x4 d4 = *reinterpret_cast<const f32x4*>(stat + QT + n * 32 + acc_row(r, half));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const bool on = valid && (full || acc_row(r + j, 0) >= see);
+                    const float pr = __builtin_amdgcn_exp2f(s[r + j] - l4[j]);
+                    s[r + j] = on ? pr : 0.f;
+                    dp[r + j] = on ? pr * (dp[r + j] - d4[j]) : 0.f;
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const Frag<T> pf = pack8<T>(s, c), df = pack8<T>(dp, c);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    mma(dv[d], col_frag<T, KS>(gs, n * 32 + c * 16, d * 32, lane), pf);
+                    mma(dk[d], col_frag<T, KS>(qs, n * 32 + c * 16, d * 32, lane), df);
+                }
+            }
+        }
+    }
+    if (key < p.Sk) {
+        T* kd = at_mut<T>(p.dk, b, key, kvh);
+        T* vd = at_mut<T>(p.dv, b, key, kvh);
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int c = d * 32 + acc_row(r, half);
+                if (c < p.D) {
+                    store4<T>(kd + c, dk[d][r] * p.scale, dk[d][r + 1] * p.scale, dk[d][r + 2] * p.scale, dk[d][r + 3] * p.scale);
+                    store4<T>(vd + c, dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]);
+                }
+            }
+    }
+}
+
+// the sums by distance of every (batch row, query tile), added in index order in kSeg segments ...
+constexpr int kSeg = 32;
+__global__ __launch_bounds__(256) void attention_dist_kernel(const float* part, float* seg, int parts, int H, int nb) {
+    const int64_t n = (int64_t)H * nb, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    const int per = (parts + kSeg - 1) / kSeg, s0 = blockIdx.y * per, s1 = min(parts, s0 + per);
+    float a = 0.f;
+    for (int s = s0; s < s1; ++s) a += part[s * n + i];
+    seg[blockIdx.y * n + i] = a;
+}
+// ... then the segments, and distances into buckets in distance order
+template <class T>
+__global__ __launch_bounds__(256) void attention_bucket_kernel(const float* seg, const int32_t* buckets, int segs, int H, int nb, int NB, T* dtable) {
+    extern __shared__ float sum[];                                     // (nb) sums, then (nb) bucket ids
+    int* ids = reinterpret_cast<int*>(sum + nb);
+    const int h = blockIdx.x;
+    for (int i = threadIdx.x; i < nb; i += 256) {
+        float a = 0.f;
+        for (int s = 0; s < segs; ++s) a += seg[((int64_t)s * H + h) * nb + i];
+        sum[i] = a;
+        ids[i] = buckets[i];
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < NB; c += 256) {
+        float a = 0.f;
+        for (int i = 0; i < nb; ++i) a += ids[i] == c ? sum[i] : 0.f;
+        dtable[(int64_t)c * H + h] = (T)a;
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void attention_zero_kernel(T* p, int64_t n) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < n) p[i] = (T)0.f;
+}
+
+// queries or keys are none: every gradient is zero
+template <class T>
+__global__ __launch_bounds__(256) void attention_zero_rows_kernel(AttnTensor t, int S, int H, int D, int64_t n) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    const int d = (int)(i % D);
+    const int64_t r = i / D, tok = r / H;
+    const int h = (int)(r % H), b = (int)(tok / S);
+    at_mut<T>(t, b, tok - (int64_t)b * S, h)[d] = (T)0.f;
+}
+
+struct BPlan { int qw, kw, qtiles, ktiles; };
+BPlan plan(const vita_attention_args* a) {
+    BPlan f{};
+    f.qw = a->Sq <= 32 ? 1 : 4;
+    f.kw = a->Sk <= 32 ? 1 : 4;
+    f.qtiles = (a->Sq + 32 * f.qw - 1) / (32 * f.qw);
+    f.ktiles = (a->Sk + 32 * f.kw - 1) / (32 * f.kw);
+    return f;
+}
+size_t carve(const vita_attention_args* a, void* ws, float** delta, float** part, float** seg) {
+    const BPlan f = plan(a);
+    Carver c(ws);
+    *delta = c.take((size_t)a->B * a->H * a->Sq);
+    *part = *seg = nullptr;
+    if (a->dtable != nullptr) {
+        const size_t n = (size_t)a->H * (2 * a->radius + 1);
+        *part = c.take((size_t)a->B * f.qtiles * n);
+        *seg = c.take(kSeg * n);
+    }
+    return c.off;
+}
+
+template <class T, int DP, int NW, int KT>
+int launch_dq(const AttnParams& p, int64_t blocks, hipStream_t s) {
+    const size_t lds = (size_t)2 * KT * lds_stride<T, DP>() * sizeof(T) + (p.table != nullptr ? (size_t)((2 * p.R + 1 + 3) & ~3) * 4 : 0) +
+                       (p.want_dtable ? (size_t)NW * (32 * kDiag + ((dist_slots(p.R) + 3) & ~3)) * 4 : 0);
+    auto kernel = attention_dq_kernel<T, DP, NW, KT>;
+    VITA_REQUIRE(lds <= 160 * 1024, "vita_attention_bwd: %zu bytes of LDS", lds);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * NW), lds, s, p);
+    VITA_CHECK_HIP(hipGetLastError());
+    return VITA_OK;
+}
+template <class T, int DP, int NW, int QT>
+int launch_dkv(const AttnParams& p, int64_t blocks, hipStream_t s) {
+    const size_t lds = (size_t)2 * QT * lds_stride<T, DP>() * sizeof(T) + 2 * QT * 4 + (p.table != nullptr ? (size_t)(2 * p.R + 1) * 4 : 0);
+    auto kernel = attention_dkv_kernel<T, DP, NW, QT>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * NW), lds, s, p);
+    VITA_CHECK_HIP(hipGetLastError());
+    return VITA_OK;
+}
+template <class T, int DP>
+int launch_dp(const vita_attention_args* a, AttnParams p, const BPlan& f, hipStream_t s) {
+    constexpr int T4 = sizeof(T) == 2 ? 64 : 32;
+    p.tiles = f.qtiles;
+    const int64_t nq = (int64_t)f.qtiles * a->H * a->B, nk = (int64_t)f.ktiles * a->Hk * a->B;
+    if (f.qw == 4) VITA_TRY((launch_dq<T, DP, 4, T4>(p, nq, s)));
+    else VITA_TRY((launch_dq<T, DP, 1, 32>(p, nq, s)));
+    p.tiles = f.ktiles;
+    if (f.kw == 4) return launch_dkv<T, DP, 4, T4>(p, nk, s);
+    return launch_dkv<T, DP, 1, 32>(p, nk, s);
+}
+template <class T>
+int run(const vita_attention_args* a, AttnParams& p, float* seg, hipStream_t s) {
+    const int64_t nt = (int64_t)a->num_buckets * a->H;
+    if (a->Sq == 0 || a->Sk == 0) {
+        auto zero = [&](const AttnTensor& t, int S, int H) -> int {
+            const int64_t n = (int64_t)a->B * S * H * a->D;
+            if (n == 0) return VITA_OK;
+            hipLaunchKernelGGL(attention_zero_rows_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, t, S, H, a->D, n);
+            VITA_CHECK_HIP(hipGetLastError());
+            return VITA_OK;
+        };
+        VITA_TRY(zero(p.dq, a->Sq, a->H));
+        VITA_TRY(zero(p.dk, a->Sk, a->Hk));
+        VITA_TRY(zero(p.dv, a->Sk, a->Hk));
+        if (a->dtable != nullptr) {
+            hipLaunchKernelGGL(attention_zero_kernel<T>, dim3((unsigned)((nt + 255) / 256)), dim3(256), 0, s, (T*)a->dtable, nt);
+            VITA_CHECK_HIP(hipGetLastError());
+        }
+        return VITA_OK;
+    }
+    const BPlan f = plan(a);
+    if (a->D <= 32) VITA_TRY((launch_dp<T, 32>(a, p, f, s)));
+    else if (a->D <= 64) VITA_TRY((launch_dp<T, 64>(a, p, f, s)));
+    else if (a->D <= 96) VITA_TRY((launch_dp<T, 96>(a, p, f, s)));
+    else VITA_TRY((launch_dp<T, 128>(a, p, f, s)));
+    if (a->dtable != nullptr) {
+        const int nb = 2 * a->radius + 1, parts = a->B * f.qtiles;
+        const int64_t n = (int64_t)a->H * nb;
+        const bool two = parts > kSeg;                                 // few parts: the bucket kernel adds them itself
+        if (two) {
+            hipLaunchKernelGGL(attention_dist_kernel, dim3((unsigned)((n + 255) / 256), kSeg), dim3(256), 0, s, p.dist_part, seg, parts, a->H, nb);
+            VITA_CHECK_HIP(hipGetLastError());
+        }
+        hipLaunchKernelGGL(attention_bucket_kernel<T>, dim3((unsigned)a->H), dim3(256), (size_t)nb * 8, s, two ? seg : p.dist_part, a->buckets,
+                           two ? kSeg : parts, a->H, nb, a->num_buckets, (T*)a->dtable);
+        VITA_CHECK_HIP(hipGetLastError());
+    }
+    return VITA_OK;
+}
+
+}  // namespace
+}  // namespace vita
+
+using namespace vita;
+
+extern "C" {
+
+size_t vita_attention_bwd_workspace_bytes(const vita_attention_args* a) {
+    if (a == nullptr || a->B <= 0 || a->Sq <= 0 || a->Sk <= 0 || a->H < 1) return 0;
+    float *d, *p, *s;
+    return carve(a, nullptr, &d, &p, &s);
+}
+
+int vita_attention_bwd(const vita_attention_args* a, void* workspace, size_t workspace_bytes, vita_stream_t stream) {
+    const char* who = "vita_attention_bwd";
+    VITA_TRY(attention_check(a, true, who));
+    if (a->B == 0 && a->dtable == nullptr) return VITA_OK;
+    VITA_REQUIRE(a->B > 0, "%s: an empty batch has no bias gradient to write", who);
+    VITA_TRY(check_ws(workspace, workspace_bytes, vita_attention_bwd_workspace_bytes(a), who));
+    VITA_REQUIRE((int64_t)a->B * a->H * ((a->Sq > a->Sk ? a->Sq : a->Sk) / 32 + 1) < (int64_t(1) << 31), "%s: too many rows", who);
+    AttnParams p{};
+    attention_fill(a, p);
+    auto t = [](const void* q, int64_t b, int64_t s, int64_t h) { return AttnTensor{(char*)const_cast<void*>(q), b, s, h}; };
+    p.dout = t(a->dout, a->dout_sb, a->dout_ss, a->dout_sh); p.dq = t(a->dq, a->dq_sb, a->dq_ss, a->dq_sh);
+    p.dk = t(a->dk, a->dk_sb, a->dk_ss, a->dk_sh); p.dv = t(a->dv, a->dv_sb, a->dv_ss, a->dv_sh);
+    p.want_dtable = a->dtable != nullptr;
+    float* seg = nullptr;
+    if (a->Sq > 0 && a->Sk > 0) carve(a, workspace, &p.delta, &p.dist_part, &seg);
+    return a->dtype == VITA_DT_F32 ? run<float>(a, p, seg, (hipStream_t)stream) : run<bf16>(a, p, seg, (hipStream_t)stream);
+}
+
+}  // extern "C"

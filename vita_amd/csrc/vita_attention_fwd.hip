@@ -1,0 +1,418 @@
+// Softmax attention with a bucketed relative position bias, forward: one pass over the keys with the running maximum and sum of every
+// query row, scores and probabilities never in memory.
+//
+//   s2 = (scale q.k + bias) log2 e;   m' = max(m, max s2);   l' = l 2^(m - m') + sum 2^(s2 - m');   O' = O 2^(m - m') + 2^(s2 - m') V
+//
+// Workgroups: NQ waves of 32 query rows each (long sequences: 4, tiny ones: 1), or one 32-row tile whose keys are dealt to NK = 4
+// waves and joined in LDS at the end (few rows over a long cache: bound by reading k and v, so a tile of 128 keys is in flight while
+// the previous one is multiplied).  With few rows the key axis is also split over workgroups, whose (O, m, l) a second launch joins in
+// split order.  Query heads that share a key head share a row tile there (row = query * G + head), so the cache is read once.
+// Tiles whose keys are all padded, or all ahead of a causal row, are skipped without being read.
+// P is rounded to bf16 for the second product of bf16 calls (the matrix unit's operand type); sums, maxima and O stay fp32.
+#include "vita_attention.h"
+
+namespace vita {
+namespace {
+
+template <class T, int DP, int NQ, int NK, int KW>
+__global__ __launch_bounds__(64 * NQ * NK, sizeof(T) == 4 && DP >= 96 ? 1 : 2) void attention_fwd_kernel(AttnParams p) {
+    constexpr int NT = 64 * NQ * NK, KT = KW * NK, KS = lds_stride<T, DP>(), NC = DP / 16, ND = DP / 32, NS = KW / 32;
+    constexpr bool AHEAD = NQ * NK > 1;      // the next tile is fetched while this one is multiplied; one-wave workgroups mostly have one tile
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    T* kt = reinterpret_cast<T*>(smem);
+    T* vt = kt + KT * KS;
+    float* ml = reinterpret_cast<float*>(vt + KT * KS);        // NK > 1: (NK, 32, 2)
+    float* bias = ml + (NK > 1 ? NK * 64 : 0);
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wq = NK > 1 ? 0 : wave, wk = NK > 1 ? wave : 0;
+
+    int id = xcd_order(blockIdx.x, gridDim.x);
+    const int qt = p.causal ? p.tiles - 1 - id % p.tiles : id % p.tiles;       // the rows with the most keys first
+    id /= p.tiles;
+    const int split = id % p.splits;
+    id /= p.splits;
+    const int groups = p.H / p.pack, hy = id % groups, b = id / groups;
+    const int rows = p.Sq * p.pack, head0 = hy * p.pack, kvh = head0 / p.G;
+
+    const int row = (qt * NQ + wq) * 32 + col;
+    const bool valid = row < rows;
+    const int qi = min(row, rows - 1) / p.pack, g = min(row, rows - 1) - qi * p.pack;
+    const int qpos = p.Sk - p.Sq + qi;
+    // positions of the wave's first and last valid row, and of the workgroup's last
+    const int first_row = (qt * NQ + wq) * 32;
+    const int pos_lo = p.Sk - p.Sq + min(first_row, rows - 1) / p.pack, pos_hi = p.Sk - p.Sq + min(first_row + 31, rows - 1) / p.pack;
+    const int wg_hi = p.Sk - p.Sq + min((qt + 1) * NQ * 32 - 1, rows - 1) / p.pack;
+
+    Frag<T> q[NC];
+    {
+        const T* src = at<T>(p.q, b, qi, head0 + g);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) q[c] = valid && c * 16 + half * 8 < p.D ? load8(src + c * 16 + half * 8) : zero8<T>();
+    }
+    const bool has_bias = p.table != nullptr;
+    const int R = p.R, nb = 2 * R + 1;
+    if (has_bias) load_bias<T>(p, bias, head0, p.pack, tid, NT);
+    const float* my_bias = bias + g * nb;
+
+    f32x16 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+    float m = -kInf, l = 0.f;
+
+    const int limit = p.causal ? min(p.Sk, wg_hi + 1) : p.Sk;                  // keys that some row of the workgroup sees
+    const int ntile = limit > 0 ? (limit + KT - 1) / KT : 0;
+    const int t0 = split * p.tiles_per_split, t1 = min(ntile, t0 + p.tiles_per_split);
+    KeyMask mask;
+    mask.init(p, b);
+    uint64_t m0 = 0, m1 = 0;
+    auto next = [&](int t) {       // the first tile from t on that has a key
+        for (; t < t1; ++t) {
+            mask.tile<KT>(t, m0, m1);
+            if ((m0 | m1) != 0) break;
+        }
+        return t;
+    };
+    Stage<T, DP, KT, NT> sk, sv;
+    const T* kbase = at<T>(p.k, b, 0, kvh);
+    const T* vbase = at<T>(p.v, b, 0, kvh);
+    auto fetch = [&](int t) {
+        sk.load(kbase + (int64_t)t * KT * p.k.ss, p.k.ss, m0, m1, p.D, tid);
+        sv.load(vbase + (int64_t)t * KT * p.v.ss, p.v.ss, m0, m1, p.D, tid);
+    };
+
+    int t = next(t0);
+    if (AHEAD && t < t1) fetch(t);
+    while (t < t1) {
+        const uint64_t c0 = m0, c1 = m1;
+        __syncthreads();           // the previous tile has been read by every wave
+        if (!AHEAD) fetch(t);
+        sk.store(kt, tid);
+        sv.store(vt, tid);
+        __syncthreads();
+        const int tn = next(t + 1);
+        if (AHEAD && tn < t1) fetch(tn);
+
+        const int key0 = t * KT + wk * KW;
+        const uint64_t bits = NK == 1 ? c0 : ((wk * KW < 64 ? c0 : c1) >> (wk * KW & 63)) & (KW == 64 ? ~uint64_t(0) : 0xffffffffu);
+        if (bits != 0 && first_row < rows && !(p.causal && key0 > pos_hi)) {
+            f32x16 s[NS];
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[n][r] = 0.f;
+#pragma unroll
+                for (int c = 0; c < NC; ++c) mma(s[n], load8(kt + (wk * KW + n * 32 + col) * KS + c * 16 + half * 8), q[c]);
+            }
+            const bool full = (KW == 64 ? bits == ~uint64_t(0) : (uint32_t)bits == 0xffffffffu) && !(p.causal && key0 + KW - 1 > pos_lo);
+            if (has_bias) {
+                const int far_lo = key0 + KW - 1 - pos_lo, far_hi = key0 - pos_hi;       // largest and smallest distance of the wave's tile
+                if (far_lo <= -R || far_hi >= R) {
+                    const float c = my_bias[far_lo <= -R ? 0 : 2 * R];
+#pragma unroll
+                    for (int n = 0; n < NS; ++n)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[n][r] = fmaf(s[n][r], p.scale_log2, c);
+                } else {
+#pragma unroll
+                    for (int n = 0; n < NS; ++n)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int dist = key0 + n * 32 + acc_row(r, half) - qpos;
+                            s[n][r] = fmaf(s[n][r], p.scale_log2, my_bias[max(-R, min(R, dist)) + R]);
+                        }
+                }
+            } else {
+#pragma unroll
+                for (int n = 0; n < NS; ++n)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[n][r] *= p.scale_log2;
+            }
+            if (!full) {
+                const uint64_t mine = bits >> (half * 4);
+                const int see = p.causal ? qpos - key0 - half * 4 : 1 << 30;
+#pragma unroll
+                for (int n = 0; n < NS; ++n)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int k = n * 32 + acc_row(r, 0);
+                        s[n][r] = ((mine >> k) & 1) != 0 && k <= see ? s[n][r] : -kInf;
+                    }
+            }
+            float top = m;
+#pragma unroll
+            for (int n = 0; n < NS; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) top = fmaxf(top, s[n][r]);
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float safe = top == -kInf ? 0.f : top;
+            if (__ballot(top > m) != 0) {
+                const float f = __builtin_amdgcn_exp2f(m - safe);
+                l *= f;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[d][r] *= f;
+                m = top;
+            }
+            float sum = 0.f;
+#pragma unroll
+            for (int n = 0; n < NS; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    s[n][r] = __builtin_amdgcn_exp2f(s[n][r] - safe);
+                    sum += s[n][r];
+                }
+            l += sum;
+#pragma unroll
+            for (int n = 0; n < NS; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const Frag<T> pf = pack8<T>(s[n], c);
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) mma(o[d], col_frag<T, KS>(vt, wk * KW + n * 32 + c * 16, d * 32, lane), pf);
+                }
+        }
+        t = tn;
+    }
+    l += __shfl_xor(l, 32, 64);
+
+    const int64_t rec = ((int64_t)b * p.H + head0 + g) * p.Sq + qi, nrec = (int64_t)p.B * p.H * p.Sq;
+    if constexpr (NK == 1) {
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        if (valid) {
+            T* dst = at_mut<T>(p.o, b, qi, head0 + g);
+            float* part = p.splits > 1 ? p.part_o + (split * nrec + rec) * p.D : nullptr;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const int c = d * 32 + acc_row(r, half);
+                    if (c < p.D) {
+                        if (part != nullptr) store4<float>(part + c, o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]);
+                        else store4<T>(dst + c, o[d][r] * inv, o[d][r + 1] * inv, o[d][r + 2] * inv, o[d][r + 3] * inv);
+                    }
+                }
+            if (half == 0) {
+                if (part != nullptr) {
+                    p.part_ml[(split * nrec + rec) * 2] = m;
+                    p.part_ml[(split * nrec + rec) * 2 + 1] = l;
+                } else if (p.lse != nullptr) {
+                    p.lse[rec] = l == 0.f ? -kInf : fmaf(m, kLn2, logf(l));
+                }
+            }
+        }
+    } else {
+        // join the waves: every wave scales its O to the common maximum, the four are added in wave order
+        if (half == 0) {
+            ml[(wk * 32 + col) * 2] = m;
+            ml[(wk * 32 + col) * 2 + 1] = l;
+        }
+        __syncthreads();
+        float top = -kInf, total = 0.f;
+#pragma unroll
+        for (int w = 0; w < NK; ++w) top = fmaxf(top, ml[(w * 32 + col) * 2]);
+        const float safe = top == -kInf ? 0.f : top;
+#pragma unroll
+        for (int w = 0; w < NK; ++w) total = fmaf(ml[(w * 32 + col) * 2 + 1], __builtin_amdgcn_exp2f(ml[(w * 32 + col) * 2] - safe), total);
+        const float f = __builtin_amdgcn_exp2f(m - safe);
+        float* buf = reinterpret_cast<float*>(smem);            // (NK, DP, 32): the tiles' room, which every wave has left
+        static_assert(NK * DP * 32 * 4 <= 2 * KT * KS * (int)sizeof(T), "the join must fit the tiles' room");
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) buf[(wk * DP + d * 32 + acc_row(r, half)) * 32 + col] = o[d][r] * f;
+        __syncthreads();
+        const float scale = p.splits > 1 ? 1.f : (total == 0.f ? 0.f : 1.0f / total);
+        if (valid) {
+            T* dst = at_mut<T>(p.o, b, qi, head0 + g);
+            float* part = p.splits > 1 ? p.part_o + (split * nrec + rec) * p.D : nullptr;
+            for (int c = (wave * 2 + half) * 4; c < p.D; c += NK * 8) {
+                float a[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    a[j] = buf[(c + j) * 32 + col];
+#pragma unroll
+                    for (int w = 1; w < NK; ++w) a[j] += buf[(w * DP + c + j) * 32 + col];
+                    a[j] *= scale;
+                }
+                if (part != nullptr) store4<float>(part + c, a[0], a[1], a[2], a[3]);
+                else store4<T>(dst + c, a[0], a[1], a[2], a[3]);
+            }
+            if (wave == 0 && half == 0) {
+                if (part != nullptr) {
+                    p.part_ml[(split * nrec + rec) * 2] = top;
+                    p.part_ml[(split * nrec + rec) * 2 + 1] = total;
+                } else if (p.lse != nullptr) {
+                    p.lse[rec] = total == 0.f ? -kInf : fmaf(top, kLn2, logf(total));
+                }
+            }
+        }
+    }
+}
+
+// the splits of a row, added in split order; D / 4 lanes a row
+template <class T>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p) {
+    const int per = p.D >> 2;
+    const int64_t nrec = (int64_t)p.B * p.H * p.Sq, i = (int64_t)blockIdx.x * 256 + threadIdx.x, rec = i / per;
+    if (rec >= nrec) return;
+    const int c = (int)(i - rec * per) * 4;
+    float top = -kInf;
+    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.part_ml[(s * nrec + rec) * 2]);
+    const float safe = top == -kInf ? 0.f : top;
+    float total = 0.f;
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < p.splits; ++s) {
+        const float f = __builtin_amdgcn_exp2f(p.part_ml[(s * nrec + rec) * 2] - safe);
+        total = fmaf(p.part_ml[(s * nrec + rec) * 2 + 1], f, total);
+        const f32x4 v = *reinterpret_cast<const f32x4*>(p.part_o + (s * nrec + rec) * p.D + c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) a[j] = fmaf(v[j], f, a[j]);
+    }
+    const float inv = total == 0.f ? 0.f : 1.0f / total;
+    const int64_t bh = rec / p.Sq;
+    const int qi = (int)(rec - bh * p.Sq), b = (int)(bh / p.H), h = (int)(bh - (int64_t)b * p.H);
+    store4<T>(at_mut<T>(p.o, b, qi, h) + c, a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv);
+    if (c == 0 && p.lse != nullptr) p.lse[rec] = total == 0.f ? -kInf : fmaf(top, kLn2, logf(total));
+}
+
+enum { FWD_ROWS4 = 0, FWD_ROWS1 = 1, FWD_KEYS4 = 2 };
+struct Plan { int mode, pack, rows, tiles, splits, tiles_per_split; int64_t blocks; };
+
+Plan plan(const vita_attention_args* a) {
+    Plan f{};
+    const int G = a->H / a->Hk;
+    // few rows of a head over many keys: the key axis is what there is to share out
+    const bool few = (int64_t)a->Sq * G <= 64 && a->Sk > 128;
+    f.mode = few ? FWD_KEYS4 : (a->Sq <= 32 ? FWD_ROWS1 : FWD_ROWS4);
+    f.pack = few ? G : 1;
+    f.rows = a->Sq * f.pack;
+    const int per = f.mode == FWD_ROWS4 ? 128 : 32;
+    f.tiles = (f.rows + per - 1) / per;
+    f.splits = 1;
+    const int64_t base = (int64_t)f.tiles * (a->H / f.pack) * a->B;
+    const int ktiles = (a->Sk + 127) / 128;
+    f.tiles_per_split = 1 << 30;
+    if (few && base < 512 && ktiles > 1) {
+        int64_t want = (768 + base - 1) / base;
+        if (want > ktiles) want = ktiles;
+        f.tiles_per_split = (int)((ktiles + want - 1) / want);
+        f.splits = (ktiles + f.tiles_per_split - 1) / f.tiles_per_split;
+    }
+    f.blocks = base * f.splits;
+    return f;
+}
+
+template <class T, int DP, int NQ, int NK, int KW>
+int launch(const AttnParams& p, int64_t blocks, hipStream_t s) {
+    const size_t lds = (size_t)2 * KW * NK * lds_stride<T, DP>() * sizeof(T) + (NK > 1 ? NK * 64 * 4 : 0) +
+                       (p.table != nullptr ? (size_t)p.pack * (2 * p.R + 1) * 4 : 0);
+    VITA_REQUIRE(lds <= 160 * 1024, "vita_attention: radius %d with %d heads to a key head needs %zu bytes of LDS", p.R, p.pack, lds);
+    auto kernel = attention_fwd_kernel<T, DP, NQ, NK, KW>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * NQ * NK), lds, s, p);
+    VITA_CHECK_HIP(hipGetLastError());
+    return VITA_OK;
+}
+template <class T, int DP>
+int launch_mode(const AttnParams& p, const Plan& f, hipStream_t s) {
+    if (f.mode == FWD_ROWS4) return launch<T, DP, 4, 1, sizeof(T) == 2 ? 64 : 32>(p, f.blocks, s);
+    if (f.mode == FWD_ROWS1) return launch<T, DP, 1, 1, 32>(p, f.blocks, s);
+    return launch<T, DP, 1, 4, 32>(p, f.blocks, s);
+}
+template <class T>
+int launch_type(const AttnParams& p, const Plan& f, hipStream_t s) {
+    if (p.D <= 32) VITA_TRY((launch_mode<T, 32>(p, f, s)));
+    else if (p.D <= 64) VITA_TRY((launch_mode<T, 64>(p, f, s)));
+    else if (p.D <= 96) VITA_TRY((launch_mode<T, 96>(p, f, s)));
+    else VITA_TRY((launch_mode<T, 128>(p, f, s)));
+    if (f.splits > 1) {
+        const int64_t n = (int64_t)p.B * p.H * p.Sq * (p.D / 4);
+        hipLaunchKernelGGL(attention_join_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, p);
+        VITA_CHECK_HIP(hipGetLastError());
+    }
+    return VITA_OK;
+}
+
+}  // namespace
+
+int attention_check(const vita_attention_args* a, bool bwd, const char* who) {
+    VITA_REQUIRE(a != nullptr, "%s: null args", who);
+    VITA_REQUIRE(a->dtype == VITA_DT_F32 || a->dtype == VITA_DT_BF16, "%s: unknown dtype %d", who, a->dtype);
+    VITA_REQUIRE(a->B >= 0 && a->Sq >= 0 && a->Sk >= 0 && a->H >= 1 && a->Hk >= 1, "%s: bad shape B=%d Sq=%d Sk=%d H=%d Hk=%d", who, a->B, a->Sq, a->Sk,
+                 a->H, a->Hk);
+    VITA_REQUIRE(a->H % a->Hk == 0, "%s: %d query heads over %d key heads", who, a->H, a->Hk);
+    VITA_REQUIRE(a->D >= 8 && a->D <= 128 && a->D % 8 == 0, "%s: head dimension %d (a multiple of 8, 8..128)", who, a->D);
+    VITA_REQUIRE(a->Sq <= (1 << 28) && a->Sk <= (1 << 28) && (int64_t)a->Sq * (a->H / a->Hk) <= (1 << 28), "%s: sequence too long", who);
+    VITA_REQUIRE(a->scale == a->scale && a->scale > -kInf && a->scale < kInf, "%s: bad scale", who);
+    const int es = a->dtype == VITA_DT_F32 ? 4 : 2, vec = 16 / es;
+    auto ok = [&](const void* q, int64_t b, int64_t t, int64_t h) {
+        return q != nullptr && (reinterpret_cast<uintptr_t>(q) & 15u) == 0 && b % vec == 0 && t % vec == 0 && h % vec == 0;
+    };
+    VITA_REQUIRE((a->B == 0 || a->Sq == 0 || (ok(a->q, a->q_sb, a->q_ss, a->q_sh) && ok(a->o, a->o_sb, a->o_ss, a->o_sh))) &&
+                     (a->B == 0 || a->Sk == 0 || (ok(a->k, a->k_sb, a->k_ss, a->k_sh) && ok(a->v, a->v_sb, a->v_ss, a->v_sh))),
+                 "%s: q, k, v and o must be non-null, 16-byte aligned, with strides that are multiples of 16 bytes", who);
+    VITA_REQUIRE(a->key_pad == nullptr || a->ld_pad == 0 || a->ld_pad >= a->Sk, "%s: bad ld_pad", who);
+    if (a->table != nullptr) {
+        VITA_REQUIRE(a->buckets != nullptr && a->radius >= 0 && a->radius <= kMaxRadius && a->num_buckets >= 1, "%s: bias with radius %d, %d buckets", who,
+                     a->radius, a->num_buckets);
+        VITA_REQUIRE((reinterpret_cast<uintptr_t>(a->table) & (es - 1)) == 0, "%s: misaligned bias table", who);
+    }
+    if (bwd) {
+        VITA_REQUIRE(a->lse != nullptr && ok(a->dout, a->dout_sb, a->dout_ss, a->dout_sh) && ok(a->dq, a->dq_sb, a->dq_ss, a->dq_sh) &&
+                         ok(a->dk, a->dk_sb, a->dk_ss, a->dk_sh) && ok(a->dv, a->dv_sb, a->dv_ss, a->dv_sh),
+                     "%s: lse, dout, dq, dk and dv must be non-null, 16-byte aligned, with strides that are multiples of 16 bytes", who);
+        VITA_REQUIRE(a->dtable == nullptr || a->table != nullptr, "%s: dtable without a table", who);
+    }
+    return VITA_OK;
+}
+
+void attention_fill(const vita_attention_args* a, AttnParams& p) {
+    auto t = [](const void* q, int64_t b, int64_t s, int64_t h) { return AttnTensor{(char*)const_cast<void*>(q), b, s, h}; };
+    p.q = t(a->q, a->q_sb, a->q_ss, a->q_sh); p.k = t(a->k, a->k_sb, a->k_ss, a->k_sh);
+    p.v = t(a->v, a->v_sb, a->v_ss, a->v_sh); p.o = t(a->o, a->o_sb, a->o_ss, a->o_sh);
+    p.lse = a->lse; p.pad = a->key_pad; p.ld_pad = a->ld_pad;
+    p.table = a->table; p.buckets = a->buckets; p.R = a->table != nullptr ? a->radius : 0; p.NB = a->num_buckets;
+    p.B = a->B; p.H = a->H; p.Hk = a->Hk; p.G = a->H / a->Hk; p.Sq = a->Sq; p.Sk = a->Sk; p.D = a->D; p.causal = a->causal != 0;
+    p.scale = a->scale; p.scale_log2 = a->scale * kLog2e;
+    p.pack = 1; p.splits = 1;
+}
+
+}  // namespace vita
+
+using namespace vita;
+
+extern "C" {
+
+size_t vita_attention_workspace_bytes(const vita_attention_args* a) {
+    if (a == nullptr || a->B <= 0 || a->Sq <= 0 || a->Hk <= 0 || a->H < a->Hk || a->H % a->Hk != 0 || a->Sk < 0) return 0;
+    const Plan f = plan(a);
+    if (f.splits == 1) return 0;
+    Carver c(nullptr);
+    const size_t n = (size_t)f.splits * a->B * a->H * a->Sq;
+    c.take(n * a->D);
+    c.take(n * 2);
+    return c.off;
+}
+
+int vita_attention(const vita_attention_args* a, void* workspace, size_t workspace_bytes, vita_stream_t stream) {
+    const char* who = "vita_attention";
+    VITA_TRY(attention_check(a, false, who));
+    if (a->B == 0 || a->Sq == 0) return VITA_OK;
+    VITA_TRY(check_ws(workspace, workspace_bytes, vita_attention_workspace_bytes(a), who));
+    const Plan f = plan(a);
+    VITA_REQUIRE(f.blocks < (int64_t(1) << 31) && (int64_t)a->B * a->H * a->Sq * (a->D / 4) < (int64_t(1) << 38), "%s: too many rows", who);
+    AttnParams p{};
+    attention_fill(a, p);
+    p.pack = f.pack; p.tiles = f.tiles; p.splits = f.splits; p.tiles_per_split = f.tiles_per_split;
+    if (f.splits > 1) {
+        Carver c(workspace);
+        const size_t n = (size_t)f.splits * a->B * a->H * a->Sq;
+        p.part_o = c.take(n * a->D);
+        p.part_ml = c.take(n * 2);
+    }
+    return a->dtype == VITA_DT_F32 ? launch_type<float>(p, f, (hipStream_t)stream) : launch_type<bf16>(p, f, (hipStream_t)stream);
+}
+
+}  // extern "C"

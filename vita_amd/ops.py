@@ -6,6 +6,7 @@ libvita_hip.so.  Nothing here falls back to torch math.
 from __future__ import annotations
 
 import ctypes as C
+import math
 from typing import Mapping, Optional
 
 import torch
@@ -1366,3 +1367,442 @@ def generate_actions_bf16(obs_b: Tensor, fw: FlowNetHandle, dw: DecoderHandle, b
                                            B, num_steps, ws.data_ptr(), ws.numel(), _stream(obs_features)),
             "vita_generate_actions_bf16")
     return (out, lat) if return_latents else out
+
+
+# --------------------------------------------------------------------------------------
+# operators of the transformer blocks (vita_amd/encoders.py): fp32 or bf16 activations
+# --------------------------------------------------------------------------------------
+_DT = {torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16}
+_NORMS = {"layer": L.NORM_LAYER, "rms": L.NORM_RMS}
+_ACTS = {"relu": L.ACT_RELU, "gelu": L.ACT_GELU_ERF, "gelu_tanh": L.ACT_GELU_TANH, "silu": L.ACT_SILU, "mish": L.ACT_MISH}
+
+
+def _act(t: Tensor, what: str, dim: int, like: Optional[Tensor] = None) -> Tensor:
+    """An activation: on the GPU, fp32 or bf16, of `dim` dimensions; of `like`'s type and device where that is given."""
+    if not t.is_cuda:
+        raise L.VitaHipError(f"{what}: expected a tensor on the GPU, got device {t.device} (vita_amd has no CPU path)")
+    if t.dtype not in _DT:
+        raise L.VitaHipError(f"{what}: expected float32 or bfloat16, got {t.dtype}")
+    if t.dim() != dim:
+        raise L.VitaHipError(f"{what}: expected {dim} dimensions, got shape {tuple(t.shape)}")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise L.VitaHipError(f"{what}: {t.dtype} on {t.device}, expected {like.dtype} on {like.device}")
+    return t
+
+
+def _param(t: Optional[Tensor], what: str, shape: tuple, device) -> Optional[Tensor]:
+    """An optional fp32 parameter of the given shape."""
+    if t is None:
+        return None
+    _f32(t, what)
+    if tuple(t.shape) != shape or t.device != device:
+        raise L.VitaHipError(f"{what}: {tuple(t.shape)} on {t.device}, expected {shape} on {device}")
+    return t.contiguous()
+
+
+def _aligned(t: Tensor) -> bool:
+    """Unit inner stride, and every row on a 16-byte border."""
+    es = t.element_size()
+    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or s * es % 16 == 0 for n, s in zip(t.shape[:-1], t.stride()[:-1]))
+
+
+def _aligned_rows(t: Tensor) -> Tensor:
+    if _aligned(t):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _out(t: Optional[Tensor], what: str, shape, like: Tensor) -> Tensor:
+    """The caller's output tensor, checked, or a new one."""
+    if t is None:
+        return torch.empty(shape, dtype=like.dtype, device=like.device)
+    if tuple(t.shape) != tuple(shape) or t.dtype != like.dtype or t.device != like.device:
+        raise L.VitaHipError(f"{what}: {t.dtype} {tuple(t.shape)} on {t.device}, expected {like.dtype} {tuple(shape)} on {like.device}")
+    if t.numel() and (t.stride(-1) != 1 or any(n > 1 and s < t.shape[-1] for n, s in zip(t.shape[:-1], t.stride()[:-1]))):
+        raise L.VitaHipError(f"{what}: needs contiguous rows that do not overlap, got strides {t.stride()}")
+    return t
+
+
+def _scratch(nbytes: int, device) -> Optional[Tensor]:
+    """Workspace of one call, from torch's allocator: two captured graphs never share it."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+class _On:
+    """Launches go to the tensor's device whatever the current one is."""
+
+    def __init__(self, device):
+        self.guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _set4(a, name: str, t: Tensor) -> None:
+    """Pointer and batch / token / head strides of a (B, S, H, D) tensor; a stride that is never walked is 0."""
+    s = t.stride()
+    n = t.shape
+    setattr(a, name, t.data_ptr())
+    setattr(a, name + "_sb", s[0] if n[0] > 1 else 0)
+    setattr(a, name + "_ss", s[1] if n[1] > 1 else 0)
+    setattr(a, name + "_sh", s[2] if n[2] > 1 else 0)
+
+
+def _norm_rope_args(q, k, rope, q_weight, q_bias, k_weight, k_bias, norm, eps, positions, who):
+    _act(q, f"{who}: q", 4)
+    _act(k, f"{who}: k", 4, q)
+    B, S, H, D = q.shape
+    Hk = k.shape[2]
+    if tuple(k.shape) != (B, S, Hk, D):
+        raise L.VitaHipError(f"{who}: q {tuple(q.shape)} and k {tuple(k.shape)} differ in more than their heads")
+    if norm not in _NORMS:
+        raise L.VitaHipError(f"{who}: norm {norm!r}, expected one of {sorted(_NORMS)}")
+    _f32(rope, f"{who}: rope")
+    if rope.dim() != 3 or rope.shape[2] != 2 or rope.device != q.device or D % 2 or rope.shape[1] not in (D // 2, H * D // 2):
+        raise L.VitaHipError(f"{who}: rope {tuple(rope.shape)} on {rope.device}, expected (positions, {D // 2} or {H * D // 2}, 2) on {q.device}")
+    keep = [rope.contiguous()]
+    a = L.NormRopeArgs()
+    a.dtype, a.norm, a.B, a.S, a.D, a.eps = _DT[q.dtype], _NORMS[norm], B, S, D, float(eps)
+    a.rope, a.rope_rows, a.rope_heads = keep[0].data_ptr(), rope.shape[0], rope.shape[1] // (D // 2)
+    if positions is not None:
+        if positions.dtype != torch.int64 or positions.device != q.device or tuple(positions.shape) not in ((S,), (B, S)):
+            raise L.VitaHipError(f"{who}: positions {positions.dtype} {tuple(positions.shape)} on {positions.device}, expected int64 ({S},) or ({B}, {S}) on {q.device}")
+        p = positions if positions.dim() == 2 else positions[None]
+        if S > 1 and p.stride(1) != 1 or (p.shape[0] > 1 and 0 < p.stride(0) < S):
+            p = p.contiguous()
+        keep.append(p)
+        a.positions, a.ld_positions = p.data_ptr(), (p.stride(0) if p.shape[0] > 1 else 0)
+    for side, name, x, w, b in ((a.q, "q", q, q_weight, q_bias), (a.k, "k", k, k_weight, k_bias)):
+        side.H = x.shape[2]
+        if x.stride(3) != 1:
+            x = x.contiguous()
+            keep.append(x)
+        _set4(side, "x", x)
+        w, b = _param(w, f"{who}: {name}_weight", (D,), q.device), _param(b, f"{who}: {name}_bias", (D,), q.device)
+        keep += [w, b]
+        side.weight, side.bias = w.data_ptr() if w is not None else None, b.data_ptr() if b is not None else None
+    return a, keep
+
+
+def _qk_norm_rope(q, k, rope, q_weight, q_bias, k_weight, k_bias, norm, eps, positions, out):
+    a, keep = _norm_rope_args(q, k, rope, q_weight, q_bias, k_weight, k_bias, norm, eps, positions, "qk_norm_rope")
+    qo, ko = out if out is not None else (None, None)
+    qo, ko = _out(qo, "qk_norm_rope: out[0]", q.shape, q), _out(ko, "qk_norm_rope: out[1]", k.shape, k)
+    _set4(a.q, "y", qo)
+    _set4(a.k, "y", ko)
+    if q.numel():
+        with _On(q.device):
+            L.check(L.load().vita_qk_norm_rope(C.byref(a), _stream(q)), "vita_qk_norm_rope")
+    return qo, ko
+
+
+def qk_norm_rope_bwd(dq: Tensor, dk: Tensor, q: Tensor, k: Tensor, rope: Tensor, *, q_weight: Optional[Tensor] = None, q_bias: Optional[Tensor] = None,
+                     k_weight: Optional[Tensor] = None, k_bias: Optional[Tensor] = None, norm: str = "layer", eps: float = 1e-5,
+                     positions: Optional[Tensor] = None, out=None):
+    """Backward of qk_norm_rope from the gradients of its results: (dq, dk, dq_weight, dq_bias, dk_weight, dk_bias) with respect to its
+    inputs, None for a parameter that was not given.  out: a pair of tensors for the first two (may be the gradients passed in)."""
+    a, keep = _norm_rope_args(q, k, rope, q_weight, q_bias, k_weight, k_bias, norm, eps, positions, "qk_norm_rope_bwd")
+    qo, ko = out if out is not None else (None, None)
+    qo, ko = _out(qo, "qk_norm_rope_bwd: out[0]", q.shape, q), _out(ko, "qk_norm_rope_bwd: out[1]", k.shape, k)
+    grads = [torch.empty_like(p, memory_format=torch.contiguous_format) if p is not None else None for p in (q_weight, q_bias, k_weight, k_bias)]
+    for side, name, d, x, y, w, b in ((a.q, "dq", dq, q, qo, grads[0], grads[1]), (a.k, "dk", dk, k, ko, grads[2], grads[3])):
+        if tuple(d.shape) != tuple(x.shape):
+            raise L.VitaHipError(f"qk_norm_rope_bwd: {name} {tuple(d.shape)}, expected {tuple(x.shape)}")
+        _act(d, f"qk_norm_rope_bwd: {name}", 4, q)
+        if d.stride(3) != 1:
+            d = d.contiguous()
+            keep.append(d)
+        _set4(side, "dy", d)
+        _set4(side, "y", y)
+        side.dweight, side.dbias = w.data_ptr() if w is not None else None, b.data_ptr() if b is not None else None
+    if q.numel() == 0:
+        for t in grads:
+            if t is not None:
+                t.zero_()
+    else:
+        lib = L.load()
+        with _On(q.device):
+            ws = _scratch(lib.vita_qk_norm_rope_bwd_workspace_bytes(C.byref(a)), q.device)
+            L.check(lib.vita_qk_norm_rope_bwd(C.byref(a), ws.data_ptr(), ws.numel(), _stream(q)), "vita_qk_norm_rope_bwd")
+    return (qo, ko, *grads)
+
+
+class _QkNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, rope, q_weight, q_bias, k_weight, k_bias, norm, eps, positions):
+        ctx.save_for_backward(q, k, rope, q_weight, q_bias, k_weight, k_bias, positions)
+        ctx.how = dict(norm=norm, eps=eps)
+        return _qk_norm_rope(q, k, rope, q_weight, q_bias, k_weight, k_bias, norm, eps, positions, None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        q, k, rope, qw, qb, kw, kb, positions = ctx.saved_tensors
+        g = qk_norm_rope_bwd(dq, dk, q, k, rope, q_weight=qw, q_bias=qb, k_weight=kw, k_bias=kb, positions=positions, **ctx.how)
+        return (g[0], g[1], None, *g[2:], None, None, None)
+
+
+def qk_norm_rope(q: Tensor, k: Tensor, rope: Tensor, *, q_weight: Optional[Tensor] = None, q_bias: Optional[Tensor] = None,
+                 k_weight: Optional[Tensor] = None, k_bias: Optional[Tensor] = None, norm: str = "layer", eps: float = 1e-5,
+                 positions: Optional[Tensor] = None, out=None):
+    """rope(norm(q)), rope(norm(k)) (attention.py:50-57) in one launch: a norm over each head ("layer": nn.LayerNorm(head_dim); "rms":
+    root mean square) with fp32 weight and bias, then the rotation of neighbouring pairs (pos_embed.py:103-125).
+    q (B, S, H, D), k (B, S, Hk, D) of any strides with contiguous rows (the halves of a packed projection as they lie), fp32 or bf16,
+    D even and at most 256.  rope (P, D / 2, 2) = (cos, sin) of every position for all heads, or (P, H * D / 2, 2) as
+    RotaryPosEmbed.cache has it (frequencies dealt to the heads in order; then Hk = H).  positions: int64 (S,) or (B, S), by default
+    0 .. S - 1; a position outside the table makes its row NaN.  out: a pair of tensors for the results (may be q and k themselves).
+    Differentiable in q, k and the parameters."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, q_bias, k_weight, k_bias)):
+        if out is not None:
+            raise L.VitaHipError("qk_norm_rope: out= cannot be used where a gradient is wanted")
+        return _QkNormRope.apply(q, k, rope, q_weight, q_bias, k_weight, k_bias, norm, eps, positions)
+    return _qk_norm_rope(q, k, rope, q_weight, q_bias, k_weight, k_bias, norm, eps, positions, out)
+
+
+def relative_buckets(num_buckets: int, max_distance: int, bidirectional: bool = True, device=None) -> Tensor:
+    """Bucket ids of the distances -max_distance .. max_distance (key position - query position) for attention(buckets=...): half the
+    buckets for keys ahead when bidirectional (else keys ahead share bucket 0); of each side's, the first half one distance each, the rest
+    in equal steps of the logarithm up to max_distance, where everything farther ends."""
+    side = num_buckets // 2 if bidirectional else num_buckets
+    exact = side // 2
+    if num_buckets < 4 or (bidirectional and num_buckets % 2) or exact < 1 or max_distance <= exact:
+        raise ValueError(f"relative_buckets: {num_buckets} buckets up to distance {max_distance}")
+    ids = []
+    for d in range(-max_distance, max_distance + 1):
+        n = abs(d) if bidirectional else max(0, -d)
+        if n >= exact:
+            n = min(side - 1, exact + int(math.log(n / exact) / math.log(max_distance / exact) * (side - exact) + 1e-9))
+        ids.append(n + (side if bidirectional and d > 0 else 0))
+    return torch.tensor(ids, dtype=torch.int32, device=device)
+
+
+def _attention_args(q, k, v, scale, causal, key_pad, table, buckets, who):
+    _act(q, f"{who}: q", 4)
+    _act(k, f"{who}: k", 4, q)
+    _act(v, f"{who}: v", 4, q)
+    B, Sq, H, D = q.shape
+    Sk, Hk = k.shape[1], k.shape[2]
+    if tuple(k.shape) != (B, Sk, Hk, D) or k.shape != v.shape or Hk < 1 or H % Hk:
+        raise L.VitaHipError(f"{who}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: expected (B, Sq, H, D) and twice (B, Sk, Hk, D) with Hk dividing H")
+    if D % 8 or not 8 <= D <= 128:
+        raise L.VitaHipError(f"{who}: head dimension {D}, expected a multiple of 8 up to 128")
+    q, k, v = _aligned_rows(q), _aligned_rows(k), _aligned_rows(v)
+    keep = [q, k, v]
+    a = L.AttentionArgs()
+    a.dtype, a.B, a.H, a.Hk, a.Sq, a.Sk, a.D, a.causal = _DT[q.dtype], B, H, Hk, Sq, Sk, D, int(bool(causal))
+    a.scale = float(scale) if scale is not None else D ** -0.5
+    _set4(a, "q", q)
+    _set4(a, "k", k)
+    _set4(a, "v", v)
+    if key_pad is not None:
+        if key_pad.dtype not in (torch.bool, torch.uint8) or tuple(key_pad.shape) != (B, Sk) or key_pad.device != q.device:
+            raise L.VitaHipError(f"{who}: key_pad {key_pad.dtype} {tuple(key_pad.shape)} on {key_pad.device}, expected bool or uint8 ({B}, {Sk}) on {q.device}")
+        if Sk > 1 and key_pad.stride(1) != 1 or (B > 1 and 0 < key_pad.stride(0) < Sk):
+            key_pad = key_pad.contiguous()
+        keep.append(key_pad)
+        a.key_pad, a.ld_pad = key_pad.data_ptr(), (key_pad.stride(0) if B > 1 else 0)
+    if (table is None) != (buckets is None):
+        raise L.VitaHipError(f"{who}: the bias needs both table and buckets")
+    if table is not None:
+        _act(table, f"{who}: table", 2, q)
+        if table.shape[0] < 1 or table.shape[1] != H:
+            raise L.VitaHipError(f"{who}: table {tuple(table.shape)}, expected (buckets, {H})")
+        if buckets.dtype != torch.int32 or buckets.dim() != 1 or buckets.numel() % 2 == 0 or buckets.device != q.device or buckets.numel() > 2049:
+            raise L.VitaHipError(f"{who}: buckets {buckets.dtype} {tuple(buckets.shape)} on {buckets.device}, expected int32, an odd number up to 2049, on {q.device}")
+        table, buckets = table.contiguous(), buckets.contiguous()
+        keep += [table, buckets]
+        a.table, a.buckets, a.radius, a.num_buckets = table.data_ptr(), buckets.data_ptr(), buckets.numel() // 2, table.shape[0]
+    return a, keep
+
+
+def _attention(q, k, v, scale, causal, key_pad, table, buckets, need_lse, out):
+    a, keep = _attention_args(q, k, v, scale, causal, key_pad, table, buckets, "attention")
+    o = _out(out, "attention: out", q.shape, q)
+    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device) if need_lse else None
+    if o.numel():
+        if not _aligned(o):
+            raise L.VitaHipError("attention: out needs 16-byte aligned rows")
+        _set4(a, "o", o)
+        a.lse = lse.data_ptr() if need_lse else None
+        lib = L.load()
+        with _On(q.device):
+            ws = _scratch(lib.vita_attention_workspace_bytes(C.byref(a)), q.device)
+            L.check(lib.vita_attention(C.byref(a), ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, _stream(q)), "vita_attention")
+    return o, lse
+
+
+def attention_bwd(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: Tensor, *, scale: Optional[float] = None, causal: bool = False,
+                  key_pad: Optional[Tensor] = None, table: Optional[Tensor] = None, buckets: Optional[Tensor] = None, need_dtable: bool = True, out=None):
+    """Backward of attention from the gradient of its result, the result and its lse (need_lse=True): (dq, dk, dv, dtable), dtable None
+    without a table.  out: tensors for the first three."""
+    a, keep = _attention_args(q, k, v, scale, causal, key_pad, table, buckets, "attention_bwd")
+    for name, t in (("dout", dout), ("o", o)):
+        _act(t, f"attention_bwd: {name}", 4, q)
+        if t.shape != q.shape:
+            raise L.VitaHipError(f"attention_bwd: {name} {tuple(t.shape)}, expected {tuple(q.shape)}")
+    _f32(lse, "attention_bwd: lse")
+    if tuple(lse.shape) != (q.shape[0], q.shape[2], q.shape[1]) or lse.device != q.device:
+        raise L.VitaHipError(f"attention_bwd: lse {tuple(lse.shape)} on {lse.device}, expected {(q.shape[0], q.shape[2], q.shape[1])} on {q.device}")
+    dout, o, lse = _aligned_rows(dout), _aligned_rows(o), lse.contiguous()
+    dq, dk, dv = out if out is not None else (None, None, None)
+    dq, dk, dv = (_out(t, f"attention_bwd: out[{i}]", x.shape, q) for i, (t, x) in enumerate(((dq, q), (dk, k), (dv, v))))
+    dtable = torch.empty(table.shape, dtype=table.dtype, device=table.device) if table is not None and need_dtable else None
+    if not all(t.numel() == 0 or _aligned(t) for t in (dq, dk, dv)):
+        raise L.VitaHipError("attention_bwd: out needs 16-byte aligned rows")
+    if q.numel() == 0 or k.numel() == 0:
+        for t in (dq, dk, dv, dtable):
+            if t is not None:
+                t.zero_()
+        return dq, dk, dv, dtable
+    for name, t in (("o", o), ("dout", dout), ("dq", dq), ("dk", dk), ("dv", dv)):
+        _set4(a, name, t)
+    a.lse, a.dtable = lse.data_ptr(), dtable.data_ptr() if dtable is not None else None
+    lib = L.load()
+    with _On(q.device):
+        ws = _scratch(lib.vita_attention_bwd_workspace_bytes(C.byref(a)), q.device)
+        L.check(lib.vita_attention_bwd(C.byref(a), ws.data_ptr(), ws.numel(), _stream(q)), "vita_attention_bwd")
+    return dq, dk, dv, dtable
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, table, scale, causal, key_pad, buckets):
+        o, lse = _attention(q, k, v, scale, causal, key_pad, table, buckets, True, None)
+        ctx.save_for_backward(q, k, v, o, lse, key_pad, table, buckets)
+        ctx.how = dict(scale=scale, causal=causal)
+        ctx.mark_non_differentiable(lse)
+        return o, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do, _dlse):
+        q, k, v, o, lse, key_pad, table, buckets = ctx.saved_tensors
+        g = attention_bwd(do, q, k, v, o, lse, key_pad=key_pad, table=table, buckets=buckets, need_dtable=ctx.needs_input_grad[3], **ctx.how)
+        return (*g, None, None, None, None)
+
+
+def attention(q: Tensor, k: Tensor, v: Tensor, *, scale: Optional[float] = None, causal: bool = False, key_pad: Optional[Tensor] = None,
+              table: Optional[Tensor] = None, buckets: Optional[Tensor] = None, need_lse: bool = False, out: Optional[Tensor] = None):
+    """Softmax attention (attention.py:58) with an optional learned relative position bias, scores never in memory.
+    q (B, Sq, H, D), k and v (B, Sk, Hk, D), fp32 or bf16, D a multiple of 8 up to 128, head h reading key head h // (H // Hk); rows that
+    are not 16-byte aligned are copied first.  The queries are the last Sq of the Sk positions (Sq = 1: one new token over a cache).
+    scale: D ** -0.5 by default.  causal: query i sees keys up to i + Sk - Sq.  key_pad (B, Sk) bool: True where a key does not exist
+    (the dataset's `*_is_pad`); a query without any key gives zeros.  table (buckets, H) of q's type with buckets = int32
+    (2 R + 1,), the bucket of each distance -R .. R (relative_buckets): adds table[bucket of (key - query position), h] to the scores.
+    need_lse: also the log sum exp of every row, (B, H, Sq) fp32.  out: the result's tensor.  Differentiable in q, k, v and table."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, table)):
+        if out is not None:
+            raise L.VitaHipError("attention: out= cannot be used where a gradient is wanted")
+        o, lse = _Attention.apply(q, k, v, table, scale, causal, key_pad, buckets)
+        return (o, lse) if need_lse else o
+    o, lse = _attention(q, k, v, scale, causal, key_pad, table, buckets, need_lse, out)
+    return (o, lse) if need_lse else o
+
+
+def _gated_args(x, w, b, act, who):
+    _act(x, f"{who}: x", 2)
+    _act(w, f"{who}: w", 2, x)
+    M, K = x.shape
+    if w.shape[1] != K or w.shape[0] % 2:
+        raise L.VitaHipError(f"{who}: x {tuple(x.shape)}, w {tuple(w.shape)}: expected (M, K) and (2 F, K)")
+    F = w.shape[0] // 2
+    if K % 8 or F % 8 or K < 8 or F < 8:
+        raise L.VitaHipError(f"{who}: K = {K} and F = {F} must be multiples of 8")
+    if act not in _ACTS:
+        raise L.VitaHipError(f"{who}: activation {act!r}, expected one of {sorted(_ACTS)}")
+    b = _param(b, f"{who}: b", (2 * F,), x.device)
+    x, w = _gated_rows(x), _gated_rows(w)
+    a = L.GatedArgs()
+    a.dtype, a.act, a.M, a.F, a.K = _DT[x.dtype], _ACTS[act], M, F, K
+    a.x, a.ldx, a.w, a.ldw, a.b = x.data_ptr(), _ld(x), w.data_ptr(), _ld(w), b.data_ptr() if b is not None else None
+    return a, (x, w, b), F
+
+
+def _gated_rows(t: Tensor) -> Tensor:
+    return t if _aligned(t) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]) else t.clone(memory_format=torch.contiguous_format)
+
+
+def _gated_linear(x, w, b, act, need_saved, out):
+    a, keep, F = _gated_args(x, w, b, act, "gated_linear")
+    h = _out(out, "gated_linear: out", (x.shape[0], F), x)
+    # fp32 calls keep the pre-activations; bf16 calls form them again in the backward pass (vita_gated.hip)
+    z = torch.empty((x.shape[0], 2 * F), dtype=torch.float32, device=x.device) if need_saved and x.dtype == torch.float32 else None
+    if h.numel():
+        if not _aligned(h):
+            raise L.VitaHipError("gated_linear: out needs 16-byte aligned rows")
+        a.h, a.ldh = h.data_ptr(), _ld(h)
+        if z is not None:
+            a.z, a.ldz = z.data_ptr(), 2 * F
+        lib = L.load()
+        with _On(x.device):
+            ws = _scratch(lib.vita_gated_linear_workspace_bytes(C.byref(a)), x.device)
+            L.check(lib.vita_gated_linear(C.byref(a), ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, _stream(x)),
+                    "vita_gated_linear")
+    return h, z
+
+
+def gated_linear_bwd(dh: Tensor, x: Tensor, w: Tensor, b: Optional[Tensor], act: str = "silu", saved: Optional[Tensor] = None, *, need_dx: bool = True,
+                     need_dw: bool = True, need_db: bool = True):
+    """Backward of gated_linear from the gradient of its result and what need_saved=True gave: (dx, dw, db), db None without b."""
+    a, keep, F = _gated_args(x, w, b, act, "gated_linear_bwd")
+    M, K = x.shape
+    _act(dh, "gated_linear_bwd: dh", 2, x)
+    if tuple(dh.shape) != (M, F):
+        raise L.VitaHipError(f"gated_linear_bwd: dh {tuple(dh.shape)}, expected {(M, F)}")
+    dh = _gated_rows(dh)
+    dx = torch.empty((M, K), dtype=x.dtype, device=x.device) if need_dx else None
+    dw = torch.empty((2 * F, K), dtype=x.dtype, device=x.device) if need_dw else None
+    db = torch.empty(2 * F, dtype=torch.float32, device=x.device) if need_db and b is not None else None
+    if M == 0:
+        for t in (dw, db):
+            if t is not None:
+                t.zero_()
+        return dx, dw, db
+    if saved is not None:
+        _f32(saved, "gated_linear_bwd: saved")
+        if tuple(saved.shape) != (M, 2 * F) or saved.device != x.device or not saved.is_contiguous():
+            raise L.VitaHipError(f"gated_linear_bwd: saved {tuple(saved.shape)} on {saved.device}, expected contiguous {(M, 2 * F)} on {x.device}")
+        a.z, a.ldz = saved.data_ptr(), 2 * F
+    a.dh, a.ld_dh = dh.data_ptr(), _ld(dh)
+    a.dx, a.ld_dx = (dx.data_ptr() if dx is not None else None), K
+    a.dw, a.ld_dw = (dw.data_ptr() if dw is not None else None), K
+    a.db = db.data_ptr() if db is not None else None
+    lib = L.load()
+    with _On(x.device):
+        ws = _scratch(lib.vita_gated_linear_bwd_workspace_bytes(C.byref(a)), x.device)
+        L.check(lib.vita_gated_linear_bwd(C.byref(a), ws.data_ptr(), ws.numel(), _stream(x)), "vita_gated_linear_bwd")
+    return dx, dw, db
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, b, act):
+        h, z = _gated_linear(x, w, b, act, True, None)
+        ctx.save_for_backward(x, w, b, z)
+        ctx.act = act
+        return h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh):
+        x, w, b, z = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, dw, db = gated_linear_bwd(dh, x, w, b, ctx.act, z, need_dx=need[0], need_dw=need[1], need_db=need[2])
+        return dx, dw, db, None
+
+
+def gated_linear(x: Tensor, w: Tensor, b: Optional[Tensor] = None, act: str = "silu", *, need_saved: bool = False, out: Optional[Tensor] = None):
+    """act(x @ w[:F].T + b[:F]) * (x @ w[F:].T + b[F:]): both projections of a gated feed-forward block, the activation and the product.
+    x (M, K), w (2 F, K), fp32 or bf16, K and F multiples of 8; b (2 F) fp32 or None; act: relu, gelu, gelu_tanh, silu or mish.
+    need_saved: also what gated_linear_bwd takes (None where it needs nothing).  out: the result's tensor.  Differentiable in x, w and b."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, b)):
+        if out is not None or need_saved:
+            raise L.VitaHipError("gated_linear: out= and need_saved= cannot be used where a gradient is wanted")
+        return _GatedLinear.apply(x, w, b, act)
+    h, z = _gated_linear(x, w, b, act, need_saved, out)
+    return (h, z) if need_saved else h

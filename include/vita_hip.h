@@ -705,9 +705,11 @@ int vita_qk_norm_rope_bwd(const vita_norm_rope_args* args, void* workspace, size
  *   exist (is_pad of the dataset's batches); whatever its k and v hold is not used.  A query that sees no key gives zeros.
  *   table (num_buckets, H) of the call's dtype, buckets int32 (2 radius + 1), radius <= 1024; table NULL = no bias.  An id outside
  *   [0, num_buckets) makes its scores NaN.
- *   D a multiple of 8, <= 128; tensors and their strides 16-byte aligned.  lse (B, H, Sq) or NULL: log sum exp of each row's scores
- *   (-inf for a query without keys), what the backward pass needs.
- * Backward: dq, dk, dv (written), dtable (num_buckets, H) of the call's dtype (NULL = not wanted), from dout, o and lse; every sum
+ *   D a multiple of 8, <= 128; tensors and their strides 16-byte aligned, token strides below 2^23 elements.  stats (B, H, Sq, 2) or
+ *   NULL: what the backward pass needs of each row, a maximum M of its scores times log2 e and 1 / sum 2^(score log2 e - M), so that
+ *   log sum exp = M ln 2 - ln(second); (0, 0) for a query without keys.  (Two numbers, because their log sum exp would lose the sum
+ *   where a mask of the type's lowest value makes every score of a row huge.)
+ * Backward: dq, dk, dv (written), dtable (num_buckets, H) of the call's dtype (NULL = not wanted), from dout, o and stats; every sum
  * in a fixed order.
  * --------------------------------------------------------------------------------------- */
 typedef struct vita_attention_args {
@@ -717,7 +719,7 @@ typedef struct vita_attention_args {
     const void* k; int64_t k_sb, k_ss, k_sh;
     const void* v; int64_t v_sb, v_ss, v_sh;
     void* o; int64_t o_sb, o_ss, o_sh;            /* backward: read */
-    float* lse;                                   /* backward: read */
+    float* stats;                                 /* backward: read */
     const uint8_t* key_pad; int64_t ld_pad;
     const void* table; const int32_t* buckets; int32_t radius, num_buckets;
     const void* dout; int64_t dout_sb, dout_ss, dout_sh;

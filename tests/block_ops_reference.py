@@ -119,6 +119,8 @@ def attention(q, k, v, scale=None, causal=False, key_pad=None, table=None, bucke
     lse = torch.where(tot == 0, -math.inf, safe + torch.log(torch.where(tot == 0, 1.0, tot)))[..., 0]
     # exponents are formed times log2 e: their argument is off by es and two roundings of its size; a probability relative to its sum
     ea = es.masked_fill(~seen.expand_as(es), 0.0) + 4 * U * torch.where(seen, (s - safe).abs() + safe.abs(), 0.0).nan_to_num(0.0, 0.0, 0.0)
+    # a mask of the type's lowest value: where a row has other keys its probability is exactly 0, else every score is that value exactly
+    ea = torch.where((p == 0) | (safe.abs() > 1e30), 0.0, ea)
     worst = ea.amax(-1, keepdim=True) if Sk else torch.zeros(B, H, Sq, 1, dtype=torch.float64)
     rp = (ea + worst + (Sk + 16) * U) * 1.01
     o = p @ v64

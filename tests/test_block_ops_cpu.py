@@ -60,14 +60,14 @@ def _attention():
         setattr(a, n + "_sb", 64 * 4 * 64)
         setattr(a, n + "_ss", 64 * 4)
         setattr(a, n + "_sh", 64)
-    a.lse = 1 << 20
+    a.stats = 1 << 20
     return a
 
 
 @pytest.mark.parametrize("change,text", [(dict(dtype=2), "dtype"), (dict(H=0), "shape"), (dict(Sq=-1), "shape"), (dict(Hk=3), "4 query heads over 3"),
                                          (dict(D=20), "head dimension 20"), (dict(D=136), "head dimension"), (dict(D=0), "head dimension"),
                                          (dict(q=None), "non-null"), (dict(v=8 + (1 << 20)), "aligned"), (dict(k_ss=60), "strides"),
-                                         (dict(o_sh=4), "strides"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
+                                         (dict(o_sh=4), "strides"), (dict(k_ss=1 << 23), "2\\^23"), (dict(q_ss=-64), "2\\^23"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
                                          (dict(key_pad=1 << 20, ld_pad=49), "ld_pad"), (dict(table=1 << 20, buckets=None), "bias"),
                                          (dict(table=1 << 20, buckets=1 << 20, radius=1025, num_buckets=4), "radius 1025"),
                                          (dict(table=1 << 20, buckets=1 << 20, radius=-1, num_buckets=4), "radius"),
@@ -85,7 +85,7 @@ def test_attention_refuses(change, text):
 
 def test_attention_bwd_refuses():
     lib = L.load()
-    for change in (dict(lse=None), dict(dout=None), dict(dq_ss=3), dict(dk=None), dict(dv=2 + (1 << 20)), dict(dtable=1 << 20)):
+    for change in (dict(stats=None), dict(stats=4 + (1 << 20)), dict(dout=None), dict(dq_ss=3), dict(dk=None), dict(dv=2 + (1 << 20)), dict(dtable=1 << 20)):
         a = _attention()
         for n, v in change.items():
             setattr(a, n, v)

@@ -142,12 +142,20 @@ def _attention_case(g, B, Sq, Sk, H, Hk, D, dtype, pad, R, nb=16):
     return q, k, v, kw
 
 
+def _lse(stats):
+    """log sum exp in 64 bits from the row statistics: m ln 2 - ln r, -inf for a row without keys."""
+    m, r = stats.double().cpu().unbind(-1)
+    return torch.where(r == 0, -math.inf, m * math.log(2) - torch.log(torch.where(r == 0, 1.0, r)))
+
+
 def _check_attention(q, k, v, kw, g, names=("o", "lse", "dq", "dk", "dv", "dtable")):
-    o, lse = ops.attention(q, k, v, need_lse=True, **kw)
+    o, stats = ops.attention(q, k, v, need_lse=True, **kw)
     do = _randn(g, *q.shape, dtype=q.dtype)
-    got = (o, lse, *ops.attention_bwd(do, q, k, v, o, lse, **kw))
+    got = (o, _lse(stats), *ops.attention_bwd(do, q, k, v, o, stats, **kw))
     want = ref.attention(q, k, v, do=do, **kw)
     for i, n in enumerate(names):
+        if n == "-":
+            continue
         if n == "dtable" and "table" not in kw:
             assert got[i] is None
             continue
@@ -192,7 +200,7 @@ def test_attention_padded_keys_may_hold_anything(dtype):
             o, lse = ops.attention(q, k2, v2, need_lse=True, **kw)
             got = (o, lse, *ops.attention_bwd(do, q, k2, v2, o, lse, **kw))
             assert all(torch.equal(a, b) for a, b in zip(got, want))
-        assert (want[0][1] == 0).all() and torch.isneginf(want[1][1]).all() and all((t[1] == 0).all() for t in want[2:5])
+        assert (want[0][1] == 0).all() and (want[1][1] == 0).all() and all((t[1] == 0).all() for t in want[2:5])
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -221,10 +229,22 @@ def test_attention_large_scores(dtype):
     q, k, v, kw = _attention_case(g, 1, 40, 500, 2, 2, 32, dtype, None, None)
     ramp = torch.linspace(-3, 3, 500, device=DEV)[None, :, None, None]
     for kk in (k * 6, (q.float().mean() + ramp * 4).to(dtype).expand_as(k).contiguous(), (-ramp * 4).to(dtype).expand_as(k).contiguous()):
-        o, lse = ops.attention(q * 4, kk, v, need_lse=True)
-        want = ref.attention(q * 4, kk, v)
-        ref.assert_close(o, want[0], want[1], "o")
-        ref.assert_close(lse, want[2], want[3], "lse")
+        _check_attention(q * 4, kk, v, {}, g)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("low", ["lowest", "-inf"])
+def test_attention_masks_in_the_table(dtype, low):
+    """Buckets that hide their keys: by the type's lowest value (a row with nothing else averages its keys, as the formula does) and by
+    -inf (such a row gives zeros), for whole tiles and inside them."""
+    g = _gen(19)
+    for Sq, Sk, R in ((40, 300, 3), (1, 300, 20), (150, 150, 60), (17, 17, 16)):
+        q, k, v, kw = _attention_case(g, 2, Sq, Sk, 2, 1, 32, dtype, None, R, nb=4)
+        value = torch.finfo(dtype).min if low == "lowest" else -math.inf
+        for hidden in ([1], [0, 1, 2], [0, 1, 2, 3]):
+            table = kw["table"].clone()
+            table[hidden] = value
+            _check_attention(q, k, v, dict(kw, table=table), g, names=("o", "-", "dq", "dk", "dv", "dtable"))
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -258,7 +278,7 @@ def test_attention_no_keys_no_queries(dtype):
     g = _gen(16)
     q, k, v, kw = _attention_case(g, 2, 3, 0, 2, 2, 16, dtype, None, 2)
     o, lse = ops.attention(q, k, v, need_lse=True, **kw)
-    assert (o == 0).all() and torch.isneginf(lse).all()
+    assert (o == 0).all() and (lse == 0).all()
     assert all((t == 0).all() for t in ops.attention_bwd(o, q, k, v, o, lse, **kw))
     o, lse = ops.attention(k, q, q, need_lse=True, **kw)
     assert o.shape == k.shape and lse.numel() == 0

@@ -156,7 +156,7 @@ class NormRopeArgs(C.Structure):
 class AttentionArgs(C.Structure):
     _fields_ = ([(n, C.c_int32) for n in ("dtype", "B", "H", "Hk", "Sq", "Sk", "D", "causal")] + [("scale", C.c_float)]
                 + [f for n in ("q", "k", "v", "o") for f in ((n, c_fp), (n + "_sb", C.c_int64), (n + "_ss", C.c_int64), (n + "_sh", C.c_int64))]
-                + [("lse", c_fp), ("key_pad", c_fp), ("ld_pad", C.c_int64), ("table", c_fp), ("buckets", c_fp), ("radius", C.c_int32),
+                + [("stats", c_fp), ("key_pad", c_fp), ("ld_pad", C.c_int64), ("table", c_fp), ("buckets", c_fp), ("radius", C.c_int32),
                    ("num_buckets", C.c_int32)]
                 + [f for n in ("dout", "dq", "dk", "dv") for f in ((n, c_fp), (n + "_sb", C.c_int64), (n + "_ss", C.c_int64), (n + "_sh", C.c_int64))]
                 + [("dtable", c_fp)])

@@ -16,15 +16,16 @@ typedef __bf16 bf16;
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef short attn_s16x4 __attribute__((ext_vector_type(4)));
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kInf = __builtin_inff();
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kInf = __builtin_inff(), kMaxFloat = 3.402823466e+38f;
+constexpr float kFoldBias = 1e6f;      // a tile's single bias joins the exponent's shift only below this: a larger one has to absorb the score first
 constexpr int kMaxRadius = 1024;
 
 struct AttnTensor { char* p; int64_t sb, ss, sh; };      // strides in elements
 
 struct AttnParams {
     AttnTensor q, k, v, o, dout, dq, dk, dv;
-    float* lse;                      // (B, H, Sq)
+    float2* stats;                   // (B, H, Sq): maximum of a row's scores times log2 e (0: no key), reciprocal of the sum of 2^(score - maximum) (0: no key)
     float* delta;                    // backward: (B, H, Sq) in the workspace
     const uint8_t* pad; int64_t ld_pad;
     const void* table; const int32_t* buckets; int R, NB;
@@ -107,18 +108,41 @@ __device__ __forceinline__ Frag<T> pack8(const f32x16& s, int chunk) {
     return f;
 }
 
-// rows of a tile: global -> registers -> LDS, 16 bytes a thread; rows whose bit is clear and columns from D on become zero
+// rows of a tile: global -> registers -> LDS, 16 bytes a thread.  A thread's place in the tile never changes, so a whole tile is fetched
+// from one uniform base with constant 32-bit offsets: no vector arithmetic (a token stride is below 2^23 elements).  Tiles with missing
+// rows (bit clear) or columns (from D on) take the slow form, which makes those zero.
 template <class T, int DP, int ROWS, int NT>
 struct Stage {
     static constexpr int NV = DP * (int)sizeof(T) / 16, E = 16 / (int)sizeof(T), NLD = ROWS * NV / NT;
+    static constexpr bool REGULAR = NT % NV == 0;                    // every load of a thread is in the same column
     static_assert(ROWS * NV % NT == 0 && NLD >= 1, "tile and workgroup do not match");
     uint4 r[NLD];
-    __device__ __forceinline__ void load(const T* base, int64_t stride, uint64_t m0, uint64_t m1, int D, int tid) {
+    uint32_t off[REGULAR ? 1 : NLD];
+    uint32_t step;                                                   // bytes between a thread's rows (REGULAR)
+    int64_t tile_bytes;
+    __device__ __forceinline__ void init(int64_t stride, int tid) {
+        const uint32_t sb = (uint32_t)(stride * (int64_t)sizeof(T));
 #pragma unroll
-        for (int j = 0; j < NLD; ++j) {
+        for (int j = 0; j < (REGULAR ? 1 : NLD); ++j) {
             const int i = j * NT + tid, row = i / NV, vec = i - row * NV;
-            const bool in = ((ROWS <= 64 || row < 64 ? m0 >> (row & 63) : m1 >> (row & 63)) & 1) != 0 && vec * E < D;
-            r[j] = in ? *reinterpret_cast<const uint4*>(base + (int64_t)row * stride + vec * E) : make_uint4(0, 0, 0, 0);
+            off[j] = (uint32_t)row * sb + (uint32_t)vec * 16;
+        }
+        step = REGULAR ? (uint32_t)(NT / NV) * sb : 0;
+        tile_bytes = (int64_t)ROWS * sb;
+    }
+    __device__ __forceinline__ void load(const T* base, uint64_t m0, uint64_t m1, int D, int tid) {
+        const char* c = reinterpret_cast<const char*>(base);
+        const bool all = ROWS == 32 ? (uint32_t)m0 == 0xffffffffu : (m0 == ~uint64_t(0) && (ROWS <= 64 || m1 == ~uint64_t(0)));
+        if (all && D == DP) {
+#pragma unroll
+            for (int j = 0; j < NLD; ++j) r[j] = *reinterpret_cast<const uint4*>(c + (REGULAR ? (int64_t)(j * step) : 0) + off[REGULAR ? 0 : j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NLD; ++j) {
+                const int i = j * NT + tid, row = i / NV, vec = i - row * NV;
+                const bool in = ((ROWS <= 64 || row < 64 ? m0 >> (row & 63) : m1 >> (row & 63)) & 1) != 0 && vec * E < D;
+                r[j] = in ? *reinterpret_cast<const uint4*>(c + (REGULAR ? (int64_t)(j * step) : 0) + off[REGULAR ? 0 : j]) : make_uint4(0, 0, 0, 0);
+            }
         }
     }
     __device__ __forceinline__ void store(T* tile, int tid) const {
@@ -129,6 +153,14 @@ struct Stage {
         }
     }
 };
+
+// the larger of the two half-waves' values, in both.  (The compiler's builtin for this exchange loses its second result where both
+// operands are one value, so it is written out; the s_nop covers the wait between a vector write and the exchange.)
+__device__ __forceinline__ float max_halves(float v) {
+    float lo = v, hi = v;
+    asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(lo), "+v"(hi));
+    return fmaxf(lo, hi);
+}
 
 // which keys exist, 64 to a word; a wave holds the words of 4096 keys, one a lane
 struct KeyMask {
@@ -188,14 +220,20 @@ __device__ __forceinline__ void load_bias(const AttnParams& p, float* bias, int 
         const int g = i / n, id = p.buckets[i - g * n];
         const bool in = id >= 0 && id < p.NB;
         const float v = (float)reinterpret_cast<const T*>(p.table)[(int64_t)(in ? id : 0) * p.H + head0 + g];
-        bias[i] = in ? v * kLog2e : __builtin_nanf("");
+        // the type's lowest value, used as a mask, stays finite: a row whose every key has it averages them, as the formula does
+        bias[i] = in ? (__builtin_fabsf(v) < kInf ? fmaxf(-kMaxFloat, fminf(kMaxFloat, v * kLog2e)) : v) : __builtin_nanf("");
     }
 }
 
-// workgroup ids go round the 8 XCDs: give each a contiguous range, so that the workgroups of one (batch row, head) share an L2
-__device__ __forceinline__ int xcd_order(int id, int n) {
-    const int per = n >> 3, rem = n & 7, x = id & 7;
-    return x * per + (x < rem ? x : rem) + (id >> 3);
+// Workgroup ids go round the 8 XCDs.  The tiles of one (batch row, head) pair stay on one XCD, whose L2 then holds what they share, and
+// neighbouring pairs are on different ones, so that batch rows of unequal length load all XCDs alike.  The grid is rounded up to whole
+// groups of 8 pairs; false = nothing to do.
+__host__ __device__ inline int64_t pair_grid(int64_t pairs, int tiles) { return (pairs + 7) / 8 * 8 * tiles; }
+__device__ __forceinline__ bool pair_order(int id, int pairs, int tiles, int& pair, int& tile) {
+    const int i = id >> 3;
+    pair = i / tiles * 8 + (id & 7);
+    tile = i % tiles;
+    return pair < pairs;
 }
 
 template <class T> __device__ __forceinline__ const T* at(const AttnTensor& t, int b, int64_t s, int h) {

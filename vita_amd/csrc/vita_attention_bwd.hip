@@ -1,4 +1,4 @@
-// Backward pass of the attention with a bucketed relative position bias.  With P from the saved log sum exp and dO the gradient of O:
+// Backward pass of the attention with a bucketed relative position bias.  With P from the saved row maxima and sums and dO the gradient of O:
 //
 //   delta_i = dO_i . O_i,   dP = dO V^T,   dS = P (dP - delta),   dQ = scale dS K,   dK = scale dS^T Q,   dV = P^T dO,
 //   dtable[c, h] = sum over batch rows and pairs (i, j) with bucket c of dS
@@ -39,9 +39,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void a
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-    int id = xcd_order(blockIdx.x, gridDim.x);
-    const int qt = p.causal ? p.tiles - 1 - id % p.tiles : id % p.tiles;
-    const int bh = id / p.tiles, h = bh % p.H, b = bh / p.H, kvh = h / p.G;
+    int bh, id;
+    if (!pair_order(blockIdx.x, p.B * p.H, p.tiles, bh, id)) return;
+    const int qt = p.causal ? p.tiles - 1 - id : id;
+    const int h = bh % p.H, b = bh / p.H, kvh = h / p.G;
 
     const int first_row = (qt * NW + wave) * 32, row = first_row + col;
     const bool valid = row < p.Sq;
@@ -69,8 +70,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void a
     delta += __shfl_xor(delta, 32, 64);
     const int64_t rec = ((int64_t)b * p.H + h) * p.Sq + qi;
     if (valid && half == 0) p.delta[rec] = delta;
-    float lse2 = p.lse[rec] * kLog2e;
-    if (!valid || lse2 == -kInf) lse2 = kInf;                         // a row without keys: every probability is 2^-inf
+    const float2 st = p.stats[rec];
+    const float top = st.x, inv = valid ? st.y : 0.f, dinv = delta * inv;      // dS = 2^(s - top) (dP inv - delta inv)
 
     const bool has_bias = p.table != nullptr, want = p.want_dtable != 0;
     const int R = p.R, nb = 2 * R + 1;
@@ -100,11 +101,13 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void a
         return t;
     };
     Stage<T, DP, KT, NT> sk, sv;
+    sk.init(p.k.ss, tid);
+    sv.init(p.v.ss, tid);
     const T* kbase = at<T>(p.k, b, 0, kvh);
     const T* vbase = at<T>(p.v, b, 0, kvh);
     auto fetch = [&](int t) {
-        sk.load(kbase + (int64_t)t * KT * p.k.ss, p.k.ss, m0, m1, p.D, tid);
-        sv.load(vbase + (int64_t)t * KT * p.v.ss, p.v.ss, m0, m1, p.D, tid);
+        sk.load(kbase + (int64_t)t * KT * p.k.ss, m0, m1, p.D, tid);
+        sv.load(vbase + (int64_t)t * KT * p.v.ss, m0, m1, p.D, tid);
     };
     int t = next(0);
     if (AHEAD && t < t1) fetch(t);
@@ -130,27 +133,21 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void a
 #pragma unroll
             for (int c = 0; c < NC; ++c) mma(dp, load8(vt + (n * 32 + col) * KS + c * 16 + half * 8), g[c]);
             const int dmax = key0 + 31 - pos_lo, dmin = key0 - pos_hi;
-            const bool far = dmax <= -R || dmin >= R;
-            if (has_bias && !far) {
+            const bool far = dmax <= -R || dmin >= R, full = bits == 0xffffffffu && !(p.causal && key0 + 31 > pos_lo);
+            const float add = has_bias ? bias[dmax <= -R ? 0 : 2 * R] : 0.f;
+            if (full && (!has_bias || (far && __builtin_fabsf(add) < kFoldBias))) {
+                const float shift = add - top;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale_log2, shift)) * fmaf(dp[r], inv, -dinv);
+            } else {
+                const uint32_t mine = bits >> (half * 4);
+                const int see = p.causal ? qpos - key0 - half * 4 : 1 << 30;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int ds = key0 + acc_row(r, half) - qpos;
-                    s[r] = fmaf(s[r], p.scale_log2, bias[max(-R, min(R, ds)) + R]);
-                }
-            } else {
-                const float c = has_bias ? bias[dmax <= -R ? 0 : 2 * R] : 0.f;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], p.scale_log2, c);
-            }
-            const bool full = bits == 0xffffffffu && !(p.causal && key0 + 31 > pos_lo);
-            const uint32_t mine = bits >> (half * 4);
-            const int see = p.causal ? qpos - key0 - half * 4 : 1 << 30;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[r] = __builtin_amdgcn_exp2f(s[r] - lse2) * (dp[r] - delta);
-                if (!full) {
                     const int k = acc_row(r, 0);
-                    s[r] = ((mine >> k) & 1) != 0 && k <= see ? s[r] : 0.f;
+                    const float bv = has_bias ? bias[max(-R, min(R, key0 + half * 4 + k - qpos)) + R] : 0.f;
+                    const float v = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale_log2, bv) - top) * fmaf(dp[r], inv, -dinv);
+                    s[r] = ((mine >> k) & 1) != 0 && k <= see ? v : 0.f;
                 }
             }
 #pragma unroll
@@ -230,13 +227,14 @@ __global__ __launch_bounds__(64 * NW, DP >= 64 ? 1 : 2) void attention_dkv_kerne
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* qs = reinterpret_cast<T*>(smem);
     T* gs = qs + QT * KS;
-    float* stat = reinterpret_cast<float*>(gs + QT * KS);            // (2, QT): log sum exp (times log2 e), delta
-    float* bias = stat + 2 * QT;
+    float* stat = reinterpret_cast<float*>(gs + QT * KS);            // (3, QT): maximum, reciprocal sum, delta of the tile's rows
+    float* bias = stat + 3 * QT;
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-    const int id = xcd_order(blockIdx.x, gridDim.x);
-    const int kt = id % p.tiles, bh = id / p.tiles, kvh = bh % p.Hk, b = bh / p.Hk;
+    int bh, kt;
+    if (!pair_order(blockIdx.x, p.B * p.Hk, p.tiles, bh, kt)) return;
+    const int kvh = bh % p.Hk, b = bh / p.Hk;
     const int key0 = (kt * NW + wave) * 32, key = key0 + col;
     const bool valid = key < p.Sk && (p.pad == nullptr || p.pad[(int64_t)b * p.ld_pad + key] == 0);
     const int wg_key0 = kt * NW * 32;
@@ -258,7 +256,7 @@ __global__ __launch_bounds__(64 * NW, DP >= 64 ? 1 : 2) void attention_dkv_kerne
 #pragma unroll
         for (int r = 0; r < 16; ++r) { dk[d][r] = 0.f; dv[d][r] = 0.f; }
 
-    const bool has_bias = p.table != nullptr, alive = __ballot(valid) != 0;
+    const bool has_bias = p.table != nullptr, alive = __ballot(valid) != 0, whole = __ballot(valid) == ~uint64_t(0);
     const int R = p.R, back = p.Sk - p.Sq;
     // causal: query i sees the workgroup's first key from i = wg_key0 - back on
     const int q_first = p.causal ? max(0, wg_key0 - back) / QT : 0, q_tiles = (p.Sq + QT - 1) / QT;
@@ -267,17 +265,19 @@ __global__ __launch_bounds__(64 * NW, DP >= 64 ? 1 : 2) void attention_dkv_kerne
     const int total = any ? per * p.G : 0;
 
     Stage<T, DP, QT, NT> sq, sg;
-    float st_l = 0.f, st_d = 0.f;
+    sq.init(p.q.ss, tid);
+    sg.init(p.dout.ss, tid);
+    float2 st = make_float2(0.f, 0.f);
+    float st_d = 0.f;
     auto fetch = [&](int i) {
         const int gi = i / per, h = kvh * p.G + gi, row0 = (q_first + i - gi * per) * QT;
         const int left = p.Sq - row0;
         const uint64_t m = left >= 64 ? ~uint64_t(0) : (uint64_t(1) << left) - 1;
-        sq.load(at<T>(p.q, b, row0, h), p.q.ss, m, 0, p.D, tid);
-        sg.load(at<T>(p.dout, b, row0, h), p.dout.ss, m, 0, p.D, tid);
+        sq.load(at<T>(p.q, b, row0, h), m, 0, p.D, tid);
+        sg.load(at<T>(p.dout, b, row0, h), m, 0, p.D, tid);
         if (tid < QT) {
             const int64_t rec = ((int64_t)b * p.H + h) * p.Sq + row0 + tid;
-            const float l = tid < left ? p.lse[rec] * kLog2e : kInf;
-            st_l = l == -kInf ? kInf : l;
+            st = tid < left ? p.stats[rec] : make_float2(0.f, 0.f);
             st_d = tid < left ? p.delta[rec] : 0.f;
         }
     };
@@ -290,8 +290,9 @@ __global__ __launch_bounds__(64 * NW, DP >= 64 ? 1 : 2) void attention_dkv_kerne
         sq.store(qs, tid);
         sg.store(gs, tid);
         if (tid < QT) {
-            stat[tid] = st_l;
-            stat[QT + tid] = st_d;
+            stat[tid] = st.x;
+            stat[QT + tid] = st.y;
+            stat[2 * QT + tid] = st_d;
         }
         if (has_bias && gi != have) {
             load_bias<T>(p, bias, kvh * p.G + gi, 1, tid, NT);
@@ -312,29 +313,35 @@ __global__ __launch_bounds__(64 * NW, DP >= 64 ? 1 : 2) void attention_dkv_kerne
 #pragma unroll
             for (int c = 0; c < NC; ++c) mma(dp, load8(gs + (n * 32 + col) * KS + c * 16 + half * 8), v[c]);
             const int dmax = key0 + 31 - pos0, dmin = key0 - pos0 - 31;
-            if (has_bias && !(dmax <= -R || dmin >= R)) {
+            const bool far = dmax <= -R || dmin >= R;
+            const float add = has_bias ? bias[dmax <= -R ? 0 : 2 * R] : 0.f;
+            if (whole && (!has_bias || (far && __builtin_fabsf(add) < kFoldBias)) && !(p.causal && key0 + 31 > pos0)) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int ds = key - pos0 - acc_row(r, half);
-                    s[r] = fmaf(s[r], p.scale_log2, bias[max(-R, min(R, ds)) + R]);
+                for (int r = 0; r < 16; r += 4) {
+                    const f32x4 m4 = *reinterpret_cast<const f32x4*>(stat + n * 32 + acc_row(r, half));
+                    const f32x4 i4 = *reinterpret_cast<const f32x4*>(stat + QT + n * 32 + acc_row(r, half));
+                    const f32x4 d4 = *reinterpret_cast<const f32x4*>(stat + 2 * QT + n * 32 + acc_row(r, half));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        s[r + j] = __builtin_amdgcn_exp2f(fmaf(s[r + j], p.scale_log2, add - m4[j])) * i4[j];
+                        dp[r + j] = s[r + j] * (dp[r + j] - d4[j]);
+                    }
                 }
             } else {
-                const float c = has_bias ? bias[dmax <= -R ? 0 : 2 * R] : 0.f;
+                const int see = p.causal ? key - pos0 - half * 4 : -(1 << 30);       // rows from `see` on see this key
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], p.scale_log2, c);
-            }
-            const bool full = !(p.causal && key0 + 31 > pos0);
-            const int see = p.causal ? key - pos0 - half * 4 : -(1 << 30);       // rows from `see` on see this key
+                for (int r = 0; r < 16; r += 4) {
+                    const f32x4 m4 = *reinterpret_cast<const f32x4*>(stat + n * 32 + acc_row(r, half));
+                    const f32x4 i4 = *reinterpret_cast<const f32x4*>(stat + QT + n * 32 + acc_row(r, half));
+                    const f32x4 d4 = *reinterpret_cast<const f32x4*>(stat + 2 * QT + n * 32 + acc_row(r, half));
 #pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const f32x4 l4 = *reinterpret_cast<const f32x4*>(stat + n * 32 + acc_row(r, half));
-                const f32x4 d4 = *reinterpret_cast<const f32x4*>(stat + QT + n * 32 + acc_row(r, half));
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const bool on = valid && (full || acc_row(r + j, 0) >= see);
-                    const float pr = __builtin_amdgcn_exp2f(s[r + j] - l4[j]);
-                    s[r + j] = on ? pr : 0.f;
-                    dp[r + j] = on ? pr * (dp[r + j] - d4[j]) : 0.f;
+                    for (int j = 0; j < 4; ++j) {
+                        const float bv = has_bias ? bias[max(-R, min(R, key - pos0 - acc_row(r + j, half))) + R] : 0.f;
+                        const bool on = valid && acc_row(r + j, 0) >= see;
+                        const float pr = __builtin_amdgcn_exp2f(fmaf(s[r + j], p.scale_log2, bv) - m4[j]) * i4[j];
+                        s[r + j] = on ? pr : 0.f;
+                        dp[r + j] = on ? pr * (dp[r + j] - d4[j]) : 0.f;
+                    }
                 }
             }
 #pragma unroll
@@ -445,7 +452,7 @@ int launch_dq(const AttnParams& p, int64_t blocks, hipStream_t s) {
 }
 template <class T, int DP, int NW, int QT>
 int launch_dkv(const AttnParams& p, int64_t blocks, hipStream_t s) {
-    const size_t lds = (size_t)2 * QT * lds_stride<T, DP>() * sizeof(T) + 2 * QT * 4 + (p.table != nullptr ? (size_t)(2 * p.R + 1) * 4 : 0);
+    const size_t lds = (size_t)2 * QT * lds_stride<T, DP>() * sizeof(T) + 3 * QT * 4 + (p.table != nullptr ? (size_t)(2 * p.R + 1) * 4 : 0);
     auto kernel = attention_dkv_kernel<T, DP, NW, QT>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * NW), lds, s, p);
     VITA_CHECK_HIP(hipGetLastError());
@@ -455,12 +462,11 @@ template <class T, int DP>
 int launch_dp(const vita_attention_args* a, AttnParams p, const BPlan& f, hipStream_t s) {
     constexpr int T4 = sizeof(T) == 2 ? 64 : 32;
     p.tiles = f.qtiles;
-    const int64_t nq = (int64_t)f.qtiles * a->H * a->B, nk = (int64_t)f.ktiles * a->Hk * a->B;
-    if (f.qw == 4) VITA_TRY((launch_dq<T, DP, 4, T4>(p, nq, s)));
-    else VITA_TRY((launch_dq<T, DP, 1, 32>(p, nq, s)));
+    if (f.qw == 4) VITA_TRY((launch_dq<T, DP, 4, T4>(p, pair_grid((int64_t)a->H * a->B, f.qtiles), s)));
+    else VITA_TRY((launch_dq<T, DP, 1, 32>(p, pair_grid((int64_t)a->H * a->B, f.qtiles), s)));
     p.tiles = f.ktiles;
-    if (f.kw == 4) return launch_dkv<T, DP, 4, T4>(p, nk, s);
-    return launch_dkv<T, DP, 1, 32>(p, nk, s);
+    if (f.kw == 4) return launch_dkv<T, DP, 4, T4>(p, pair_grid((int64_t)a->Hk * a->B, f.ktiles), s);
+    return launch_dkv<T, DP, 1, 32>(p, pair_grid((int64_t)a->Hk * a->B, f.ktiles), s);
 }
 template <class T>
 int run(const vita_attention_args* a, AttnParams& p, float* seg, hipStream_t s) {
@@ -521,7 +527,7 @@ int vita_attention_bwd(const vita_attention_args* a, void* workspace, size_t wor
     if (a->B == 0 && a->dtable == nullptr) return VITA_OK;
     VITA_REQUIRE(a->B > 0, "%s: an empty batch has no bias gradient to write", who);
     VITA_TRY(check_ws(workspace, workspace_bytes, vita_attention_bwd_workspace_bytes(a), who));
-    VITA_REQUIRE((int64_t)a->B * a->H * ((a->Sq > a->Sk ? a->Sq : a->Sk) / 32 + 1) < (int64_t(1) << 31), "%s: too many rows", who);
+    VITA_REQUIRE(((int64_t)a->B * a->H + 8) * ((a->Sq > a->Sk ? a->Sq : a->Sk) / 32 + 1) < (int64_t(1) << 31), "%s: too many rows", who);
     AttnParams p{};
     attention_fill(a, p);
     auto t = [](const void* q, int64_t b, int64_t s, int64_t h) { return AttnTensor{(char*)const_cast<void*>(q), b, s, h}; };

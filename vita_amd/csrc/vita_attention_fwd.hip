@@ -26,12 +26,11 @@ __global__ __launch_bounds__(64 * NQ * NK, sizeof(T) == 4 && DP >= 96 ? 1 : 2) v
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wq = NK > 1 ? 0 : wave, wk = NK > 1 ? wave : 0;
 
-    int id = xcd_order(blockIdx.x, gridDim.x);
+    const int groups = p.H / p.pack;
+    int pair, id;
+    if (!pair_order(blockIdx.x, p.B * groups, p.tiles * p.splits, pair, id)) return;
     const int qt = p.causal ? p.tiles - 1 - id % p.tiles : id % p.tiles;       // the rows with the most keys first
-    id /= p.tiles;
-    const int split = id % p.splits;
-    id /= p.splits;
-    const int groups = p.H / p.pack, hy = id % groups, b = id / groups;
+    const int split = id / p.tiles, hy = pair % groups, b = pair / groups;
     const int rows = p.Sq * p.pack, head0 = hy * p.pack, kvh = head0 / p.G;
 
     const int row = (qt * NQ + wq) * 32 + col;
@@ -75,11 +74,13 @@ __global__ __launch_bounds__(64 * NQ * NK, sizeof(T) == 4 && DP >= 96 ? 1 : 2) v
         return t;
     };
     Stage<T, DP, KT, NT> sk, sv;
+    sk.init(p.k.ss, tid);
+    sv.init(p.v.ss, tid);
     const T* kbase = at<T>(p.k, b, 0, kvh);
     const T* vbase = at<T>(p.v, b, 0, kvh);
     auto fetch = [&](int t) {
-        sk.load(kbase + (int64_t)t * KT * p.k.ss, p.k.ss, m0, m1, p.D, tid);
-        sv.load(vbase + (int64_t)t * KT * p.v.ss, p.v.ss, m0, m1, p.D, tid);
+        sk.load(kbase + (int64_t)t * KT * p.k.ss, m0, m1, p.D, tid);
+        sv.load(vbase + (int64_t)t * KT * p.v.ss, m0, m1, p.D, tid);
     };
 
     int t = next(t0);
@@ -106,30 +107,16 @@ __global__ __launch_bounds__(64 * NQ * NK, sizeof(T) == 4 && DP >= 96 ? 1 : 2) v
                 for (int c = 0; c < NC; ++c) mma(s[n], load8(kt + (wk * KW + n * 32 + col) * KS + c * 16 + half * 8), q[c]);
             }
             const bool full = (KW == 64 ? bits == ~uint64_t(0) : (uint32_t)bits == 0xffffffffu) && !(p.causal && key0 + KW - 1 > pos_lo);
-            if (has_bias) {
-                const int far_lo = key0 + KW - 1 - pos_lo, far_hi = key0 - pos_hi;       // largest and smallest distance of the wave's tile
-                if (far_lo <= -R || far_hi >= R) {
-                    const float c = my_bias[far_lo <= -R ? 0 : 2 * R];
-#pragma unroll
-                    for (int n = 0; n < NS; ++n)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) s[n][r] = fmaf(s[n][r], p.scale_log2, c);
-                } else {
-#pragma unroll
-                    for (int n = 0; n < NS; ++n)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int dist = key0 + n * 32 + acc_row(r, half) - qpos;
-                            s[n][r] = fmaf(s[n][r], p.scale_log2, my_bias[max(-R, min(R, dist)) + R]);
-                        }
-                }
-            } else {
-#pragma unroll
-                for (int n = 0; n < NS; ++n)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[n][r] *= p.scale_log2;
+            const int far_lo = key0 + KW - 1 - pos_lo, far_hi = key0 - pos_hi;           // largest and smallest distance of the wave's tile
+            // a tile that every row sees whole, its bias one number: the scale goes into the exponent's multiply-add
+            float mul = p.scale_log2, add = 0.f;
+            bool fold = full && p.scale_log2 > 0.f;
+            if (has_bias && fold) {
+                add = my_bias[far_lo <= -R ? 0 : 2 * R];
+                fold = (far_lo <= -R || far_hi >= R) && __ballot(__builtin_fabsf(add) < kFoldBias) == ~uint64_t(0);
+                if (!fold) add = 0.f;
             }
-            if (!full) {
+            if (!fold) {
                 const uint64_t mine = bits >> (half * 4);
                 const int see = p.causal ? qpos - key0 - half * 4 : 1 << 30;
 #pragma unroll
@@ -137,31 +124,36 @@ __global__ __launch_bounds__(64 * NQ * NK, sizeof(T) == 4 && DP >= 96 ? 1 : 2) v
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         const int k = n * 32 + acc_row(r, 0);
-                        s[n][r] = ((mine >> k) & 1) != 0 && k <= see ? s[n][r] : -kInf;
+                        const float bv = has_bias ? my_bias[max(-R, min(R, key0 + half * 4 + k - qpos)) + R] : 0.f;
+                        const float v = fmaf(s[n][r], mul, bv);
+                        s[n][r] = ((mine >> k) & 1) != 0 && k <= see ? v : -kInf;
                     }
+                mul = 1.f;
             }
-            float top = m;
+            float top = s[0][0];
 #pragma unroll
             for (int n = 0; n < NS; ++n)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) top = fmaxf(top, s[n][r]);
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float safe = top == -kInf ? 0.f : top;
-            if (__ballot(top > m) != 0) {
-                const float f = __builtin_amdgcn_exp2f(m - safe);
+            top = fmaf(max_halves(top), mul, add);
+            // the running maximum moves when a score passes it by 2^8: what is summed stays far inside fp32's range, and O is rarely rescaled
+            if (__ballot(top > m + 8.f) != 0) {
+                const float to = fmaxf(top, m);
+                const float f = to == -kInf ? 0.f : __builtin_amdgcn_exp2f(m - to);
                 l *= f;
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) o[d][r] *= f;
-                m = top;
+                m = to;
             }
+            const float shift = add - (m == -kInf ? 0.f : m);
             float sum = 0.f;
 #pragma unroll
             for (int n = 0; n < NS; ++n)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    s[n][r] = __builtin_amdgcn_exp2f(s[n][r] - safe);
+                    s[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], mul, shift));
                     sum += s[n][r];
                 }
             l += sum;
@@ -198,8 +190,8 @@ __global__ __launch_bounds__(64 * NQ * NK, sizeof(T) == 4 && DP >= 96 ? 1 : 2) v
                 if (part != nullptr) {
                     p.part_ml[(split * nrec + rec) * 2] = m;
                     p.part_ml[(split * nrec + rec) * 2 + 1] = l;
-                } else if (p.lse != nullptr) {
-                    p.lse[rec] = l == 0.f ? -kInf : fmaf(m, kLn2, logf(l));
+                } else if (p.stats != nullptr) {
+                    p.stats[rec] = make_float2(m == -kInf ? 0.f : m, inv);
                 }
             }
         }
@@ -244,8 +236,8 @@ __global__ __launch_bounds__(64 * NQ * NK, sizeof(T) == 4 && DP >= 96 ? 1 : 2) v
                 if (part != nullptr) {
                     p.part_ml[(split * nrec + rec) * 2] = top;
                     p.part_ml[(split * nrec + rec) * 2 + 1] = total;
-                } else if (p.lse != nullptr) {
-                    p.lse[rec] = total == 0.f ? -kInf : fmaf(top, kLn2, logf(total));
+                } else if (p.stats != nullptr) {
+                    p.stats[rec] = make_float2(safe, scale);
                 }
             }
         }
@@ -275,7 +267,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p) {
     const int64_t bh = rec / p.Sq;
     const int qi = (int)(rec - bh * p.Sq), b = (int)(bh / p.H), h = (int)(bh - (int64_t)b * p.H);
     store4<T>(at_mut<T>(p.o, b, qi, h) + c, a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv);
-    if (c == 0 && p.lse != nullptr) p.lse[rec] = total == 0.f ? -kInf : fmaf(top, kLn2, logf(total));
+    if (c == 0 && p.stats != nullptr) p.stats[rec] = make_float2(safe, inv);
 }
 
 enum { FWD_ROWS4 = 0, FWD_ROWS1 = 1, FWD_KEYS4 = 2 };
@@ -301,7 +293,7 @@ Plan plan(const vita_attention_args* a) {
         f.tiles_per_split = (int)((ktiles + want - 1) / want);
         f.splits = (ktiles + f.tiles_per_split - 1) / f.tiles_per_split;
     }
-    f.blocks = base * f.splits;
+    f.blocks = pair_grid((int64_t)(a->H / f.pack) * a->B, f.tiles * f.splits);
     return f;
 }
 
@@ -353,6 +345,10 @@ int attention_check(const vita_attention_args* a, bool bwd, const char* who) {
     VITA_REQUIRE((a->B == 0 || a->Sq == 0 || (ok(a->q, a->q_sb, a->q_ss, a->q_sh) && ok(a->o, a->o_sb, a->o_ss, a->o_sh))) &&
                      (a->B == 0 || a->Sk == 0 || (ok(a->k, a->k_sb, a->k_ss, a->k_sh) && ok(a->v, a->v_sb, a->v_ss, a->v_sh))),
                  "%s: q, k, v and o must be non-null, 16-byte aligned, with strides that are multiples of 16 bytes", who);
+    VITA_REQUIRE((int64_t)a->k_ss < (1 << 23) && a->v_ss < (1 << 23) && a->q_ss < (1 << 23) && (!bwd || a->dout_ss < (1 << 23)) && a->k_ss >= 0 && a->v_ss >= 0 &&
+                     a->q_ss >= 0 && (!bwd || a->dout_ss >= 0),
+                 "%s: token strides must be below 2^23 elements", who);
+    VITA_REQUIRE((reinterpret_cast<uintptr_t>(a->stats) & 7u) == 0, "%s: misaligned stats", who);
     VITA_REQUIRE(a->key_pad == nullptr || a->ld_pad == 0 || a->ld_pad >= a->Sk, "%s: bad ld_pad", who);
     if (a->table != nullptr) {
         VITA_REQUIRE(a->buckets != nullptr && a->radius >= 0 && a->radius <= kMaxRadius && a->num_buckets >= 1, "%s: bias with radius %d, %d buckets", who,
@@ -360,9 +356,9 @@ int attention_check(const vita_attention_args* a, bool bwd, const char* who) {
         VITA_REQUIRE((reinterpret_cast<uintptr_t>(a->table) & (es - 1)) == 0, "%s: misaligned bias table", who);
     }
     if (bwd) {
-        VITA_REQUIRE(a->lse != nullptr && ok(a->dout, a->dout_sb, a->dout_ss, a->dout_sh) && ok(a->dq, a->dq_sb, a->dq_ss, a->dq_sh) &&
+        VITA_REQUIRE(a->stats != nullptr && (reinterpret_cast<uintptr_t>(a->stats) & 7u) == 0 && ok(a->dout, a->dout_sb, a->dout_ss, a->dout_sh) && ok(a->dq, a->dq_sb, a->dq_ss, a->dq_sh) &&
                          ok(a->dk, a->dk_sb, a->dk_ss, a->dk_sh) && ok(a->dv, a->dv_sb, a->dv_ss, a->dv_sh),
-                     "%s: lse, dout, dq, dk and dv must be non-null, 16-byte aligned, with strides that are multiples of 16 bytes", who);
+                     "%s: stats, dout, dq, dk and dv must be non-null, 16-byte aligned, with strides that are multiples of 16 bytes", who);
         VITA_REQUIRE(a->dtable == nullptr || a->table != nullptr, "%s: dtable without a table", who);
     }
     return VITA_OK;
@@ -372,7 +368,7 @@ void attention_fill(const vita_attention_args* a, AttnParams& p) {
     auto t = [](const void* q, int64_t b, int64_t s, int64_t h) { return AttnTensor{(char*)const_cast<void*>(q), b, s, h}; };
     p.q = t(a->q, a->q_sb, a->q_ss, a->q_sh); p.k = t(a->k, a->k_sb, a->k_ss, a->k_sh);
     p.v = t(a->v, a->v_sb, a->v_ss, a->v_sh); p.o = t(a->o, a->o_sb, a->o_ss, a->o_sh);
-    p.lse = a->lse; p.pad = a->key_pad; p.ld_pad = a->ld_pad;
+    p.stats = reinterpret_cast<float2*>(a->stats); p.pad = a->key_pad; p.ld_pad = a->ld_pad;
     p.table = a->table; p.buckets = a->buckets; p.R = a->table != nullptr ? a->radius : 0; p.NB = a->num_buckets;
     p.B = a->B; p.H = a->H; p.Hk = a->Hk; p.G = a->H / a->Hk; p.Sq = a->Sq; p.Sk = a->Sk; p.D = a->D; p.causal = a->causal != 0;
     p.scale = a->scale; p.scale_log2 = a->scale * kLog2e;

@@ -1407,7 +1407,7 @@ def _aligned(t: Tensor) -> bool:
 
 
 def _aligned_rows(t: Tensor) -> Tensor:
-    if _aligned(t):
+    if _aligned(t) and (t.shape[1] <= 1 or t.stride(1) < 1 << 23):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -1623,32 +1623,33 @@ def _attention_args(q, k, v, scale, causal, key_pad, table, buckets, who):
 def _attention(q, k, v, scale, causal, key_pad, table, buckets, need_lse, out):
     a, keep = _attention_args(q, k, v, scale, causal, key_pad, table, buckets, "attention")
     o = _out(out, "attention: out", q.shape, q)
-    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device) if need_lse else None
+    stats = torch.empty((q.shape[0], q.shape[2], q.shape[1], 2), dtype=torch.float32, device=q.device) if need_lse else None
     if o.numel():
         if not _aligned(o):
             raise L.VitaHipError("attention: out needs 16-byte aligned rows")
         _set4(a, "o", o)
-        a.lse = lse.data_ptr() if need_lse else None
+        a.stats = stats.data_ptr() if need_lse else None
         lib = L.load()
         with _On(q.device):
             ws = _scratch(lib.vita_attention_workspace_bytes(C.byref(a)), q.device)
             L.check(lib.vita_attention(C.byref(a), ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, _stream(q)), "vita_attention")
-    return o, lse
+    return o, stats
 
 
-def attention_bwd(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: Tensor, *, scale: Optional[float] = None, causal: bool = False,
+def attention_bwd(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, o: Tensor, stats: Tensor, *, scale: Optional[float] = None, causal: bool = False,
                   key_pad: Optional[Tensor] = None, table: Optional[Tensor] = None, buckets: Optional[Tensor] = None, need_dtable: bool = True, out=None):
-    """Backward of attention from the gradient of its result, the result and its lse (need_lse=True): (dq, dk, dv, dtable), dtable None
+    """Backward of attention from the gradient of its result, the result and its row statistics (need_lse=True): (dq, dk, dv, dtable), dtable None
     without a table.  out: tensors for the first three."""
     a, keep = _attention_args(q, k, v, scale, causal, key_pad, table, buckets, "attention_bwd")
     for name, t in (("dout", dout), ("o", o)):
         _act(t, f"attention_bwd: {name}", 4, q)
         if t.shape != q.shape:
             raise L.VitaHipError(f"attention_bwd: {name} {tuple(t.shape)}, expected {tuple(q.shape)}")
-    _f32(lse, "attention_bwd: lse")
-    if tuple(lse.shape) != (q.shape[0], q.shape[2], q.shape[1]) or lse.device != q.device:
-        raise L.VitaHipError(f"attention_bwd: lse {tuple(lse.shape)} on {lse.device}, expected {(q.shape[0], q.shape[2], q.shape[1])} on {q.device}")
-    dout, o, lse = _aligned_rows(dout), _aligned_rows(o), lse.contiguous()
+    _f32(stats, "attention_bwd: stats")
+    rows = (q.shape[0], q.shape[2], q.shape[1], 2)
+    if tuple(stats.shape) != rows or stats.device != q.device:
+        raise L.VitaHipError(f"attention_bwd: stats {tuple(stats.shape)} on {stats.device}, expected {rows} on {q.device}")
+    dout, o, stats = _aligned_rows(dout), _aligned_rows(o), stats.contiguous()
     dq, dk, dv = out if out is not None else (None, None, None)
     dq, dk, dv = (_out(t, f"attention_bwd: out[{i}]", x.shape, q) for i, (t, x) in enumerate(((dq, q), (dk, k), (dv, v))))
     dtable = torch.empty(table.shape, dtype=table.dtype, device=table.device) if table is not None and need_dtable else None
@@ -1661,7 +1662,7 @@ def attention_bwd(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse:
         return dq, dk, dv, dtable
     for name, t in (("o", o), ("dout", dout), ("dq", dq), ("dk", dk), ("dv", dv)):
         _set4(a, name, t)
-    a.lse, a.dtable = lse.data_ptr(), dtable.data_ptr() if dtable is not None else None
+    a.stats, a.dtable = stats.data_ptr(), dtable.data_ptr() if dtable is not None else None
     lib = L.load()
     with _On(q.device):
         ws = _scratch(lib.vita_attention_bwd_workspace_bytes(C.byref(a)), q.device)
@@ -1672,17 +1673,17 @@ def attention_bwd(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse:
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, scale, causal, key_pad, buckets):
-        o, lse = _attention(q, k, v, scale, causal, key_pad, table, buckets, True, None)
-        ctx.save_for_backward(q, k, v, o, lse, key_pad, table, buckets)
+        o, stats = _attention(q, k, v, scale, causal, key_pad, table, buckets, True, None)
+        ctx.save_for_backward(q, k, v, o, stats, key_pad, table, buckets)
         ctx.how = dict(scale=scale, causal=causal)
-        ctx.mark_non_differentiable(lse)
-        return o, lse
+        ctx.mark_non_differentiable(stats)
+        return o, stats
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, do, _dlse):
-        q, k, v, o, lse, key_pad, table, buckets = ctx.saved_tensors
-        g = attention_bwd(do, q, k, v, o, lse, key_pad=key_pad, table=table, buckets=buckets, need_dtable=ctx.needs_input_grad[3], **ctx.how)
+    def backward(ctx, do, _dstats):
+        q, k, v, o, stats, key_pad, table, buckets = ctx.saved_tensors
+        g = attention_bwd(do, q, k, v, o, stats, key_pad=key_pad, table=table, buckets=buckets, need_dtable=ctx.needs_input_grad[3], **ctx.how)
         return (*g, None, None, None, None)
 
 
@@ -1694,14 +1695,15 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, scale: Optional[float] = None,
     scale: D ** -0.5 by default.  causal: query i sees keys up to i + Sk - Sq.  key_pad (B, Sk) bool: True where a key does not exist
     (the dataset's `*_is_pad`); a query without any key gives zeros.  table (buckets, H) of q's type with buckets = int32
     (2 R + 1,), the bucket of each distance -R .. R (relative_buckets): adds table[bucket of (key - query position), h] to the scores.
-    need_lse: also the log sum exp of every row, (B, H, Sq) fp32.  out: the result's tensor.  Differentiable in q, k, v and table."""
+    need_lse: also the row statistics that attention_bwd takes, (B, H, Sq, 2) fp32: a maximum m of the row's scores times log2 e and
+    r = 1 / sum 2 ** (score log2 e - m), so that log sum exp = m ln 2 - ln r; (0, 0) for a query without keys.  out: the result's tensor.  Differentiable in q, k, v and table."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, table)):
         if out is not None:
             raise L.VitaHipError("attention: out= cannot be used where a gradient is wanted")
-        o, lse = _Attention.apply(q, k, v, table, scale, causal, key_pad, buckets)
-        return (o, lse) if need_lse else o
-    o, lse = _attention(q, k, v, scale, causal, key_pad, table, buckets, need_lse, out)
-    return (o, lse) if need_lse else o
+        o, stats = _Attention.apply(q, k, v, table, scale, causal, key_pad, buckets)
+        return (o, stats) if need_lse else o
+    o, stats = _attention(q, k, v, scale, causal, key_pad, table, buckets, need_lse, out)
+    return (o, stats) if need_lse else o
 
 
 def _gated_args(x, w, b, act, who):

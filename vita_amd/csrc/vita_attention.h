@@ -100,6 +100,27 @@ __device__ __forceinline__ Frag<T> col_frag(const T* tile, int row0, int col0, i
     return f;
 }
 
+// Products of one tile in steps, the next step's fragments requested before this step multiplies: a step is long enough to cover the
+// LDS reads (one fp32 fragment feeds 512 cycles of MFMA, one bf16 fragment 32, so a bf16 step takes N of them), and the scheduler may not
+// move reads over a step's border.  a(i, j): the A fragment of column block j at step i;  mul(i, j, a): uses it.
+template <class T, int STEPS, int N, class Read, class Use>
+__device__ __forceinline__ void pipelined(Read read, Use use) {
+    constexpr int W = sizeof(T) == 2 ? N : 1, TOTAL = STEPS * N / W;
+    Frag<T> a[2][W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) a[0][j] = read(0, j);
+#pragma unroll
+    for (int i = 0; i < TOTAL; ++i) {
+        if (i + 1 < TOTAL) {
+#pragma unroll
+            for (int j = 0; j < W; ++j) a[(i + 1) & 1][j] = read((i + 1) * W / N, (i + 1) * W % N + j);
+        }
+#pragma unroll
+        for (int j = 0; j < W; ++j) use(i * W / N, i * W % N + j, a[i & 1][j]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
 template <class T>
 __device__ __forceinline__ Frag<T> pack8(const f32x16& s, int chunk) {
     Frag<T> f;
@@ -226,13 +247,15 @@ __device__ __forceinline__ void load_bias(const AttnParams& p, float* bias, int 
 }
 
 // Workgroup ids go round the 8 XCDs.  The tiles of one (batch row, head) pair stay on one XCD, whose L2 then holds what they share, and
-// neighbouring pairs are on different ones, so that batch rows of unequal length load all XCDs alike.  The grid is rounded up to whole
-// groups of 8 pairs; false = nothing to do.
+// neighbouring pairs are on different ones, so that batch rows of unequal length load all XCDs alike.  Within an XCD pair after pair, or
+// (causal: tiles cost from one to all of the keys) tile after tile, the costliest of every pair first: 32 pairs of 4095 tokens end
+// within 1 % of an even share that way, 47 % over it pair after pair.  The grid is rounded up to whole groups of 8 pairs; false = nothing
+// to do.
 __host__ __device__ inline int64_t pair_grid(int64_t pairs, int tiles) { return (pairs + 7) / 8 * 8 * tiles; }
-__device__ __forceinline__ bool pair_order(int id, int pairs, int tiles, int& pair, int& tile) {
-    const int i = id >> 3;
-    pair = i / tiles * 8 + (id & 7);
-    tile = i % tiles;
+__device__ __forceinline__ bool pair_order(int id, int pairs, int tiles, int by_tile, int& pair, int& tile) {
+    const int i = id >> 3, per = (pairs + 7) >> 3;
+    tile = by_tile ? i / per : i % tiles;
+    pair = (by_tile ? i - tile * per : i / tiles) * 8 + (id & 7);
     return pair < pairs;
 }
 

@@ -40,7 +40,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void a
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
     int bh, id;
-    if (!pair_order(blockIdx.x, p.B * p.H, p.tiles, bh, id)) return;
+    if (!pair_order(blockIdx.x, p.B * p.H, p.tiles, p.causal, bh, id)) return;
     const int qt = p.causal ? p.tiles - 1 - id : id;
     const int h = bh % p.H, b = bh / p.H, kvh = h / p.G;
 
@@ -128,10 +128,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void a
             f32x16 s, dp;
 #pragma unroll
             for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
-#pragma unroll
-            for (int c = 0; c < NC; ++c) mma(s, load8(kt + (n * 32 + col) * KS + c * 16 + half * 8), q[c]);
-#pragma unroll
-            for (int c = 0; c < NC; ++c) mma(dp, load8(vt + (n * 32 + col) * KS + c * 16 + half * 8), g[c]);
+            pipelined<T, NC, 2>([&](int c, int j) { return load8((j == 0 ? kt : vt) + (n * 32 + col) * KS + c * 16 + half * 8); },
+                                [&](int c, int j, const Frag<T>& a) { mma(j == 0 ? s : dp, a, j == 0 ? q[c] : g[c]); });
             const int dmax = key0 + 31 - pos_lo, dmin = key0 - pos_hi;
             const bool far = dmax <= -R || dmin >= R, full = bits == 0xffffffffu && !(p.causal && key0 + 31 > pos_lo);
             const float add = has_bias ? bias[dmax <= -R ? 0 : 2 * R] : 0.f;
@@ -150,11 +148,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void a
                     s[r] = ((mine >> k) & 1) != 0 && k <= see ? v : 0.f;
                 }
             }
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const Frag<T> df = pack8<T>(s, c);
-#pragma unroll
-                for (int d = 0; d < ND; ++d) mma(dq[d], col_frag<T, KS>(kt, n * 32 + c * 16, d * 32, lane), df);
+            {
+                const Frag<T> df[2] = {pack8<T>(s, 0), pack8<T>(s, 1)};
+                pipelined<T, 2, ND>([&](int c, int d) { return col_frag<T, KS>(kt, n * 32 + c * 16, d * 32, lane); },
+                                    [&](int c, int d, const Frag<T>& a) { mma(dq[d], a, df[c]); });
             }
             if (want) {
                 if (far) {
@@ -233,7 +230,7 @@ __global__ __launch_bounds__(64 * NW, DP >= 64 ? 1 : 2) void attention_dkv_kerne
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
     int bh, kt;
-    if (!pair_order(blockIdx.x, p.B * p.Hk, p.tiles, bh, kt)) return;
+    if (!pair_order(blockIdx.x, p.B * p.Hk, p.tiles, p.causal, bh, kt)) return;
     const int kvh = bh % p.Hk, b = bh / p.Hk;
     const int key0 = (kt * NW + wave) * 32, key = key0 + col;
     const bool valid = key < p.Sk && (p.pad == nullptr || p.pad[(int64_t)b * p.ld_pad + key] == 0);
@@ -308,10 +305,8 @@ __global__ __launch_bounds__(64 * NW, DP >= 64 ? 1 : 2) void attention_dkv_kerne
             f32x16 s, dp;
 #pragma unroll
             for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
-#pragma unroll
-            for (int c = 0; c < NC; ++c) mma(s, load8(qs + (n * 32 + col) * KS + c * 16 + half * 8), k[c]);
-#pragma unroll
-            for (int c = 0; c < NC; ++c) mma(dp, load8(gs + (n * 32 + col) * KS + c * 16 + half * 8), v[c]);
+            pipelined<T, NC, 2>([&](int c, int j) { return load8((j == 0 ? qs : gs) + (n * 32 + col) * KS + c * 16 + half * 8); },
+                                [&](int c, int j, const Frag<T>& a) { mma(j == 0 ? s : dp, a, j == 0 ? k[c] : v[c]); });
             const int dmax = key0 + 31 - pos0, dmin = key0 - pos0 - 31;
             const bool far = dmax <= -R || dmin >= R;
             const float add = has_bias ? bias[dmax <= -R ? 0 : 2 * R] : 0.f;
@@ -344,14 +339,13 @@ __global__ __launch_bounds__(64 * NW, DP >= 64 ? 1 : 2) void attention_dkv_kerne
                     }
                 }
             }
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const Frag<T> pf = pack8<T>(s, c), df = pack8<T>(dp, c);
-#pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    mma(dv[d], col_frag<T, KS>(gs, n * 32 + c * 16, d * 32, lane), pf);
-                    mma(dk[d], col_frag<T, KS>(qs, n * 32 + c * 16, d * 32, lane), df);
-                }
+            {
+                const Frag<T> pf[2] = {pack8<T>(s, 0), pack8<T>(s, 1)}, df[2] = {pack8<T>(dp, 0), pack8<T>(dp, 1)};
+                pipelined<T, 4, ND>([&](int i, int d) { return col_frag<T, KS>((i & 1) == 0 ? gs : qs, n * 32 + (i >> 1) * 16, d * 32, lane); },
+                                    [&](int i, int d, const Frag<T>& a) {
+                                        if ((i & 1) == 0) mma(dv[d], a, pf[i >> 1]);
+                                        else mma(dk[d], a, df[i >> 1]);
+                                    });
             }
         }
     }
@@ -378,26 +372,43 @@ __global__ __launch_bounds__(256) void attention_dist_kernel(const float* part, 
     if (i >= n) return;
     const int per = (parts + kSeg - 1) / kSeg, s0 = blockIdx.y * per, s1 = min(parts, s0 + per);
     float a = 0.f;
-    for (int s = s0; s < s1; ++s) a += part[s * n + i];
+    for (int s = s0; s < s1; s += 8) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = s + j < s1 ? part[(s + j) * n + i] : 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a += v[j];
+    }
     seg[blockIdx.y * n + i] = a;
 }
-// ... then the segments, and distances into buckets in distance order
+// ... then the segments (four groups of them a workgroup), and distances into buckets: 32 lanes a bucket, each adding every 32nd distance
 template <class T>
-__global__ __launch_bounds__(256) void attention_bucket_kernel(const float* seg, const int32_t* buckets, int segs, int H, int nb, int NB, T* dtable) {
-    extern __shared__ float sum[];                                     // (nb) sums, then (nb) bucket ids
-    int* ids = reinterpret_cast<int*>(sum + nb);
-    const int h = blockIdx.x;
-    for (int i = threadIdx.x; i < nb; i += 256) {
+__global__ __launch_bounds__(1024) void attention_bucket_kernel(const float* seg, const int32_t* buckets, int segs, int H, int nb, int NB, T* dtable) {
+    extern __shared__ float sum[];                                     // (4, nb) sums, then (nb) bucket ids
+    int* ids = reinterpret_cast<int*>(sum + 4 * nb);
+    const int h = blockIdx.x, group = threadIdx.x >> 8, per = (segs + 3) / 4, s0 = group * per, s1 = min(segs, s0 + per);
+    for (int i = threadIdx.x & 255; i < nb; i += 256) {
+        const float* src = seg + (int64_t)h * nb + i;
         float a = 0.f;
-        for (int s = 0; s < segs; ++s) a += seg[((int64_t)s * H + h) * nb + i];
-        sum[i] = a;
-        ids[i] = buckets[i];
+        for (int s = s0; s < s1; s += 8) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = s + j < s1 ? src[(int64_t)(s + j) * H * nb] : 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) a += v[j];
+        }
+        sum[group * nb + i] = a;
+        if (group == 0) ids[i] = buckets[i];
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < NB; c += 256) {
+    const int l = threadIdx.x & 31;
+    for (int c = threadIdx.x >> 5; c < NB; c += 32) {
         float a = 0.f;
-        for (int i = 0; i < nb; ++i) a += ids[i] == c ? sum[i] : 0.f;
-        dtable[(int64_t)c * H + h] = (T)a;
+        for (int i = l; i < nb; i += 32)
+            if (ids[i] == c) a += (sum[i] + sum[nb + i]) + (sum[2 * nb + i] + sum[3 * nb + i]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) a += __shfl_xor(a, o, 64);
+        if (l == 0) dtable[(int64_t)c * H + h] = (T)a;
     }
 }
 
@@ -461,8 +472,9 @@ int launch_dkv(const AttnParams& p, int64_t blocks, hipStream_t s) {
 template <class T, int DP>
 int launch_dp(const vita_attention_args* a, AttnParams p, const BPlan& f, hipStream_t s) {
     constexpr int T4 = sizeof(T) == 2 ? 64 : 32;
+    constexpr int TQ = sizeof(T) == 2 && DP < 128 ? 64 : 32;      // dq at 128: with tiles of 64 keys the prefetch does not fit two waves a SIMD
     p.tiles = f.qtiles;
-    if (f.qw == 4) VITA_TRY((launch_dq<T, DP, 4, T4>(p, pair_grid((int64_t)a->H * a->B, f.qtiles), s)));
+    if (f.qw == 4) VITA_TRY((launch_dq<T, DP, 4, TQ>(p, pair_grid((int64_t)a->H * a->B, f.qtiles), s)));
     else VITA_TRY((launch_dq<T, DP, 1, 32>(p, pair_grid((int64_t)a->H * a->B, f.qtiles), s)));
     p.tiles = f.ktiles;
     if (f.kw == 4) return launch_dkv<T, DP, 4, T4>(p, pair_grid((int64_t)a->Hk * a->B, f.ktiles), s);
@@ -496,12 +508,12 @@ int run(const vita_attention_args* a, AttnParams& p, float* seg, hipStream_t s) 
     if (a->dtable != nullptr) {
         const int nb = 2 * a->radius + 1, parts = a->B * f.qtiles;
         const int64_t n = (int64_t)a->H * nb;
-        const bool two = parts > kSeg;                                 // few parts: the bucket kernel adds them itself
+        const bool two = parts > 8 * kSeg;                                 // few parts: the bucket kernel adds them itself
         if (two) {
             hipLaunchKernelGGL(attention_dist_kernel, dim3((unsigned)((n + 255) / 256), kSeg), dim3(256), 0, s, p.dist_part, seg, parts, a->H, nb);
             VITA_CHECK_HIP(hipGetLastError());
         }
-        hipLaunchKernelGGL(attention_bucket_kernel<T>, dim3((unsigned)a->H), dim3(256), (size_t)nb * 8, s, two ? seg : p.dist_part, a->buckets,
+        hipLaunchKernelGGL(attention_bucket_kernel<T>, dim3((unsigned)a->H), dim3(1024), (size_t)nb * 20, s, two ? seg : p.dist_part, a->buckets,
                            two ? kSeg : parts, a->H, nb, a->num_buckets, (T*)a->dtable);
         VITA_CHECK_HIP(hipGetLastError());
     }

@@ -28,9 +28,9 @@ __global__ __launch_bounds__(64 * NQ * NK, sizeof(T) == 4 && DP >= 96 ? 1 : 2) v
 
     const int groups = p.H / p.pack;
     int pair, id;
-    if (!pair_order(blockIdx.x, p.B * groups, p.tiles * p.splits, pair, id)) return;
-    const int qt = p.causal ? p.tiles - 1 - id % p.tiles : id % p.tiles;       // the rows with the most keys first
-    const int split = id / p.tiles, hy = pair % groups, b = pair / groups;
+    if (!pair_order(blockIdx.x, p.B * groups, p.tiles * p.splits, p.causal, pair, id)) return;
+    const int split = id % p.splits, qt = p.causal ? p.tiles - 1 - id / p.splits : id / p.splits;       // the rows with the most keys first
+    const int hy = pair % groups, b = pair / groups;
     const int rows = p.Sq * p.pack, head0 = hy * p.pack, kvh = head0 / p.G;
 
     const int row = (qt * NQ + wq) * 32 + col;
@@ -100,12 +100,11 @@ __global__ __launch_bounds__(64 * NQ * NK, sizeof(T) == 4 && DP >= 96 ? 1 : 2) v
         if (bits != 0 && first_row < rows && !(p.causal && key0 > pos_hi)) {
             f32x16 s[NS];
 #pragma unroll
-            for (int n = 0; n < NS; ++n) {
+            for (int n = 0; n < NS; ++n)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[n][r] = 0.f;
-#pragma unroll
-                for (int c = 0; c < NC; ++c) mma(s[n], load8(kt + (wk * KW + n * 32 + col) * KS + c * 16 + half * 8), q[c]);
-            }
+            pipelined<T, NC, NS>([&](int c, int n) { return load8(kt + (wk * KW + n * 32 + col) * KS + c * 16 + half * 8); },
+                                 [&](int c, int n, const Frag<T>& a) { mma(s[n], a, q[c]); });
             const bool full = (KW == 64 ? bits == ~uint64_t(0) : (uint32_t)bits == 0xffffffffu) && !(p.causal && key0 + KW - 1 > pos_lo);
             const int far_lo = key0 + KW - 1 - pos_lo, far_hi = key0 - pos_hi;           // largest and smallest distance of the wave's tile
             // a tile that every row sees whole, its bias one number: the scale goes into the exponent's multiply-add
@@ -148,23 +147,24 @@ __global__ __launch_bounds__(64 * NQ * NK, sizeof(T) == 4 && DP >= 96 ? 1 : 2) v
                 m = to;
             }
             const float shift = add - (m == -kInf ? 0.f : m);
-            float sum = 0.f;
+            // probabilities of 16 keys at a time, so that a step's exponentials run beside the previous step's products
+            Frag<T> pf;
+            pipelined<T, 2 * NS, ND>(
+                [&](int i, int d) { return col_frag<T, KS>(vt, wk * KW + i * 16, d * 32, lane); },
+                [&](int i, int d, const Frag<T>& a) {
+                    if (d == 0) {
+                        f32x16& sn = s[i >> 1];
+                        float sum = 0.f;
 #pragma unroll
-            for (int n = 0; n < NS; ++n)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    s[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], mul, shift));
-                    sum += s[n][r];
-                }
-            l += sum;
-#pragma unroll
-            for (int n = 0; n < NS; ++n)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const Frag<T> pf = pack8<T>(s[n], c);
-#pragma unroll
-                    for (int d = 0; d < ND; ++d) mma(o[d], col_frag<T, KS>(vt, wk * KW + n * 32 + c * 16, d * 32, lane), pf);
-                }
+                        for (int r = (i & 1) * 8; r < (i & 1) * 8 + 8; ++r) {
+                            sn[r] = __builtin_amdgcn_exp2f(fmaf(sn[r], mul, shift));
+                            sum += sn[r];
+                        }
+                        l += sum;
+                        pf = pack8<T>(sn, i & 1);
+                    }
+                    mma(o[d], a, pf);
+                });
         }
         t = tn;
     }

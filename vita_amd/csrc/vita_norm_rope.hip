@@ -20,7 +20,9 @@ namespace vita {
 namespace {
 
 constexpr int RNT = 256;
-constexpr int kMaxBlocks = 2048;       // workgroups a side, and partial rows of the weight gradients
+// rows a group has in flight: enough to cover the latency at 4 workgroups a CU (backward: 2 leave room for those 4)
+constexpr int rows_in_flight(bool bwd) { return bwd ? 2 : 4; }
+constexpr int kMaxBlocks = 1024;       // backward: workgroups (4 a CU, shared out by the sides' rows), and partial rows of the weight gradients
 
 template <class T> struct Vec;
 template <> struct Vec<float> { static constexpr int N = 4; };
@@ -43,23 +45,24 @@ struct Params {
     const int64_t* positions; int64_t ld_positions;
 };
 
+// a lane's columns of a row as they lie in memory; `wide` turns them into fp32 where they are used, so that the loads of several rows
+// are in flight together at their own size
+template <class T, int N> struct Raw { T v[N] __attribute__((aligned(16))); };
 template <class T, int N, bool ALIGNED>
-__device__ __forceinline__ void load_row(const char* base, int64_t off, int c0, int D, float (&v)[N]) {
+__device__ __forceinline__ void load_row(const char* base, int64_t off, int c0, int D, Raw<T, N>& r) {
     const T* p = reinterpret_cast<const T*>(base) + off + c0;
     if constexpr (ALIGNED) {
-        typedef T vec __attribute__((ext_vector_type(N)));
-        if (c0 < D) {
-            const vec u = *reinterpret_cast<const vec*>(p);
-#pragma unroll
-            for (int j = 0; j < N; ++j) v[j] = (float)u[j];
-        } else {
-#pragma unroll
-            for (int j = 0; j < N; ++j) v[j] = 0.f;
-        }
+        const uint4 u = c0 < D ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+        r = __builtin_bit_cast(Raw<T , N>, u);
     } else {
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = c0 + j < D ? (float)p[j] : 0.f;
+        for (int j = 0; j < N; ++j) r.v[j] = c0 + j < D ? p[j] : (T)0.f;
     }
+}
+template <class T, int N>
+__device__ __forceinline__ void wide(const Raw<T, N>& r, float (&v)[N]) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = (float)r.v[j];
 }
 
 template <class T, int N, bool ALIGNED>
@@ -89,17 +92,15 @@ __device__ __forceinline__ float group_sum(float v) {
 
 // cos / sin of the lane's N / 2 pairs.  A position outside the table never leaves it: its row becomes NaN.
 template <int N>
-__device__ __forceinline__ void load_turn(const Params& p, int b, int s, int h, int c0, float (&c)[N / 2], float (&sn)[N / 2]) {
+__device__ __forceinline__ void load_turn(const Params& p, int b, int s, int h, int c0, float2 (&t)[N / 2]) {
     const int64_t pos = p.positions != nullptr ? p.positions[(int64_t)b * p.ld_positions + s] : (int64_t)s;
     const bool in = pos >= 0 && pos < p.rope_rows;
     const int half = p.D >> 1;
-    const float* t = p.rope + (((in ? pos : 0) * p.rope_heads + (p.rope_heads > 1 ? h : 0)) * half + (c0 >> 1)) * 2;
+    const float* src = p.rope + (((in ? pos : 0) * p.rope_heads + (p.rope_heads > 1 ? h : 0)) * half + (c0 >> 1)) * 2;
 #pragma unroll
     for (int j = 0; j < N / 2; ++j) {
-        const bool col = c0 + 2 * j < p.D;
-        const float2 v = col ? *reinterpret_cast<const float2*>(t + 2 * j) : make_float2(1.f, 0.f);
-        c[j] = in ? v.x : __builtin_nanf("");
-        sn[j] = in ? v.y : __builtin_nanf("");
+        const float2 v = c0 + 2 * j < p.D ? *reinterpret_cast<const float2*>(src + 2 * j) : make_float2(1.f, 0.f);
+        t[j] = in ? v : make_float2(__builtin_nanf(""), __builtin_nanf(""));
     }
 }
 
@@ -125,7 +126,7 @@ __device__ __forceinline__ void normalise(float (&x)[N], int c0, int D, float ep
 
 template <class T, int LPR, bool LAYER, bool ALIGNED, bool BWD>
 __global__ __launch_bounds__(RNT) void norm_rope_kernel(Params p) {
-    constexpr int N = Vec<T>::N, GPB = RNT / LPR;
+    constexpr int N = Vec<T>::N, GPB = RNT / LPR, U = rows_in_flight(BWD);
     const bool second = (int)blockIdx.x >= p.side[0].blocks;
     const Side& sd = p.side[second];
     const int block = (int)blockIdx.x - (second ? p.side[0].blocks : 0);
@@ -139,48 +140,76 @@ __global__ __launch_bounds__(RNT) void norm_rope_kernel(Params p) {
     }
     float dw[N] = {}, db[N] = {};
 
-    const unsigned stride = (unsigned)sd.blocks * GPB;      // rows + stride < 2^32: the walk cannot wrap
-    for (unsigned row = (unsigned)block * GPB + group; row < sd.rows; row += stride) {
-        const unsigned tok = row / (unsigned)sd.H;
-        const int h = (int)(row - tok * sd.H);
-        const int b = (int)(tok / (unsigned)p.S), s = (int)(tok - (unsigned)b * p.S);
-        float x[N], c[N / 2], sn[N / 2], r;
-        load_row<T, N, ALIGNED>(sd.x, (int64_t)b * sd.x_sb + (int64_t)s * sd.x_ss + (int64_t)h * sd.x_sh, c0, D, x);
-        load_turn<N>(p, b, s, h, c0, c, sn);
-        if constexpr (!BWD) {
+    // U rows of a group at a time: their loads are in flight together, and where they are heads of one token under one table (H a
+    // multiple of U) the token's place and its cos / sin are formed once
+    const bool share = sd.H % U == 0, one_turn = share && p.rope_heads == 1;
+    const uint64_t stride = (uint64_t)sd.blocks * GPB * U;
+    for (uint64_t row0 = ((uint64_t)block * GPB + group) * U; row0 < sd.rows; row0 += stride) {
+        Raw<T, N> xr[U], gr[BWD ? U : 1];
+        float2 turn[U][N / 2];
+        int b[U], s[U], h[U];
+        const int n = sd.rows - (unsigned)row0 < U ? (int)(sd.rows - (unsigned)row0) : U;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (u > 0 && share) {
+                b[u] = b[0];
+                s[u] = s[0];
+                h[u] = h[0] + u;
+            } else {
+                const unsigned row = (unsigned)row0 + (u < n ? u : 0), tok = row / (unsigned)sd.H;
+                h[u] = (int)(row - tok * sd.H);
+                b[u] = (int)(tok / (unsigned)p.S);
+                s[u] = (int)(tok - (unsigned)b[u] * p.S);
+            }
+            load_row<T, N, ALIGNED>(sd.x, (int64_t)b[u] * sd.x_sb + (int64_t)s[u] * sd.x_ss + (int64_t)h[u] * sd.x_sh, c0, D, xr[u]);
+            if constexpr (BWD)
+                load_row<T, N, ALIGNED>(sd.dy, (int64_t)b[u] * sd.dy_sb + (int64_t)s[u] * sd.dy_ss + (int64_t)h[u] * sd.dy_sh, c0, D, gr[u]);
+            if (u == 0 || !one_turn) load_turn<N>(p, b[u], s[u], h[u], c0, turn[u]);
+            else {
+#pragma unroll
+                for (int j = 0; j < N / 2; ++j) turn[u][j] = turn[0][j];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (u >= n) break;
+            float x[N], r;
+            wide<T, N>(xr[u], x);
             normalise<N, LPR, LAYER>(x, c0, D, p.eps, r);
-            float y[N];
+            const int64_t to = (int64_t)b[u] * sd.y_sb + (int64_t)s[u] * sd.y_ss + (int64_t)h[u] * sd.y_sh;
+            float out[N];
+            if constexpr (!BWD) {
 #pragma unroll
-            for (int j = 0; j < N / 2; ++j) {
-                const float t0 = fmaf(x[2 * j], w[2 * j], bias[2 * j]), t1 = fmaf(x[2 * j + 1], w[2 * j + 1], bias[2 * j + 1]);
-                y[2 * j] = fmaf(t0, c[j], -(t1 * sn[j]));
-                y[2 * j + 1] = fmaf(t1, c[j], t0 * sn[j]);
+                for (int j = 0; j < N / 2; ++j) {
+                    const float c = turn[u][j].x, sn = turn[u][j].y;
+                    const float t0 = fmaf(x[2 * j], w[2 * j], bias[2 * j]), t1 = fmaf(x[2 * j + 1], w[2 * j + 1], bias[2 * j + 1]);
+                    out[2 * j] = fmaf(t0, c, -(t1 * sn));
+                    out[2 * j + 1] = fmaf(t1, c, t0 * sn);
+                }
+            } else {
+                float g[N], e_sum = 0.f, en_sum = 0.f;
+                wide<T, N>(gr[u], g);
+#pragma unroll
+                for (int j = 0; j < N / 2; ++j) {
+                    const float c = turn[u][j].x, sn = turn[u][j].y;
+                    out[2 * j] = fmaf(g[2 * j], c, g[2 * j + 1] * sn);
+                    out[2 * j + 1] = fmaf(g[2 * j + 1], c, -(g[2 * j] * sn));
+                }
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    dw[j] = fmaf(out[j], x[j], dw[j]);
+                    db[j] += out[j];
+                    out[j] *= w[j];
+                    e_sum += out[j];
+                    en_sum = fmaf(out[j], x[j], en_sum);
+                }
+                const float inv = 1.0f / (float)D;
+                const float en = group_sum<LPR>(en_sum) * inv;
+                const float em = LAYER ? group_sum<LPR>(e_sum) * inv : 0.f;
+#pragma unroll
+                for (int j = 0; j < N; ++j) out[j] = r * (out[j] - em - x[j] * en);
             }
-            store_row<T, N, ALIGNED>(sd.y, (int64_t)b * sd.y_sb + (int64_t)s * sd.y_ss + (int64_t)h * sd.y_sh, c0, D, y);
-        } else {
-            float g[N], d[N];
-            load_row<T, N, ALIGNED>(sd.dy, (int64_t)b * sd.dy_sb + (int64_t)s * sd.dy_ss + (int64_t)h * sd.dy_sh, c0, D, g);
-            normalise<N, LPR, LAYER>(x, c0, D, p.eps, r);
-            float e_sum = 0.f, en_sum = 0.f;
-#pragma unroll
-            for (int j = 0; j < N / 2; ++j) {
-                d[2 * j] = fmaf(g[2 * j], c[j], g[2 * j + 1] * sn[j]);
-                d[2 * j + 1] = fmaf(g[2 * j + 1], c[j], -(g[2 * j] * sn[j]));
-            }
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                dw[j] = fmaf(d[j], x[j], dw[j]);
-                db[j] += d[j];
-                d[j] *= w[j];
-                e_sum += d[j];
-                en_sum = fmaf(d[j], x[j], en_sum);
-            }
-            const float inv = 1.0f / (float)D;
-            const float en = group_sum<LPR>(en_sum) * inv;
-            const float em = LAYER ? group_sum<LPR>(e_sum) * inv : 0.f;
-#pragma unroll
-            for (int j = 0; j < N; ++j) d[j] = r * (d[j] - em - x[j] * en);
-            store_row<T, N, ALIGNED>(sd.y, (int64_t)b * sd.y_sb + (int64_t)s * sd.y_ss + (int64_t)h * sd.y_sh, c0, D, d);
+            store_row<T, N, ALIGNED>(sd.y, to, c0, D, out);
         }
     }
     if constexpr (BWD) {
@@ -201,22 +230,30 @@ __global__ __launch_bounds__(RNT) void norm_rope_kernel(Params p) {
     }
 }
 
-// the partial rows of a side, added in index order: 16 segments of rows a workgroup, then the segments
+// the partial rows of a side, added in index order: 64 segments of rows a workgroup, 16 columns each, then the segments
 struct ReduceSide { const float* partial; float* dweight; float* dbias; int blocks; };
-__global__ __launch_bounds__(256) void norm_rope_reduce_kernel(ReduceSide q, ReduceSide k, int D) {
+__global__ __launch_bounds__(1024) void norm_rope_reduce_kernel(ReduceSide q, ReduceSide k, int D) {
     const ReduceSide& s = blockIdx.y ? k : q;
-    __shared__ float part[16][17];
+    __shared__ float part[64][17];
     const int col = blockIdx.x * 16 + (threadIdx.x & 15), seg = threadIdx.x >> 4;
-    const int per = (s.blocks + 15) / 16;
+    const int per = (s.blocks + 63) / 64, r0 = seg * per, r1 = min(s.blocks, r0 + per);
     float a = 0.f;
-    if (col < 2 * D)
-        for (int r = seg * per; r < min(s.blocks, (seg + 1) * per); ++r) a += s.partial[(int64_t)r * 2 * D + col];
+    if (col < 2 * D) {
+        const float* src = s.partial + col;
+        for (int r = r0; r < r1; r += 8) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = r + j < r1 ? src[(int64_t)(r + j) * 2 * D] : 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) a += v[j];
+        }
+    }
     part[seg][threadIdx.x & 15] = a;
     __syncthreads();
     if (seg == 0 && col < 2 * D) {
         float t = 0.f;
 #pragma unroll
-        for (int g = 0; g < 16; ++g) t += part[g][threadIdx.x & 15];
+        for (int g = 0; g < 64; ++g) t += part[g][threadIdx.x & 15];
         if (col < D) {
             if (s.dweight != nullptr) s.dweight[col] = t;
         } else if (s.dbias != nullptr) {
@@ -257,9 +294,10 @@ int group_lanes(int dtype, int D) {
 int side_blocks(const vita_norm_rope_args* a, int H, bool bwd) {
     const int gpb = RNT / group_lanes(a->dtype, a->D);
     const int64_t rows = (int64_t)a->B * a->S * H;
-    // forward: 4 rows a group amortise the weight loads; backward: at most kMaxBlocks partial rows
-    const int64_t want = bwd ? (rows + gpb - 1) / gpb : (rows + 4 * gpb - 1) / (4 * gpb);
-    return (int)(want < 1 ? 1 : (bwd && want > kMaxBlocks ? kMaxBlocks : (want > (1 << 20) ? (1 << 20) : want)));
+    const int64_t per = (int64_t)rows_in_flight(bwd) * gpb, want = (rows + per - 1) / per;
+    if (!bwd) return (int)(want < 1 ? 1 : want);
+    const int64_t most = kMaxBlocks * (int64_t)H / (a->q.H + a->k.H);
+    return (int)(want < 1 || most < 1 ? 1 : (want > most ? most : want));
 }
 
 int check(const vita_norm_rope_args* a, bool bwd, const char* who) {
@@ -330,7 +368,7 @@ int run(const vita_norm_rope_args* a, bool bwd, void* ws, hipStream_t s) {
     }
     VITA_CHECK_HIP(hipGetLastError());
     if (any) {
-        hipLaunchKernelGGL(norm_rope_reduce_kernel, dim3((2 * a->D + 15) / 16, 2), dim3(256), 0, s, red[0], red[1], a->D);
+        hipLaunchKernelGGL(norm_rope_reduce_kernel, dim3((2 * a->D + 15) / 16, 2), dim3(1024), 0, s, red[0], red[1], a->D);
         VITA_CHECK_HIP(hipGetLastError());
     }
     return VITA_OK;

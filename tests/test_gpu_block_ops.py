@@ -349,6 +349,14 @@ def test_gated(dtype, M, K, F):
     _check_gated(*_gated_case(g, M, K, F, dtype, False), "gelu_tanh", g)
 
 
+@pytest.mark.parametrize("M,K,F,act", [(2049, 72, 2816, "silu"), (2300, 40, 2568, "gelu_tanh"), (2100, 264, 2720, "mish"),       # the product's tiles fill the chip
+                                       (12289, 1000, 40, "silu"),                                                             # dx's do
+                                       (40, 1000, 6152, "gelu"), (77, 1032, 6400, "silu")])                                   # dw's do
+def test_gated_wide(M, K, F, act):
+    g = _gen(M + F)
+    _check_gated(*_gated_case(g, M, K, F, torch.bfloat16, M != 2300), act, g)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("act", ["relu", "gelu", "gelu_tanh", "silu", "mish"])
 def test_gated_activations(dtype, act):

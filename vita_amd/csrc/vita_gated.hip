@@ -1,13 +1,19 @@
 // The gated feed-forward product h = act(x Wg^T + bg) * (x Wu^T + bu) and its backward pass (see include/vita_hip.h).
 //
-// First form: one product for both projections into a pre-activation matrix z (M, 2F) with the library's GEMMs, then one elementwise
-// pass.  Backward: z (saved, or formed again), one pass for dz and the bias gradient's partial sums, then dx = dz W and dw = dz^T x.
-#include "vita_host.h"
+// bf16 products that fill the chip run on the 256 x 256 tile of vita_gemm_bf16_wide.h: a tile's columns are 128 features' gate and up
+// projections, a wave's two column blocks the same 32 features, so both are in one lane's registers and the epilogue writes h alone.
+// Backward: the same product again with another epilogue (reads dh, writes dz = [dg | du] in bf16 and fp32 partial sums for db), then
+// dx = dz W and dw = dz^T x on the operands as they lie.  Forming z again costs 2 of 8 products but keeps nothing between the passes:
+// saved in bf16 it would round the slopes' arguments, saved in fp32 it would move 4 M F bytes twice.  dz is rounded to bf16 because the
+// matrix unit takes bf16 operands; db is summed before that rounding.
+// Everything else goes over z (M, 2F) in fp32 with the library's GEMMs and one elementwise pass: fp32 (where the product runs at a
+// sixteenth of the rate and saving z is the cheap choice) and small bf16 calls.
+#include <type_traits>
+
+#include "vita_gemm_bf16_wide.h"
 
 namespace vita {
 namespace {
-
-typedef __bf16 bf16;
 
 template <class T>
 __global__ __launch_bounds__(256) void gated_product_kernel(const float* z, int64_t ldz, T* h, int64_t ldh, int M, int F, int act) {
@@ -61,11 +67,147 @@ __global__ __launch_bounds__(256) void to_bf16_kernel(const float* src, bf16* ds
     dst[r * ldd + (i - r * cols)] = (bf16)src[i];
 }
 
+// ---- the wide bf16 products ------------------------------------------------------------------------------------------------------
+struct WideOut {
+    const float* bias;
+    bf16* c; int64_t ldc;                 // h, or C
+    const bf16* dh; int64_t ld_dh;        // dz
+    bf16* dz; int64_t ld_dz;
+    float* db_part;                       // (tiles_m, 2 F)
+};
+enum { WIDE_H = 0, WIDE_DZ = 1, WIDE_C = 2 };
+
+// EPI WIDE_H: h (M, F) of a gated product; WIDE_DZ: dz (M, 2F) of a gated product; WIDE_C: plain C (M, N)
+template <bool ACOL, bool BCOL, int EPI, int ACT>
+__global__ __launch_bounds__(WNT, 2) void wide_gemm_kernel(WideGemm g, WideOut o) {
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    constexpr bool GATED = EPI != WIDE_C;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 2, wn = wave & 3, col = lane & 31, half = lane >> 5;
+    int tm, tn;
+    wide_place(g, blockIdx.x, gridDim.x, tm, tn);
+    const int m0 = tm * WBM, n0 = tn * (GATED ? WBN / 2 : WBN);
+    f32x16 acc[4][2];
+    wide_tile<ACOL, BCOL, GATED>(g, lds, m0, n0, acc);
+
+    // through LDS, so that the global stores are whole 16-byte pieces of rows
+    if constexpr (!GATED) {
+        bf16* t = reinterpret_cast<bf16*>(lds);
+        constexpr int LD = WBN;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    t[(wm * 128 + i * 32 + (r >> 2) * 8 + half * 4 + (r & 3)) * LD + wn * 64 + j * 32 + col] = (bf16)acc[i][j][r];
+        __syncthreads();
+        for (int i = tid; i < WBM * (WBN / 8); i += WNT) {
+            const int row = i / (WBN / 8), c = (i - row * (WBN / 8)) * 8;
+            if (m0 + row < g.M && n0 + c < g.N)
+                *reinterpret_cast<uint4*>(o.c + (int64_t)(m0 + row) * o.ldc + n0 + c) = *reinterpret_cast<const uint4*>(t + row * LD + c);
+        }
+        return;
+    }
+    const int f = n0 + wn * 32 + col;
+    float bg = 0.f, bu = 0.f;
+    if (o.bias != nullptr && f < g.F) {
+        bg = o.bias[f];
+        bu = o.bias[g.F + f];
+    }
+    constexpr int LD = WBN / 2;
+    bf16* t = reinterpret_cast<bf16*>(lds);               // (256, 128): h, or dh and then dg
+    bf16* tu = t + WBM * LD;                              // (256, 128): du
+    if constexpr (EPI == WIDE_DZ) {
+        for (int i = tid; i < WBM * (LD / 8); i += WNT) {
+            const int row = i / (LD / 8), c = (i - row * (LD / 8)) * 8;
+            const bool in = m0 + row < g.M && n0 + c < g.F;
+            *reinterpret_cast<uint4*>(t + row * LD + c) = in ? *reinterpret_cast<const uint4*>(o.dh + (int64_t)(m0 + row) * o.ld_dh + n0 + c) : make_uint4(0, 0, 0, 0);
+        }
+        __syncthreads();
+    }
+    float sg = 0.f, su = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int at = (wm * 128 + i * 32 + (r >> 2) * 8 + half * 4 + (r & 3)) * LD + wn * 32 + col;
+            const float zg = acc[i][0][r] + bg, zu = acc[i][1][r] + bu;
+            if constexpr (EPI == WIDE_H) {
+                t[at] = (bf16)(apply_act_t<ACT>(zg) * zu);
+            } else {
+                const float d = (float)t[at];
+                const float dg = d * zu * act_grad(zg, ACT), du = d * apply_act_t<ACT>(zg);
+                t[at] = (bf16)dg;
+                tu[at] = (bf16)du;
+                sg += dg;
+                su += du;
+            }
+        }
+    __syncthreads();
+    for (int i = tid; i < WBM * (LD / 8); i += WNT) {
+        const int row = i / (LD / 8), c = (i - row * (LD / 8)) * 8;
+        if (m0 + row < g.M && n0 + c < g.F) {
+            if constexpr (EPI == WIDE_H) {
+                *reinterpret_cast<uint4*>(o.c + (int64_t)(m0 + row) * o.ldc + n0 + c) = *reinterpret_cast<const uint4*>(t + row * LD + c);
+            } else {
+                bf16* dst = o.dz + (int64_t)(m0 + row) * o.ld_dz + n0 + c;
+                *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(t + row * LD + c);
+                *reinterpret_cast<uint4*>(dst + g.F) = *reinterpret_cast<const uint4*>(tu + row * LD + c);
+            }
+        }
+    }
+    if constexpr (EPI == WIDE_DZ) {
+        if (o.db_part != nullptr) {                       // the halves, then the two waves of a column block, in that order
+            __syncthreads();
+            float* part = reinterpret_cast<float*>(lds);  // (2, 4, 2, 32)
+            sg += __shfl_xor(sg, 32, 64);
+            su += __shfl_xor(su, 32, 64);
+            if (half == 0) {
+                part[((wm * 4 + wn) * 2 + 0) * 32 + col] = sg;
+                part[((wm * 4 + wn) * 2 + 1) * 32 + col] = su;
+            }
+            __syncthreads();
+            if (wm == 0 && half == 0 && f < g.F) {
+                float* dst = o.db_part + (int64_t)tm * 2 * g.F + f;
+                dst[0] = part[(wn * 2 + 0) * 32 + col] + part[((4 + wn) * 2 + 0) * 32 + col];
+                dst[g.F] = part[(wn * 2 + 1) * 32 + col] + part[((4 + wn) * 2 + 1) * 32 + col];
+            }
+        }
+    }
+}
+
+template <bool ACOL, bool BCOL, int EPI, int ACT = VITA_ACT_NONE>
+int launch_wide(const bf16* A, int64_t lda, const bf16* B, int64_t ldb, int M, int N, int K, int F, const WideOut& o, hipStream_t s) {
+    WideGemm g{{A, lda}, {B, ldb}, M, N, K, (M + WBM - 1) / WBM, 0, F};
+    g.tiles_n = EPI == WIDE_C ? (N + WBN - 1) / WBN : (F + WBN / 2 - 1) / (WBN / 2);
+    hipLaunchKernelGGL((wide_gemm_kernel<ACOL, BCOL, EPI, ACT>), dim3((unsigned)(g.tiles_m * g.tiles_n)), dim3(WNT), WLDS, s, g, o);
+    VITA_CHECK_HIP(hipGetLastError());
+    return VITA_OK;
+}
+template <int EPI>
+int launch_wide_gated(const vita_gated_args* a, const WideOut& o, hipStream_t s) {
+    auto go = [&](auto act) {
+        return launch_wide<false, false, EPI, decltype(act)::value>((const bf16*)a->x, a->ldx, (const bf16*)a->w, a->ldw, a->M, 2 * a->F, a->K, a->F, o, s);
+    };
+    switch (a->act) {
+        case VITA_ACT_RELU: return go(std::integral_constant<int, VITA_ACT_RELU>{});
+        case VITA_ACT_GELU_ERF: return go(std::integral_constant<int, VITA_ACT_GELU_ERF>{});
+        case VITA_ACT_GELU_TANH: return go(std::integral_constant<int, VITA_ACT_GELU_TANH>{});
+        case VITA_ACT_SILU: return go(std::integral_constant<int, VITA_ACT_SILU>{});
+        default: return go(std::integral_constant<int, VITA_ACT_MISH>{});
+    }
+}
+// whether a C of M x N has enough 256 x 256 tiles to keep the 256 CUs busy
+bool wide_fills(int64_t M, int64_t N) {
+    const int64_t t = ((M + WBM - 1) / WBM) * ((N + WBN - 1) / WBN);
+    return t >= 192 && t < (int64_t(1) << 31);
+}
+
 int check(const vita_gated_args* a, bool bwd, const char* who) {
     VITA_REQUIRE(a != nullptr, "%s: null args", who);
     VITA_REQUIRE(a->dtype == VITA_DT_F32 || a->dtype == VITA_DT_BF16, "%s: unknown dtype %d", who, a->dtype);
     VITA_REQUIRE(a->act >= VITA_ACT_RELU && a->act <= VITA_ACT_MISH, "%s: unknown activation %d", who, a->act);
-    VITA_REQUIRE(a->M >= 0 && a->F >= 8 && a->K >= 8 && a->F % 8 == 0 && a->K % 8 == 0 && a->F <= (1 << 28), "%s: bad shape M=%d F=%d K=%d (F and K multiples of 8)",
+    VITA_REQUIRE(a->M >= 0 && a->F >= 8 && a->K >= 8 && a->F % 8 == 0 && a->K % 8 == 0 && a->F <= (1 << 28) && a->M <= (1 << 28), "%s: bad shape M=%d F=%d K=%d (F and K multiples of 8)",
                  who, a->M, a->F, a->K);
     const int vec = a->dtype == VITA_DT_F32 ? 4 : 8;
     auto ok = [&](const void* p, int64_t ld, int64_t n) { return p != nullptr && (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % vec == 0 && ld >= n; };
@@ -83,18 +225,22 @@ int check(const vita_gated_args* a, bool bwd, const char* who) {
     return VITA_OK;
 }
 
+// bf16 products whose z is not given and whose tiles fill the chip
+bool wide_product(const vita_gated_args* a) { return a->dtype == VITA_DT_BF16 && a->z == nullptr && wide_fills(a->M, 2 * (int64_t)a->F); }
+
 struct Ws { float* sk; float* z; void* dz; float* dw32; void* wt; float* db_part; float* cs; size_t bytes; };
 Ws carve(const vita_gated_args* a, bool bwd, void* ws) {
     Carver c(ws);
     Ws r{};
     const size_t M = a->M, F2 = 2 * (size_t)a->F, K = a->K;
-    r.sk = c.take(kSplitkBytes / 4);
-    if (a->z == nullptr) r.z = c.take(M * F2);
+    const bool wide = wide_product(a);
+    if (bwd || !wide) r.sk = c.take(kSplitkBytes / 4);
+    if (a->z == nullptr && !wide) r.z = c.take(M * F2);
     if (bwd) {
         const size_t es = a->dtype == VITA_DT_F32 ? 4 : 2;
         r.dz = c.take((M * F2 * es + 3) / 4);
-        if (a->dtype == VITA_DT_BF16) r.dw32 = c.take(F2 * K);
-        r.wt = c.take((F2 * K * es + 3) / 4);
+        if (a->dtype == VITA_DT_BF16 && a->dw != nullptr && !wide_fills(F2, K)) r.dw32 = c.take(F2 * K);
+        if (a->dtype == VITA_DT_BF16 && a->dx != nullptr && !wide_fills(M, K)) r.wt = c.take((F2 * K * es + 3) / 4);
         const size_t segs = (M + kDzRows - 1) / kDzRows;
         r.db_part = c.take(segs * F2);
         r.cs = c.take((size_t)vita_colsum_partials_count((int32_t)F2));
@@ -120,15 +266,21 @@ int run_bwd(const vita_gated_args* a, void* workspace, hipStream_t s) {
     const int M = a->M, F = a->F, F2 = 2 * a->F, K = a->K;
     const float* z = a->z;
     int64_t ldz = a->ldz;
-    if (z == nullptr) {
+    const bool wide = wide_product(a);
+    if (z == nullptr && !wide) {
         VITA_TRY(preact(a, ws.z, F2, ws, s));
         z = ws.z;
         ldz = F2;
     }
-    const int segs = (M + kDzRows - 1) / kDzRows;
-    const dim3 grid((F + 255) / 256, segs);
     float* part = a->db != nullptr ? ws.db_part : nullptr;
-    if (a->dtype == VITA_DT_F32)
+    int segs = (M + kDzRows - 1) / kDzRows;
+    const dim3 grid((F + 255) / 256, segs);
+    if (wide) {
+        WideOut o{};
+        o.bias = a->b; o.dh = (const bf16*)a->dh; o.ld_dh = a->ld_dh; o.dz = (bf16*)ws.dz; o.ld_dz = F2; o.db_part = part;
+        VITA_TRY(launch_wide_gated<WIDE_DZ>(a, o, s));
+        segs = (M + WBM - 1) / WBM;
+    } else if (a->dtype == VITA_DT_F32)
         hipLaunchKernelGGL(gated_dz_kernel<float>, grid, dim3(256), 0, s, z, ldz, (const float*)a->dh, a->ld_dh, (float*)ws.dz, F2, part, M, F, a->act);
     else
         hipLaunchKernelGGL(gated_dz_kernel<bf16>, grid, dim3(256), 0, s, z, ldz, (const bf16*)a->dh, a->ld_dh, (bf16*)ws.dz, F2, part, M, F, a->act);
@@ -140,14 +292,22 @@ int run_bwd(const vita_gated_args* a, void* workspace, hipStream_t s) {
         if (a->dw != nullptr) VITA_TRY(gemm_f32(wgrad((const float*)ws.dz, F2, (const float*)a->x, a->ldx, (float*)a->dw, a->ld_dw, M, K, F2), s));
         return VITA_OK;
     }
-    if (a->dx != nullptr) {
+    if (a->dx != nullptr && wide_fills(M, K)) {
+        WideOut o{};
+        o.c = (bf16*)a->dx; o.ldc = a->ld_dx;
+        VITA_TRY((launch_wide<false, true, WIDE_C>((const bf16*)ws.dz, F2, (const bf16*)a->w, a->ldw, M, K, F2, 0, o, s)));
+    } else if (a->dx != nullptr) {
         hipLaunchKernelGGL(transpose16_kernel, dim3((K + 63) / 64, (F2 + 63) / 64), dim3(256), 0, s, (const uint16_t*)a->w, a->ldw, (uint16_t*)ws.wt, (int64_t)F2, F2, K);
         VITA_CHECK_HIP(hipGetLastError());
         vita_linear_args l{};
         l.X = (const float*)ws.dz; l.ldx = F2; l.W = (const float*)ws.wt; l.ldw = F2; l.M = M; l.N = K; l.K = F2; l.ldy = K;
         VITA_TRY(gemm_bf16_dma(l, (uint16_t*)a->dx, a->ld_dx, s));
     }
-    if (a->dw != nullptr) {
+    if (a->dw != nullptr && wide_fills(F2, K)) {
+        WideOut o{};
+        o.c = (bf16*)a->dw; o.ldc = a->ld_dw;
+        VITA_TRY((launch_wide<true, true, WIDE_C>((const bf16*)ws.dz, F2, (const bf16*)a->x, a->ldx, F2, K, M, 0, o, s)));
+    } else if (a->dw != nullptr) {
         vita_linear_args l{};
         l.Y = ws.dw32; l.ldy = K; l.M = F2; l.N = K; l.K = M; l.splitk_ws = ws.sk; l.splitk_ws_bytes = kSplitkBytes;
         VITA_TRY(gemm_bf16_wgrad_tn((const uint16_t*)ws.dz, F2, (const uint16_t*)a->x, a->ldx, l, s));
@@ -175,6 +335,11 @@ int vita_gated_linear(const vita_gated_args* a, void* workspace, size_t workspac
     if (a->M == 0) return VITA_OK;
     VITA_TRY(check_ws(workspace, workspace_bytes, vita_gated_linear_workspace_bytes(a), who));
     hipStream_t s = (hipStream_t)stream;
+    if (wide_product(a)) {
+        WideOut o{};
+        o.bias = a->b; o.c = (bf16*)a->h; o.ldc = a->ldh;
+        return launch_wide_gated<WIDE_H>(a, o, s);
+    }
     const Ws ws = carve(a, false, workspace);
     float* z = a->z != nullptr ? a->z : ws.z;
     const int64_t ldz = a->z != nullptr ? a->ldz : 2 * (int64_t)a->F;

@@ -87,14 +87,10 @@ __device__ __forceinline__ void wide_dma(const char* src, unsigned lds) {
 
 // `left`: k rows from the tile's first to K (<= 0: behind the end).  What is outside A or B comes from the zero piece.
 template <int BK, bool COL, bool GATED>
-__device__ __forceinline__ void wide_issue(WideSource<BK, COL, GATED>& s, unsigned lds, int left, int wave) {
+__device__ __forceinline__ void wide_issue(WideSource<BK, COL, GATED>& s, int j, unsigned lds, int left, int wave) {
     const char* zero = reinterpret_cast<const char*>(g_wide_zero);
-#pragma unroll
-    for (int j = 0; j < WideSource<BK, COL, GATED>::DMA; ++j) {
-        const char* src = s.kk[j] < left ? s.p[j] : zero;
-        wide_dma(src, lds + (unsigned)(j * 8 + wave) * 1024);
-        s.p[j] += s.step;
-    }
+    wide_dma(s.kk[j] < left ? s.p[j] : zero, lds + (unsigned)(j * 8 + wave) * 1024);
+    s.p[j] += s.step;
 }
 
 // Fragments of one 16-deep step.  ROW: 16-byte LDS reads.  COL: transposed reads, issued and waited for in one asm block (a read in
@@ -146,13 +142,15 @@ __device__ __forceinline__ void wide_tile(const WideGemm& g, char* lds, int m0, 
     sb.init(g.b, n0, g.N, g.F, wave, lane);
     const int nk = (g.K + BK - 1) / BK;
     const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds);
-    auto issue = [&](int kt) {
+    auto issue = [&](int kt, int j) {
         const unsigned st = lds0 + (unsigned)(kt & (NS - 1)) * STAGE;
-        wide_issue(sa, st, g.K - kt * BK, wave);
-        wide_issue(sb, st + HALF, g.K - kt * BK, wave);
+        wide_issue(sa, j, st, g.K - kt * BK, wave);
+        wide_issue(sb, j, st + HALF, g.K - kt * BK, wave);
     };
 #pragma unroll
-    for (int t = 0; t < NS - 1; ++t) issue(t);
+    for (int t = 0; t < NS - 1; ++t)
+#pragma unroll
+        for (int j = 0; j < BK / 16; ++j) issue(t, j);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -214,24 +212,31 @@ __device__ __forceinline__ void wide_tile(const WideGemm& g, char* lds, int m0, 
                 else { if (!row) wide_read_col<ks * 16 * 512>(xb, b[ks & 1]); }
             }
         };
-        auto products = [&](int ks) {
+        auto products = [&](int ks, int i0, int i1) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = i0; i < i1; ++i)
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
                     acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a[ks & 1][i]), __builtin_bit_cast(bf16x8, b[ks & 1][j]), acc[i][j], 0, 0, 0);
         };
+        // the next tile's requests go between the products of the first steps, a pair at a time: all of them at once would fill the
+        // memory pipe's queue and hold the wave (behind the last tile they fetch zero pieces, so that the wait's count holds)
         auto step = [&](auto next) {
+            constexpr int ks = decltype(next)::value - 1;
             read(next, true);
-            products(decltype(next)::value - 1);
+            products(ks, 0, 2);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (ks < 2) {
+#pragma unroll
+                for (int j = 0; j < BK / 32; ++j) issue(kt + NS - 1, ks * (BK / 32) + j);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            products(ks, 2, 4);
             __builtin_amdgcn_sched_barrier(0);
             read(next, false);
             __builtin_amdgcn_sched_barrier(0);
         };
         read(std::integral_constant<int, 0>{}, true);
-        __builtin_amdgcn_sched_barrier(0);
-        issue(kt + NS - 1);      // beside the first reads; behind the last tile: zero pieces, so that the wait's count holds
-        __builtin_amdgcn_sched_barrier(0);
         read(std::integral_constant<int, 0>{}, false);
         step(std::integral_constant<int, 1>{});
         step(std::integral_constant<int, 2>{});

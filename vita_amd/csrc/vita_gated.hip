@@ -28,26 +28,46 @@ __global__ __launch_bounds__(256) void gated_product_kernel(const float* z, int6
     for (int j = 0; j < 4; ++j) o[j] = (T)(apply_act(g[j], act) * u[j]);
 }
 
-constexpr int kDzRows = 64;      // rows of one partial sum of the bias gradient
+// dz and the partial sums of db: a workgroup has 256 features and kDzRows rows, a thread 4 features of every 4th row; 16-byte accesses
+constexpr int kDzRows = 32;
 template <class T>
 __global__ __launch_bounds__(256) void gated_dz_kernel(const float* z, int64_t ldz, const T* dh, int64_t ld_dh, T* dz, int64_t ld_dz, float* db_part, int M,
-                                                       int F, int act) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= F) return;
-    const int r0 = blockIdx.y * kDzRows, r1 = min(M, r0 + kDzRows);
-    float sg = 0.f, su = 0.f;
-    for (int r = r0; r < r1; ++r) {
-        const float g = z[(int64_t)r * ldz + c], u = z[(int64_t)r * ldz + F + c], d = (float)dh[(int64_t)r * ld_dh + c];
-        const float dg = d * u * act_grad(g, act), du = d * apply_act(g, act);
-        dz[(int64_t)r * ld_dz + c] = (T)dg;
-        dz[(int64_t)r * ld_dz + F + c] = (T)du;
-        sg += dg;
-        su += du;
+                                                       int F, int act, int64_t segs) {
+    typedef T vec4 __attribute__((ext_vector_type(4)));
+    __shared__ float part[4][2][256];
+    const int lane = threadIdx.x & 63, y = threadIdx.x >> 6, blocks = (F + 255) / 256;
+    const int64_t seg = blockIdx.x / blocks;
+    const int c = (int)(blockIdx.x - seg * blocks) * 256 + lane * 4;
+    const int64_t r0 = seg * kDzRows, r1 = min((int64_t)M, r0 + kDzRows);
+    f32x4 sg = {0.f, 0.f, 0.f, 0.f}, su = sg;
+    if (c < F)
+        for (int64_t r = r0 + y; r < r1; r += 4) {
+            const f32x4 g = *reinterpret_cast<const f32x4*>(z + r * ldz + c), u = *reinterpret_cast<const f32x4*>(z + r * ldz + F + c);
+            const vec4 d = *reinterpret_cast<const vec4*>(dh + r * ld_dh + c);
+            vec4 og, ou;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float dg = (float)d[j] * u[j] * act_grad(g[j], act), du = (float)d[j] * apply_act(g[j], act);
+                og[j] = (T)dg;
+                ou[j] = (T)du;
+                sg[j] += dg;
+                su[j] += du;
+            }
+            *reinterpret_cast<vec4*>(dz + r * ld_dz + c) = og;
+            *reinterpret_cast<vec4*>(dz + r * ld_dz + F + c) = ou;
+        }
+    if (db_part == nullptr) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        part[y][0][lane * 4 + j] = sg[j];
+        part[y][1][lane * 4 + j] = su[j];
     }
-    if (db_part != nullptr) {
-        db_part[(int64_t)blockIdx.y * 2 * F + c] = sg;
-        db_part[(int64_t)blockIdx.y * 2 * F + F + c] = su;
-    }
+    __syncthreads();
+    const int f = (int)(blockIdx.x - seg * blocks) * 256 + threadIdx.x;
+    if (f < F)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            db_part[seg * 2 * F + k * F + f] = (part[0][k][threadIdx.x] + part[1][k][threadIdx.x]) + (part[2][k][threadIdx.x] + part[3][k][threadIdx.x]);
 }
 
 // (rows, cols) -> (cols, rows) of 16-bit elements
@@ -76,6 +96,27 @@ struct WideOut {
     float* db_part;                       // (tiles_m, 2 F)
 };
 enum { WIDE_H = 0, WIDE_DZ = 1, WIDE_C = 2 };
+
+// act(z), and its slope where SLOPE, on the hardware's exp2 and reciprocal (one unit in the last place each; the results are rounded to
+// bf16, and the sums for db are within 1e-6 of 64 bits).  The library's forms divide and range-reduce: they cost the dz product's epilogue
+// a seventh of the kernel.
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ void wide_act(float z, float& a, float& slope) {
+    if constexpr (ACT == VITA_ACT_SILU) {
+        const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));      // z -> -inf: rcp(inf) = 0
+        a = z * s;
+        if constexpr (SLOPE) slope = fmaf(a, 1.0f - s, s);
+    } else if constexpr (ACT == VITA_ACT_GELU_TANH && SLOPE) {
+        // 0.5 (1 + tanh(u)) = s with s = 1 / (1 + exp(-2 u)); a = z s; a' = s + 2 z s (1 - s) u'
+        const float c0 = -2.8853900817779268f * 0.7978845608028654f, c1 = c0 * 0.044715f, z2 = z * z;
+        const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * fmaf(z2, c1, c0)));
+        a = z * s;
+        slope = fmaf(a * (1.0f - s), fmaf(z2, 2.0f * 0.7978845608028654f * 3.0f * 0.044715f, 2.0f * 0.7978845608028654f), s);
+    } else {
+        a = apply_act_t<ACT>(z);
+        if constexpr (SLOPE) slope = act_grad(z, ACT);
+    }
+}
 
 // EPI WIDE_H: h (M, F) of a gated product; WIDE_DZ: dz (M, 2F) of a gated product; WIDE_C: plain C (M, N)
 template <bool ACOL, bool BCOL, int EPI, int ACT>
@@ -132,11 +173,13 @@ __global__ __launch_bounds__(WNT, 2) void wide_gemm_kernel(WideGemm g, WideOut o
         for (int r = 0; r < 16; ++r) {
             const int at = (wm * 128 + i * 32 + (r >> 2) * 8 + half * 4 + (r & 3)) * LD + wn * 32 + col;
             const float zg = acc[i][0][r] + bg, zu = acc[i][1][r] + bu;
+            float a, slope;
+            wide_act<ACT, EPI == WIDE_DZ>(zg, a, slope);
             if constexpr (EPI == WIDE_H) {
-                t[at] = (bf16)(apply_act_t<ACT>(zg) * zu);
+                t[at] = (bf16)(a * zu);
             } else {
                 const float d = (float)t[at];
-                const float dg = d * zu * act_grad(zg, ACT), du = d * apply_act_t<ACT>(zg);
+                const float dg = d * zu * slope, du = d * a;
                 t[at] = (bf16)dg;
                 tu[at] = (bf16)du;
                 sg += dg;
@@ -180,7 +223,7 @@ template <bool ACOL, bool BCOL, int EPI, int ACT = VITA_ACT_NONE>
 int launch_wide(const bf16* A, int64_t lda, const bf16* B, int64_t ldb, int M, int N, int K, int F, const WideOut& o, hipStream_t s) {
     WideGemm g{{A, lda}, {B, ldb}, M, N, K, (M + WBM - 1) / WBM, 0, F};
     g.tiles_n = EPI == WIDE_C ? (N + WBN - 1) / WBN : (F + WBN / 2 - 1) / (WBN / 2);
-    hipLaunchKernelGGL((wide_gemm_kernel<ACOL, BCOL, EPI, ACT>), dim3((unsigned)(g.tiles_m * g.tiles_n)), dim3(WNT), WLDS, s, g, o);
+    hipLaunchKernelGGL((wide_gemm_kernel<ACOL, BCOL, EPI, ACT>), dim3((unsigned)(g.tiles_m * g.tiles_n)), dim3(WNT), wide_stages(ACOL, BCOL) * WSTAGE, s, g, o);
     VITA_CHECK_HIP(hipGetLastError());
     return VITA_OK;
 }
@@ -241,6 +284,9 @@ Ws carve(const vita_gated_args* a, bool bwd, void* ws) {
         r.dz = c.take((M * F2 * es + 3) / 4);
         if (a->dtype == VITA_DT_BF16 && a->dw != nullptr && !wide_fills(F2, K)) r.dw32 = c.take(F2 * K);
         if (a->dtype == VITA_DT_BF16 && a->dx != nullptr && !wide_fills(M, K)) r.wt = c.take((F2 * K * es + 3) / 4);
+        // fp32 dx: W transposed once lets the product take the row-operand GEMM (2176 x 512 x 4096: 162 us on W as it lies), from as many
+        // rows as the training step does so; the transpose wants W without gaps
+        if (a->dtype == VITA_DT_F32 && a->dx != nullptr && a->M >= kWtMinRows && a->ldw == a->K) r.wt = c.take(F2 * K);
         const size_t segs = (M + kDzRows - 1) / kDzRows;
         r.db_part = c.take(segs * F2);
         r.cs = c.take((size_t)vita_colsum_partials_count((int32_t)F2));
@@ -274,21 +320,28 @@ int run_bwd(const vita_gated_args* a, void* workspace, hipStream_t s) {
     }
     float* part = a->db != nullptr ? ws.db_part : nullptr;
     int segs = (M + kDzRows - 1) / kDzRows;
-    const dim3 grid((F + 255) / 256, segs);
+    const int64_t blocks = (int64_t)segs * ((F + 255) / 256);
+    VITA_REQUIRE(blocks < (int64_t(1) << 31), "vita_gated_linear_bwd: too many elements");
+    const dim3 grid((unsigned)blocks);
     if (wide) {
         WideOut o{};
         o.bias = a->b; o.dh = (const bf16*)a->dh; o.ld_dh = a->ld_dh; o.dz = (bf16*)ws.dz; o.ld_dz = F2; o.db_part = part;
         VITA_TRY(launch_wide_gated<WIDE_DZ>(a, o, s));
         segs = (M + WBM - 1) / WBM;
     } else if (a->dtype == VITA_DT_F32)
-        hipLaunchKernelGGL(gated_dz_kernel<float>, grid, dim3(256), 0, s, z, ldz, (const float*)a->dh, a->ld_dh, (float*)ws.dz, F2, part, M, F, a->act);
+        hipLaunchKernelGGL(gated_dz_kernel<float>, grid, dim3(256), 0, s, z, ldz, (const float*)a->dh, a->ld_dh, (float*)ws.dz, F2, part, M, F, a->act, (int64_t)segs);
     else
-        hipLaunchKernelGGL(gated_dz_kernel<bf16>, grid, dim3(256), 0, s, z, ldz, (const bf16*)a->dh, a->ld_dh, (bf16*)ws.dz, F2, part, M, F, a->act);
+        hipLaunchKernelGGL(gated_dz_kernel<bf16>, grid, dim3(256), 0, s, z, ldz, (const bf16*)a->dh, a->ld_dh, (bf16*)ws.dz, F2, part, M, F, a->act, (int64_t)segs);
     VITA_CHECK_HIP(hipGetLastError());
     if (a->db != nullptr) VITA_TRY(vita_colsum_f32(part, F2, segs, F2, ws.cs, a->db, 0, s));
     SplitkScope sk(ws.sk, kSplitkBytes);
     if (a->dtype == VITA_DT_F32) {
-        if (a->dx != nullptr) VITA_TRY(gemm_f32(dgrad((const float*)ws.dz, F2, (const float*)a->w, a->ldw, (float*)a->dx, a->ld_dx, M, K, F2), s));
+        if (a->dx != nullptr && ws.wt != nullptr) {
+            VITA_TRY(launch_transpose_f32((const float*)a->w, F2, K, (float*)ws.wt, s));
+            VITA_TRY(gemm_f32(lin((const float*)ws.dz, F2, (const float*)ws.wt, F2, nullptr, (float*)a->dx, a->ld_dx, M, K, F2, VITA_ACT_NONE), s));
+        } else if (a->dx != nullptr) {
+            VITA_TRY(gemm_f32(dgrad((const float*)ws.dz, F2, (const float*)a->w, a->ldw, (float*)a->dx, a->ld_dx, M, K, F2), s));
+        }
         if (a->dw != nullptr) VITA_TRY(gemm_f32(wgrad((const float*)ws.dz, F2, (const float*)a->x, a->ldx, (float*)a->dw, a->ld_dw, M, K, F2), s));
         return VITA_OK;
     }

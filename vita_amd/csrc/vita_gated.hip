@@ -6,6 +6,7 @@
 // dx = dz W and dw = dz^T x on the operands as they lie.  Forming z again costs 2 of 8 products but keeps nothing between the passes:
 // saved in bf16 it would round the slopes' arguments, saved in fp32 it would move 4 M F bytes twice.  dz is rounded to bf16 because the
 // matrix unit takes bf16 operands; db is summed before that rounding.
+// Up to 64 bf16 rows: a kernel of its own, bound by reading the weights once.
 // Everything else goes over z (M, 2F) in fp32 with the library's GEMMs and one elementwise pass: fp32 (where the product runs at a
 // sixteenth of the rate and saving z is the cheap choice) and small bf16 calls.
 #include <type_traits>
@@ -227,12 +228,9 @@ int launch_wide(const bf16* A, int64_t lda, const bf16* B, int64_t ldb, int M, i
     VITA_CHECK_HIP(hipGetLastError());
     return VITA_OK;
 }
-template <int EPI>
-int launch_wide_gated(const vita_gated_args* a, const WideOut& o, hipStream_t s) {
-    auto go = [&](auto act) {
-        return launch_wide<false, false, EPI, decltype(act)::value>((const bf16*)a->x, a->ldx, (const bf16*)a->w, a->ldw, a->M, 2 * a->F, a->K, a->F, o, s);
-    };
-    switch (a->act) {
+template <class Go>
+int by_act(int act, Go go) {
+    switch (act) {
         case VITA_ACT_RELU: return go(std::integral_constant<int, VITA_ACT_RELU>{});
         case VITA_ACT_GELU_ERF: return go(std::integral_constant<int, VITA_ACT_GELU_ERF>{});
         case VITA_ACT_GELU_TANH: return go(std::integral_constant<int, VITA_ACT_GELU_TANH>{});
@@ -240,10 +238,108 @@ int launch_wide_gated(const vita_gated_args* a, const WideOut& o, hipStream_t s)
         default: return go(std::integral_constant<int, VITA_ACT_MISH>{});
     }
 }
+template <int EPI>
+int launch_wide_gated(const vita_gated_args* a, const WideOut& o, hipStream_t s) {
+    auto go = [&](auto act) {
+        return launch_wide<false, false, EPI, decltype(act)::value>((const bf16*)a->x, a->ldx, (const bf16*)a->w, a->ldw, a->M, 2 * a->F, a->K, a->F, o, s);
+    };
+    return by_act(a->act, go);
+}
 // whether a C of M x N has enough 256 x 256 tiles to keep the 256 CUs busy
 bool wide_fills(int64_t M, int64_t N) {
     const int64_t t = ((M + WBM - 1) / WBM) * ((N + WBN - 1) / WBN);
     return t >= 192 && t < (int64_t(1) << 31);
+}
+
+// ---- few rows, bf16 ---------------------------------------------------------------------------------------------------------------
+// h of up to 64 rows: bound by reading the weights once.  A workgroup has 16 features (their 16 gate and 16 up rows of W), its 8 waves an
+// eighth of k each; a wave's fragments of v_mfma_f32_16x16x32_bf16 come straight from memory, 64 bytes of a row to a load (32 x 32 tiles
+// would take 32: 18.6 against 18.2 us for 25 x 2048 x 8192, 67 MB of weights, 3.7 TB/s), those of U steps in flight together, x from the caches;
+// the waves' sums meet in LDS in wave order.  RB: blocks of 16 rows.
+template <int ACT, int RB>
+__global__ __launch_bounds__(512, 4) void gated_few_rows_kernel(const bf16* x, int64_t ldx, const bf16* w, int64_t ldw, const float* bias, bf16* h, int64_t ldh,
+                                                                int M, int F, int K) {
+    constexpr int U = RB <= 2 ? 4 : 2;
+    __shared__ float part[8][2][4 * 64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, quad = lane >> 4;
+    const int f = blockIdx.x * 16 + col;
+    const bool in = f < F;
+    const bf16* wg = w + (int64_t)(in ? f : 0) * ldw + quad * 8;
+    const bf16* wu = w + ((int64_t)(in ? f : 0) + F) * ldw + quad * 8;
+    const bf16* xr[RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) xr[b] = x + (int64_t)min(b * 16 + col, M - 1) * ldx + quad * 8;
+    f32x4 g[RB], u[RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) { g[b][r] = 0.f; u[b][r] = 0.f; }
+    const bf16x8 zero = {};
+    const int steps = (K + 31) / 32, per = (steps + 7) / 8, s0 = wave * per, s1 = min(steps, s0 + per);
+    for (int s = s0; s < s1; s += U) {
+        bf16x8 a[U][RB], bg[U], bu[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int k = (s + j) * 32;
+            const bool ok = s + j < s1 && k + quad * 8 < K;
+            bg[j] = ok ? *reinterpret_cast<const bf16x8*>(wg + k) : zero;
+            bu[j] = ok ? *reinterpret_cast<const bf16x8*>(wu + k) : zero;
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int k = (s + j) * 32;
+            const bool ok = s + j < s1 && k + quad * 8 < K;
+#pragma unroll
+            for (int b = 0; b < RB; ++b) a[j][b] = ok ? *reinterpret_cast<const bf16x8*>(xr[b] + k) : zero;
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+#pragma unroll
+            for (int b = 0; b < RB; ++b) {
+                g[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[j][b], bg[j], g[b], 0, 0, 0);
+                u[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[j][b], bu[j], u[b], 0, 0, 0);
+            }
+    }
+    const float b0 = bias != nullptr && in ? bias[f] : 0.f, b1 = bias != nullptr && in ? bias[F + f] : 0.f;
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        if (b > 0) __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            part[wave][0][r * 64 + lane] = g[b][r];
+            part[wave][1][r * 64 + lane] = u[b][r];
+        }
+        __syncthreads();
+        if (wave < 4) {                                    // a wave finishes one of the 4 accumulator rows
+            const int row = b * 16 + quad * 4 + wave;
+            float zg = b0, zu = b1;
+#pragma unroll
+            for (int v = 0; v < 8; ++v) {
+                zg += part[v][0][wave * 64 + lane];
+                zu += part[v][1][wave * 64 + lane];
+            }
+            float act, slope;
+            wide_act<ACT, false>(zg, act, slope);
+            if (in && row < M) h[(int64_t)row * ldh + f] = (bf16)(act * zu);
+        }
+    }
+}
+constexpr int kFewRows = 64;
+int launch_few_rows(const vita_gated_args* a, hipStream_t s) {
+    auto go = [&](auto act) -> int {
+        constexpr int ACT = decltype(act)::value;
+        const dim3 grid((a->F + 15) / 16);
+        auto launch = [&](auto rb) {
+            hipLaunchKernelGGL((gated_few_rows_kernel<ACT, decltype(rb)::value>), grid, dim3(512), 0, s, (const bf16*)a->x, a->ldx, (const bf16*)a->w, a->ldw, a->b,
+                               (bf16*)a->h, a->ldh, a->M, a->F, a->K);
+        };
+        if (a->M <= 16) launch(std::integral_constant<int, 1>{});
+        else if (a->M <= 32) launch(std::integral_constant<int, 2>{});
+        else launch(std::integral_constant<int, 4>{});
+        VITA_CHECK_HIP(hipGetLastError());
+        return VITA_OK;
+    };
+    return by_act(a->act, go);
 }
 
 int check(const vita_gated_args* a, bool bwd, const char* who) {
@@ -271,12 +367,16 @@ int check(const vita_gated_args* a, bool bwd, const char* who) {
 // bf16 products whose z is not given and whose tiles fill the chip
 bool wide_product(const vita_gated_args* a) { return a->dtype == VITA_DT_BF16 && a->z == nullptr && wide_fills(a->M, 2 * (int64_t)a->F); }
 
+// a forward call that the few-row kernel takes (z wanted: the general path, which writes it)
+bool few_rows(const vita_gated_args* a) { return a->dtype == VITA_DT_BF16 && a->z == nullptr && a->M <= kFewRows; }
+
 struct Ws { float* sk; float* z; void* dz; float* dw32; void* wt; float* db_part; float* cs; size_t bytes; };
 Ws carve(const vita_gated_args* a, bool bwd, void* ws) {
     Carver c(ws);
     Ws r{};
     const size_t M = a->M, F2 = 2 * (size_t)a->F, K = a->K;
     const bool wide = wide_product(a);
+    if (!bwd && few_rows(a)) return r;
     if (bwd || !wide) r.sk = c.take(kSplitkBytes / 4);
     if (a->z == nullptr && !wide) r.z = c.take(M * F2);
     if (bwd) {
@@ -293,6 +393,20 @@ Ws carve(const vita_gated_args* a, bool bwd, void* ws) {
     }
     r.bytes = c.off;
     return r;
+}
+
+// Parts of dx's long reduction (2 F): the product's 64 x 128 tiles go over the 256 CUs in whole rounds, so S parts take
+// ceil(tiles S / 256) / S rounds, and each part costs the sum of partial results about 2 % of one.  2176 x 512 x 4096: 136 tiles, 1 part
+// 141 us, 5 parts 115 us.
+int dx_splits(int M, int K, int F2) {
+    const long tiles = (long)((M + 63) / 64) * ((K + 127) / 128);
+    int best = 1;
+    double cost = 1e30;
+    for (int S = 1; S <= 8 && F2 / S >= 512; ++S) {
+        const double c = (double)((tiles * S + 255) / 256) / S + 0.02 * S;
+        if (c < cost) { cost = c; best = S; }
+    }
+    return best;
 }
 
 // z = x w^T + b (fp32)
@@ -338,7 +452,8 @@ int run_bwd(const vita_gated_args* a, void* workspace, hipStream_t s) {
     if (a->dtype == VITA_DT_F32) {
         if (a->dx != nullptr && ws.wt != nullptr) {
             VITA_TRY(launch_transpose_f32((const float*)a->w, F2, K, (float*)ws.wt, s));
-            VITA_TRY(gemm_f32(lin((const float*)ws.dz, F2, (const float*)ws.wt, F2, nullptr, (float*)a->dx, a->ld_dx, M, K, F2, VITA_ACT_NONE), s));
+            VITA_TRY(gemm_f32_rows_split(lin((const float*)ws.dz, F2, (const float*)ws.wt, F2, nullptr, (float*)a->dx, a->ld_dx, M, K, F2, VITA_ACT_NONE),
+                                         dx_splits(M, K, F2), s));
         } else if (a->dx != nullptr) {
             VITA_TRY(gemm_f32(dgrad((const float*)ws.dz, F2, (const float*)a->w, a->ldw, (float*)a->dx, a->ld_dx, M, K, F2), s));
         }
@@ -388,6 +503,7 @@ int vita_gated_linear(const vita_gated_args* a, void* workspace, size_t workspac
     if (a->M == 0) return VITA_OK;
     VITA_TRY(check_ws(workspace, workspace_bytes, vita_gated_linear_workspace_bytes(a), who));
     hipStream_t s = (hipStream_t)stream;
+    if (few_rows(a)) return launch_few_rows(a, s);
     if (wide_product(a)) {
         WideOut o{};
         o.bias = a->b; o.c = (bf16*)a->h; o.ldc = a->ldh;

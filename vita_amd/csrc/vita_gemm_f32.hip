@@ -659,6 +659,20 @@ int gemm_f32_wgrad_pair(const vita_linear_args& a0, const vita_linear_args& a1, 
     return gemm_f32_wgrad_batch(a, 2, stream);
 }
 
+int gemm_f32_rows_split(const vita_linear_args& a, int splits, hipStream_t stream) {
+    VITA_REQUIRE(gemm_f32_dma_eligible(a) && a.pro == VITA_PRO_NONE && !a.a_col && !a.b_col && a.splitk_ws != nullptr, "gemm_f32_rows_split: not a row-operand call");
+    SplitK sk;
+    int kps = (a.K + splits - 1) / splits;
+    kps = (kps + SPLITK_MIN_K - 1) / SPLITK_MIN_K * SPLITK_MIN_K;
+    sk.splits = (a.K + kps - 1) / kps;
+    sk.k_per_split = kps;
+    sk.ld_partial = ((int64_t)a.N + 3) & ~int64_t(3);
+    sk.partial = static_cast<float*>(a.splitk_ws);
+    if (sk.splits < 2 || (size_t)sk.splits * a.M * sk.ld_partial * sizeof(float) > a.splitk_ws_bytes) return gemm_f32(a, stream);
+    VITA_TRY_RC(gemm_f32_dma(a, stream, &sk));
+    return launch_splitk_reduce(epi_of(a), sk.partial, sk.ld_partial, sk.splits, stream);
+}
+
 int gemm_f32(const vita_linear_args& a, hipStream_t stream) {
     if (a.M == 0 && a.N > 0 && a.K > 0) return VITA_OK;  // empty batch: nothing to do (pointers may be null)
     VITA_REQUIRE(a.X && a.W && a.Y, "vita_linear_f32: X, W and Y must be non-null");

@@ -5,6 +5,7 @@ libvita_hip.so.  Nothing here falls back to torch math.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
 from typing import Mapping, Optional
@@ -1402,8 +1403,16 @@ def _param(t: Optional[Tensor], what: str, shape: tuple, device) -> Optional[Ten
 
 def _aligned(t: Tensor) -> bool:
     """Unit inner stride, and every row on a 16-byte border."""
-    es = t.element_size()
-    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or s * es % 16 == 0 for n, s in zip(t.shape[:-1], t.stride()[:-1]))
+    unit = 16 // t.element_size()
+    if t.data_ptr() % 16:
+        return False
+    *lead, last = t.stride()
+    if last != 1:
+        return False
+    for n, s in zip(t.shape, lead):
+        if s % unit and n != 1:
+            return False
+    return True
 
 
 def _aligned_rows(t: Tensor) -> Tensor:
@@ -1428,76 +1437,69 @@ def _scratch(nbytes: int, device) -> Optional[Tensor]:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
-class _On:
+_here = contextlib.nullcontext()
+
+
+def _On(device):
     """Launches go to the tensor's device whatever the current one is."""
-
-    def __init__(self, device):
-        self.guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+    return _here if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
-def _set4(a, name: str, t: Tensor) -> None:
+def _raw_stream(device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _bshd(t: Tensor) -> tuple:
     """Pointer and batch / token / head strides of a (B, S, H, D) tensor; a stride that is never walked is 0."""
-    s = t.stride()
-    n = t.shape
-    setattr(a, name, t.data_ptr())
-    setattr(a, name + "_sb", s[0] if n[0] > 1 else 0)
-    setattr(a, name + "_ss", s[1] if n[1] > 1 else 0)
-    setattr(a, name + "_sh", s[2] if n[2] > 1 else 0)
+    n0, n1, n2, _ = t.shape
+    s0, s1, s2, _ = t.stride()
+    return t.data_ptr(), s0 if n0 > 1 else 0, s1 if n1 > 1 else 0, s2 if n2 > 1 else 0
+
+
+def _ptr(t: Optional[Tensor]) -> Optional[int]:
+    return t.data_ptr() if t is not None else None
+
+
+_NO_TENSOR = (None, 0, 0, 0)
 
 
 def _norm_rope_args(q, k, rope, q_weight, q_bias, k_weight, k_bias, norm, eps, positions, who):
+    """Checks, and what both passes pass on: the scalars of vita_norm_rope_args, (x, weight, bias) of q and of k."""
     _act(q, f"{who}: q", 4)
     _act(k, f"{who}: k", 4, q)
+    dev = q.device
     B, S, H, D = q.shape
     Hk = k.shape[2]
-    if tuple(k.shape) != (B, S, Hk, D):
+    if k.shape[0] != B or k.shape[1] != S or k.shape[3] != D:
         raise L.VitaHipError(f"{who}: q {tuple(q.shape)} and k {tuple(k.shape)} differ in more than their heads")
     if norm not in _NORMS:
         raise L.VitaHipError(f"{who}: norm {norm!r}, expected one of {sorted(_NORMS)}")
     _f32(rope, f"{who}: rope")
-    if rope.dim() != 3 or rope.shape[2] != 2 or rope.device != q.device or D % 2 or rope.shape[1] not in (D // 2, H * D // 2):
-        raise L.VitaHipError(f"{who}: rope {tuple(rope.shape)} on {rope.device}, expected (positions, {D // 2} or {H * D // 2}, 2) on {q.device}")
-    keep = [rope.contiguous()]
-    a = L.NormRopeArgs()
-    a.dtype, a.norm, a.B, a.S, a.D, a.eps = _DT[q.dtype], _NORMS[norm], B, S, D, float(eps)
-    a.rope, a.rope_rows, a.rope_heads = keep[0].data_ptr(), rope.shape[0], rope.shape[1] // (D // 2)
+    if rope.dim() != 3 or rope.shape[2] != 2 or rope.device != dev or D % 2 or rope.shape[1] not in (D // 2, H * D // 2):
+        raise L.VitaHipError(f"{who}: rope {tuple(rope.shape)} on {rope.device}, expected (positions, {D // 2} or {H * D // 2}, 2) on {dev}")
+    rope = rope.contiguous()
+    ld = 0
     if positions is not None:
-        if positions.dtype != torch.int64 or positions.device != q.device or tuple(positions.shape) not in ((S,), (B, S)):
-            raise L.VitaHipError(f"{who}: positions {positions.dtype} {tuple(positions.shape)} on {positions.device}, expected int64 ({S},) or ({B}, {S}) on {q.device}")
-        p = positions if positions.dim() == 2 else positions[None]
-        if S > 1 and p.stride(1) != 1 or (p.shape[0] > 1 and 0 < p.stride(0) < S):
-            p = p.contiguous()
-        keep.append(p)
-        a.positions, a.ld_positions = p.data_ptr(), (p.stride(0) if p.shape[0] > 1 else 0)
-    for side, name, x, w, b in ((a.q, "q", q, q_weight, q_bias), (a.k, "k", k, k_weight, k_bias)):
-        side.H = x.shape[2]
-        if x.stride(3) != 1:
-            x = x.contiguous()
-            keep.append(x)
-        _set4(side, "x", x)
-        w, b = _param(w, f"{who}: {name}_weight", (D,), q.device), _param(b, f"{who}: {name}_bias", (D,), q.device)
-        keep += [w, b]
-        side.weight, side.bias = w.data_ptr() if w is not None else None, b.data_ptr() if b is not None else None
-    return a, keep
+        if positions.dtype != torch.int64 or positions.device != dev or tuple(positions.shape) not in ((S,), (1, S), (B, S)):
+            raise L.VitaHipError(f"{who}: positions {positions.dtype} {tuple(positions.shape)} on {positions.device}, expected int64 ({S},) or ({B}, {S}) on {dev}")
+        if S > 1 and positions.stride(-1) != 1 or (positions.dim() == 2 and positions.shape[0] > 1 and 0 < positions.stride(0) < S):
+            positions = positions.contiguous()
+        ld = positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
+    head = (_DT[q.dtype], _NORMS[norm], B, S, D, eps, rope.data_ptr(), rope.shape[0], rope.shape[1] // (D // 2), _ptr(positions), ld)
+    sides = tuple((x if x.stride(3) == 1 else x.contiguous(), _param(w, f"{who}: {n}_weight", (D,), dev), _param(b, f"{who}: {n}_bias", (D,), dev))
+                  for n, x, w, b in (("q", q, q_weight, q_bias), ("k", k, k_weight, k_bias)))
+    return head, sides, (rope, positions)
 
 
 def _qk_norm_rope(q, k, rope, q_weight, q_bias, k_weight, k_bias, norm, eps, positions, out):
-    a, keep = _norm_rope_args(q, k, rope, q_weight, q_bias, k_weight, k_bias, norm, eps, positions, "qk_norm_rope")
+    head, sides, keep = _norm_rope_args(q, k, rope, q_weight, q_bias, k_weight, k_bias, norm, eps, positions, "qk_norm_rope")
     qo, ko = out if out is not None else (None, None)
     qo, ko = _out(qo, "qk_norm_rope: out[0]", q.shape, q), _out(ko, "qk_norm_rope: out[1]", k.shape, k)
-    _set4(a.q, "y", qo)
-    _set4(a.k, "y", ko)
     if q.numel():
+        a = L.NormRopeArgs(*head, *(L.NormRopeSide(*_bshd(x), *_bshd(y), *_NO_TENSOR, _ptr(w), _ptr(b), None, None, x.shape[2])
+                                    for (x, w, b), y in zip(sides, (qo, ko))))
         with _On(q.device):
-            L.check(L.load().vita_qk_norm_rope(C.byref(a), _stream(q)), "vita_qk_norm_rope")
+            L.check(L.load().vita_qk_norm_rope(C.byref(a), _raw_stream(q.device)), "vita_qk_norm_rope")
     return qo, ko
 
 
@@ -1506,29 +1508,26 @@ def qk_norm_rope_bwd(dq: Tensor, dk: Tensor, q: Tensor, k: Tensor, rope: Tensor,
                      positions: Optional[Tensor] = None, out=None):
     """Backward of qk_norm_rope from the gradients of its results: (dq, dk, dq_weight, dq_bias, dk_weight, dk_bias) with respect to its
     inputs, None for a parameter that was not given.  out: a pair of tensors for the first two (may be the gradients passed in)."""
-    a, keep = _norm_rope_args(q, k, rope, q_weight, q_bias, k_weight, k_bias, norm, eps, positions, "qk_norm_rope_bwd")
+    head, sides, keep = _norm_rope_args(q, k, rope, q_weight, q_bias, k_weight, k_bias, norm, eps, positions, "qk_norm_rope_bwd")
     qo, ko = out if out is not None else (None, None)
     qo, ko = _out(qo, "qk_norm_rope_bwd: out[0]", q.shape, q), _out(ko, "qk_norm_rope_bwd: out[1]", k.shape, k)
-    grads = [torch.empty_like(p, memory_format=torch.contiguous_format) if p is not None else None for p in (q_weight, q_bias, k_weight, k_bias)]
-    for side, name, d, x, y, w, b in ((a.q, "dq", dq, q, qo, grads[0], grads[1]), (a.k, "dk", dk, k, ko, grads[2], grads[3])):
-        if tuple(d.shape) != tuple(x.shape):
+    grads = [torch.empty(p.shape, dtype=p.dtype, device=p.device) if p is not None else None for p in (q_weight, q_bias, k_weight, k_bias)]
+    for name, d, x in (("dq", dq, q), ("dk", dk, k)):
+        if d.shape != x.shape:
             raise L.VitaHipError(f"qk_norm_rope_bwd: {name} {tuple(d.shape)}, expected {tuple(x.shape)}")
         _act(d, f"qk_norm_rope_bwd: {name}", 4, q)
-        if d.stride(3) != 1:
-            d = d.contiguous()
-            keep.append(d)
-        _set4(side, "dy", d)
-        _set4(side, "y", y)
-        side.dweight, side.dbias = w.data_ptr() if w is not None else None, b.data_ptr() if b is not None else None
+    dq, dk = (d if d.stride(3) == 1 else d.contiguous() for d in (dq, dk))
     if q.numel() == 0:
         for t in grads:
             if t is not None:
                 t.zero_()
     else:
+        a = L.NormRopeArgs(*head, *(L.NormRopeSide(*_bshd(x), *_bshd(y), *_bshd(d), _ptr(w), _ptr(b), _ptr(gw), _ptr(gb), x.shape[2])
+                                    for (x, w, b), y, d, gw, gb in zip(sides, (qo, ko), (dq, dk), grads[0::2], grads[1::2])))
         lib = L.load()
         with _On(q.device):
             ws = _scratch(lib.vita_qk_norm_rope_bwd_workspace_bytes(C.byref(a)), q.device)
-            L.check(lib.vita_qk_norm_rope_bwd(C.byref(a), ws.data_ptr(), ws.numel(), _stream(q)), "vita_qk_norm_rope_bwd")
+            L.check(lib.vita_qk_norm_rope_bwd(C.byref(a), ws.data_ptr(), ws.numel(), _raw_stream(q.device)), "vita_qk_norm_rope_bwd")
     return (qo, ko, *grads)
 
 
@@ -1592,47 +1591,41 @@ def _attention_args(q, k, v, scale, causal, key_pad, table, buckets, who):
     if D % 8 or not 8 <= D <= 128:
         raise L.VitaHipError(f"{who}: head dimension {D}, expected a multiple of 8 up to 128")
     q, k, v = _aligned_rows(q), _aligned_rows(k), _aligned_rows(v)
-    keep = [q, k, v]
-    a = L.AttentionArgs()
-    a.dtype, a.B, a.H, a.Hk, a.Sq, a.Sk, a.D, a.causal = _DT[q.dtype], B, H, Hk, Sq, Sk, D, int(bool(causal))
-    a.scale = float(scale) if scale is not None else D ** -0.5
-    _set4(a, "q", q)
-    _set4(a, "k", k)
-    _set4(a, "v", v)
+    ld = 0
     if key_pad is not None:
         if key_pad.dtype not in (torch.bool, torch.uint8) or tuple(key_pad.shape) != (B, Sk) or key_pad.device != q.device:
             raise L.VitaHipError(f"{who}: key_pad {key_pad.dtype} {tuple(key_pad.shape)} on {key_pad.device}, expected bool or uint8 ({B}, {Sk}) on {q.device}")
         if Sk > 1 and key_pad.stride(1) != 1 or (B > 1 and 0 < key_pad.stride(0) < Sk):
             key_pad = key_pad.contiguous()
-        keep.append(key_pad)
-        a.key_pad, a.ld_pad = key_pad.data_ptr(), (key_pad.stride(0) if B > 1 else 0)
+        ld = key_pad.stride(0) if B > 1 else 0
     if (table is None) != (buckets is None):
         raise L.VitaHipError(f"{who}: the bias needs both table and buckets")
+    radius = nb = 0
     if table is not None:
         _act(table, f"{who}: table", 2, q)
         if table.shape[0] < 1 or table.shape[1] != H:
             raise L.VitaHipError(f"{who}: table {tuple(table.shape)}, expected (buckets, {H})")
-        if buckets.dtype != torch.int32 or buckets.dim() != 1 or buckets.numel() % 2 == 0 or buckets.device != q.device or buckets.numel() > 2049:
+        radius, nb = buckets.numel() // 2, table.shape[0]
+        if buckets.dtype != torch.int32 or buckets.dim() != 1 or buckets.numel() % 2 == 0 or buckets.device != q.device or radius > 1024:
             raise L.VitaHipError(f"{who}: buckets {buckets.dtype} {tuple(buckets.shape)} on {buckets.device}, expected int32, an odd number up to 2049, on {q.device}")
         table, buckets = table.contiguous(), buckets.contiguous()
-        keep += [table, buckets]
-        a.table, a.buckets, a.radius, a.num_buckets = table.data_ptr(), buckets.data_ptr(), buckets.numel() // 2, table.shape[0]
-    return a, keep
+    head = (_DT[q.dtype], B, H, Hk, Sq, Sk, D, 1 if causal else 0, scale if scale is not None else D ** -0.5, *_bshd(q), *_bshd(k), *_bshd(v))
+    tail = (_ptr(key_pad), ld, _ptr(table), _ptr(buckets), radius, nb)
+    return head, tail, (q, k, v, key_pad, table, buckets)
 
 
 def _attention(q, k, v, scale, causal, key_pad, table, buckets, need_lse, out):
-    a, keep = _attention_args(q, k, v, scale, causal, key_pad, table, buckets, "attention")
+    head, tail, keep = _attention_args(q, k, v, scale, causal, key_pad, table, buckets, "attention")
     o = _out(out, "attention: out", q.shape, q)
     stats = torch.empty((q.shape[0], q.shape[2], q.shape[1], 2), dtype=torch.float32, device=q.device) if need_lse else None
     if o.numel():
-        if not _aligned(o):
+        if out is not None and not _aligned(o):
             raise L.VitaHipError("attention: out needs 16-byte aligned rows")
-        _set4(a, "o", o)
-        a.stats = stats.data_ptr() if need_lse else None
+        a = L.AttentionArgs(*head, *_bshd(o), _ptr(stats), *tail)
         lib = L.load()
         with _On(q.device):
             ws = _scratch(lib.vita_attention_workspace_bytes(C.byref(a)), q.device)
-            L.check(lib.vita_attention(C.byref(a), ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, _stream(q)), "vita_attention")
+            L.check(lib.vita_attention(C.byref(a), _ptr(ws), ws.numel() if ws is not None else 0, _raw_stream(q.device)), "vita_attention")
     return o, stats
 
 
@@ -1640,7 +1633,7 @@ def attention_bwd(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, o: Tensor, stat
                   key_pad: Optional[Tensor] = None, table: Optional[Tensor] = None, buckets: Optional[Tensor] = None, need_dtable: bool = True, out=None):
     """Backward of attention from the gradient of its result, the result and its row statistics (need_lse=True): (dq, dk, dv, dtable), dtable None
     without a table.  out: tensors for the first three."""
-    a, keep = _attention_args(q, k, v, scale, causal, key_pad, table, buckets, "attention_bwd")
+    head, tail, keep = _attention_args(q, k, v, scale, causal, key_pad, table, buckets, "attention_bwd")
     for name, t in (("dout", dout), ("o", o)):
         _act(t, f"attention_bwd: {name}", 4, q)
         if t.shape != q.shape:
@@ -1653,20 +1646,18 @@ def attention_bwd(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, o: Tensor, stat
     dq, dk, dv = out if out is not None else (None, None, None)
     dq, dk, dv = (_out(t, f"attention_bwd: out[{i}]", x.shape, q) for i, (t, x) in enumerate(((dq, q), (dk, k), (dv, v))))
     dtable = torch.empty(table.shape, dtype=table.dtype, device=table.device) if table is not None and need_dtable else None
-    if not all(t.numel() == 0 or _aligned(t) for t in (dq, dk, dv)):
+    if out is not None and not all(t.numel() == 0 or _aligned(t) for t in (dq, dk, dv)):
         raise L.VitaHipError("attention_bwd: out needs 16-byte aligned rows")
     if q.numel() == 0 or k.numel() == 0:
         for t in (dq, dk, dv, dtable):
             if t is not None:
                 t.zero_()
         return dq, dk, dv, dtable
-    for name, t in (("o", o), ("dout", dout), ("dq", dq), ("dk", dk), ("dv", dv)):
-        _set4(a, name, t)
-    a.stats, a.dtable = stats.data_ptr(), dtable.data_ptr() if dtable is not None else None
+    a = L.AttentionArgs(*head, *_bshd(o), _ptr(stats), *tail, *_bshd(dout), *_bshd(dq), *_bshd(dk), *_bshd(dv), _ptr(dtable))
     lib = L.load()
     with _On(q.device):
         ws = _scratch(lib.vita_attention_bwd_workspace_bytes(C.byref(a)), q.device)
-        L.check(lib.vita_attention_bwd(C.byref(a), ws.data_ptr(), ws.numel(), _stream(q)), "vita_attention_bwd")
+        L.check(lib.vita_attention_bwd(C.byref(a), ws.data_ptr(), ws.numel(), _raw_stream(q.device)), "vita_attention_bwd")
     return dq, dk, dv, dtable
 
 
@@ -1719,9 +1710,7 @@ def _gated_args(x, w, b, act, who):
         raise L.VitaHipError(f"{who}: activation {act!r}, expected one of {sorted(_ACTS)}")
     b = _param(b, f"{who}: b", (2 * F,), x.device)
     x, w = _gated_rows(x), _gated_rows(w)
-    a = L.GatedArgs()
-    a.dtype, a.act, a.M, a.F, a.K = _DT[x.dtype], _ACTS[act], M, F, K
-    a.x, a.ldx, a.w, a.ldw, a.b = x.data_ptr(), _ld(x), w.data_ptr(), _ld(w), b.data_ptr() if b is not None else None
+    a = L.GatedArgs(_DT[x.dtype], _ACTS[act], M, F, K, x.data_ptr(), _ld(x), w.data_ptr(), _ld(w), _ptr(b))
     return a, (x, w, b), F
 
 
@@ -1735,7 +1724,7 @@ def _gated_linear(x, w, b, act, need_saved, out):
     # fp32 calls keep the pre-activations; bf16 calls form them again in the backward pass (vita_gated.hip)
     z = torch.empty((x.shape[0], 2 * F), dtype=torch.float32, device=x.device) if need_saved and x.dtype == torch.float32 else None
     if h.numel():
-        if not _aligned(h):
+        if out is not None and not _aligned(h):
             raise L.VitaHipError("gated_linear: out needs 16-byte aligned rows")
         a.h, a.ldh = h.data_ptr(), _ld(h)
         if z is not None:
@@ -1743,7 +1732,7 @@ def _gated_linear(x, w, b, act, need_saved, out):
         lib = L.load()
         with _On(x.device):
             ws = _scratch(lib.vita_gated_linear_workspace_bytes(C.byref(a)), x.device)
-            L.check(lib.vita_gated_linear(C.byref(a), ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, _stream(x)),
+            L.check(lib.vita_gated_linear(C.byref(a), ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, _raw_stream(x.device)),
                     "vita_gated_linear")
     return h, z
 
@@ -1777,7 +1766,7 @@ def gated_linear_bwd(dh: Tensor, x: Tensor, w: Tensor, b: Optional[Tensor], act:
     lib = L.load()
     with _On(x.device):
         ws = _scratch(lib.vita_gated_linear_bwd_workspace_bytes(C.byref(a)), x.device)
-        L.check(lib.vita_gated_linear_bwd(C.byref(a), ws.data_ptr(), ws.numel(), _stream(x)), "vita_gated_linear_bwd")
+        L.check(lib.vita_gated_linear_bwd(C.byref(a), ws.data_ptr(), ws.numel(), _raw_stream(x.device)), "vita_gated_linear_bwd")
     return dx, dw, db
 
 

@@ -705,10 +705,11 @@ int vita_qk_norm_rope_bwd(const vita_norm_rope_args* args, void* workspace, size
  *   exist (is_pad of the dataset's batches); whatever its k and v hold is not used.  A query that sees no key gives zeros.
  *   table (num_buckets, H) of the call's dtype, buckets int32 (2 radius + 1), radius <= 1024; table NULL = no bias.  An id outside
  *   [0, num_buckets) makes its scores NaN.
- *   D a multiple of 8, <= 128; tensors and their strides 16-byte aligned, token strides below 2^23 elements.  stats (B, H, Sq, 2) or
- *   NULL: what the backward pass needs of each row, a maximum M of its scores times log2 e and 1 / sum 2^(score log2 e - M), so that
- *   log sum exp = M ln 2 - ln(second); (0, 0) for a query without keys.  (Two numbers, because their log sum exp would lose the sum
- *   where a mask of the type's lowest value makes every score of a row huge.)
+ *   D a multiple of 8, <= 128; tensors and their strides 16-byte aligned, token strides below 2^23 elements.
+ *   stats: NULL, or what the backward pass needs of each row, (B, H, Sq, vita_attention_stats_row) fp32, 16-byte aligned: a maximum M of
+ *   its scores times log2 e and 1 / sum 2^(score log2 e - M), so that log sum exp = M ln 2 - ln(second), (0, 0) for a query without keys
+ *   (two numbers, because their log sum exp would lose the sum where a mask of the type's lowest value makes every score of a row
+ *   huge); behind them, in bf16 calls, what o lost when it was rounded.
  * Backward: dq, dk, dv (written), dtable (num_buckets, H) of the call's dtype (NULL = not wanted), from dout, o and stats; every sum
  * in a fixed order.
  * --------------------------------------------------------------------------------------- */
@@ -728,6 +729,7 @@ typedef struct vita_attention_args {
     void* dv; int64_t dv_sb, dv_ss, dv_sh;
     void* dtable;
 } vita_attention_args;
+int32_t vita_attention_stats_row(int32_t dtype, int32_t D);       /* floats: 2 (fp32) or 4 + D / 2 (bf16) */
 size_t vita_attention_workspace_bytes(const vita_attention_args* args);
 int vita_attention(const vita_attention_args* args, void* workspace, size_t workspace_bytes, vita_stream_t stream);
 size_t vita_attention_bwd_workspace_bytes(const vita_attention_args* args);

@@ -85,7 +85,7 @@ def test_attention_refuses(change, text):
 
 def test_attention_bwd_refuses():
     lib = L.load()
-    for change in (dict(stats=None), dict(stats=4 + (1 << 20)), dict(dout=None), dict(dq_ss=3), dict(dk=None), dict(dv=2 + (1 << 20)), dict(dtable=1 << 20)):
+    for change in (dict(stats=None), dict(stats=8 + (1 << 20)), dict(dout=None), dict(dq_ss=3), dict(dk=None), dict(dv=2 + (1 << 20)), dict(dtable=1 << 20)):
         a = _attention()
         for n, v in change.items():
             setattr(a, n, v)

@@ -144,7 +144,7 @@ def _attention_case(g, B, Sq, Sk, H, Hk, D, dtype, pad, R, nb=16):
 
 def _lse(stats):
     """log sum exp in 64 bits from the row statistics: m ln 2 - ln r, -inf for a row without keys."""
-    m, r = stats.double().cpu().unbind(-1)
+    m, r = stats[..., 0].double().cpu(), stats[..., 1].double().cpu()
     return torch.where(r == 0, -math.inf, m * math.log(2) - torch.log(torch.where(r == 0, 1.0, r)))
 
 
@@ -261,14 +261,17 @@ def test_attention_layouts(dtype):
         for a, b, c in ((head_major(q), head_major(k), head_major(v)), (q, kv[:, :, 0], kv[:, :, 1]), (off(q), off(k), off(v)),
                         (q.transpose(2, 3).contiguous().transpose(2, 3), k, v)):
             out = head_major(torch.empty_like(q))
-            assert ops.attention(a, b, c, out=out, **kw) is out
+            assert ops.attention(a, b, c, out=out, need_lse=True, **kw)[0] is out
             grads = (torch.full_like(kv, 7.0), head_major(torch.empty_like(q)))
             got = (out, lse, *ops.attention_bwd(do, a, b, c, out, lse, out=(grads[1], grads[0][:, :, 0], grads[0][:, :, 1]), **kw))
             assert all(torch.equal(x, y) for x, y in zip(got, want))
         wide = torch.zeros(B, 2 * Sk, dtype=torch.bool, device=DEV)
         wide[:, :Sk] = kw["key_pad"]
-        assert torch.equal(ops.attention(q, k, v, **dict(kw, key_pad=wide[:, :Sk])), want[0])
-        assert torch.equal(ops.attention(q, k, v, **dict(kw, key_pad=kw["key_pad"].to(torch.uint8) * 200)), want[0])
+        plain = ops.attention(q, k, v, **kw)
+        assert torch.equal(ops.attention(q, k, v, **dict(kw, key_pad=wide[:, :Sk])), plain)
+        assert torch.equal(ops.attention(q, k, v, **dict(kw, key_pad=kw["key_pad"].to(torch.uint8) * 200)), plain)
+        ref_o = ref.attention(q, k, v, **kw)
+        ref.assert_close(plain, ref_o[0], ref_o[1], "without statistics")
         one = kw["key_pad"][:1].expand(B, Sk)                                                # one mask for the batch
         assert torch.equal(ops.attention(q, k, v, **dict(kw, key_pad=one)), ops.attention(q, k, v, **dict(kw, key_pad=one.contiguous())))
 

@@ -283,6 +283,7 @@ SIGNATURES = {
     "vita_qk_norm_rope": (C.c_int, [C.POINTER(NormRopeArgs), c_fp]),
     "vita_qk_norm_rope_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(NormRopeArgs)]),
     "vita_qk_norm_rope_bwd": (C.c_int, [C.POINTER(NormRopeArgs), c_fp, C.c_size_t, c_fp]),
+    "vita_attention_stats_row": (C.c_int32, [C.c_int32, C.c_int32]),
     "vita_attention_workspace_bytes": (C.c_size_t, [C.POINTER(AttentionArgs)]),
     "vita_attention": (C.c_int, [C.POINTER(AttentionArgs), c_fp, C.c_size_t, c_fp]),
     "vita_attention_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(AttentionArgs)]),

@@ -25,7 +25,9 @@ struct AttnTensor { char* p; int64_t sb, ss, sh; };      // strides in elements
 
 struct AttnParams {
     AttnTensor q, k, v, o, dout, dq, dk, dv;
-    float2* stats;                   // (B, H, Sq): maximum of a row's scores times log2 e (0: no key), reciprocal of the sum of 2^(score - maximum) (0: no key)
+    float* stats;                    // (B, H, Sq, stats_row): maximum of a row's scores times log2 e (0: no key), reciprocal of the sum of
+                                     // 2^(score - maximum) (0: no key); bf16: two zeros, then D bf16, what o lost when it was rounded
+    int stats_row;
     float* delta;                    // backward: (B, H, Sq) in the workspace
     const uint8_t* pad; int64_t ld_pad;
     const void* table; const int32_t* buckets; int R, NB;
@@ -126,6 +128,13 @@ __device__ __forceinline__ Frag<T> pack8(const f32x16& s, int chunk) {
     Frag<T> f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) f.v[j] = (T)s[chunk * 8 + j];
+    return f;
+}
+// ... and what that rounding lost
+__device__ __forceinline__ Frag<bf16> pack8_rest(const f32x16& s, int chunk, const Frag<bf16>& hi) {
+    Frag<bf16> f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f.v[j] = (bf16)(s[chunk * 8 + j] - (float)hi.v[j]);
     return f;
 }
 
@@ -265,7 +274,8 @@ template <class T> __device__ __forceinline__ const T* at(const AttnTensor& t, i
 template <class T> __device__ __forceinline__ T* at_mut(const AttnTensor& t, int b, int64_t s, int h) {
     return reinterpret_cast<T*>(t.p) + b * t.sb + s * t.ss + h * t.sh;
 }
-// 4 consecutive columns of an output row
+__host__ __device__ constexpr int stats_row(bool bf, int D) { return bf ? 4 + D / 2 : 2; }
+// 4 consecutive columns of a result row, and of its stats row where the backward pass will want them
 template <class T>
 __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
     if constexpr (sizeof(T) == 2) {
@@ -274,6 +284,16 @@ __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d)
     } else {
         *reinterpret_cast<f32x4*>(p) = f32x4{a, b, c, d};
     }
+}
+
+// what bf16 leaves of 4 numbers, in bf16 again
+__device__ __forceinline__ void store_rest4(float* stats, int c, float a, float b, float d, float e) {
+    store4<bf16>(reinterpret_cast<bf16*>(stats + 4) + c, a - (float)(bf16)a, b - (float)(bf16)b, d - (float)(bf16)d, e - (float)(bf16)e);
+}
+template <class T>
+__device__ __forceinline__ void store_stats(float* stats, float m, float r) {
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<f32x4*>(stats) = f32x4{m, r, 0.f, 0.f};
+    else *reinterpret_cast<float2*>(stats) = make_float2(m, r);
 }
 
 int attention_check(const vita_attention_args* a, bool bwd, const char* who);

@@ -50,6 +50,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void a
     const int pos_lo = p.Sk - p.Sq + min(first_row, p.Sq - 1), pos_hi = p.Sk - p.Sq + min(first_row + 31, p.Sq - 1);
     const int wg_hi = p.Sk - p.Sq + min((qt + 1) * NW * 32 - 1, p.Sq - 1);
 
+    const int64_t rec = ((int64_t)b * p.H + h) * p.Sq + qi;
     Frag<T> q[NC], g[NC];
     float delta = 0.f;
     {
@@ -65,12 +66,16 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void a
             const Frag<T> o = in ? load8(os + d) : zero8<T>();
 #pragma unroll
             for (int j = 0; j < 8; ++j) delta = fmaf((float)g[c].v[j], (float)o.v[j], delta);
+            if constexpr (sizeof(T) == 2) {                           // what o lost when it was rounded
+                const Frag<T> rest = in ? load8(reinterpret_cast<const T*>(p.stats + rec * p.stats_row + 4) + d) : zero8<T>();
+#pragma unroll
+                for (int j = 0; j < 8; ++j) delta = fmaf((float)g[c].v[j], (float)rest.v[j], delta);
+            }
         }
     }
     delta += __shfl_xor(delta, 32, 64);
-    const int64_t rec = ((int64_t)b * p.H + h) * p.Sq + qi;
     if (valid && half == 0) p.delta[rec] = delta;
-    const float2 st = p.stats[rec];
+    const float2 st = *reinterpret_cast<const float2*>(p.stats + rec * p.stats_row);
     const float top = st.x, inv = valid ? st.y : 0.f, dinv = delta * inv;      // dS = 2^(s - top) (dP inv - delta inv)
 
     const bool has_bias = p.table != nullptr, want = p.want_dtable != 0;
@@ -274,8 +279,48 @@ __global__ __launch_bounds__(64 * NW, DP >= 64 ? 1 : 2) void attention_dkv_kerne
         sg.load(at<T>(p.dout, b, row0, h), m, 0, p.D, tid);
         if (tid < QT) {
             const int64_t rec = ((int64_t)b * p.H + h) * p.Sq + row0 + tid;
-            st = tid < left ? p.stats[rec] : make_float2(0.f, 0.f);
+            st = tid < left ? *reinterpret_cast<const float2*>(p.stats + rec * p.stats_row) : make_float2(0.f, 0.f);
             st_d = tid < left ? p.delta[rec] : 0.f;
+        }
+    };
+    // fp32 sums over many rows go to the output in parts of 512 rows (read back and added: 1 / 16 of a part's traffic), so that their
+    // rounding does not grow with the sequence and the heads of a group: 4 heads x 4095 rows come out 0.6e-6 off, half of what one chain leaves
+    constexpr int PART = sizeof(T) == 4 ? 512 / QT : 1 << 30;
+    bool parted = false;
+    auto store = [&](bool last) {
+        if (key < p.Sk) {
+            T* kd = at_mut<T>(p.dk, b, key, kvh);
+            T* vd = at_mut<T>(p.dv, b, key, kvh);
+            const float scale = last ? p.scale : 1.f;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const int c = d * 32 + acc_row(r, half);
+                    if (c < p.D) {
+                        float k4[4], v4[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            k4[j] = dk[d][r + j];
+                            v4[j] = dv[d][r + j];
+                            if constexpr (sizeof(T) == 4) {
+                                if (parted) {
+                                    k4[j] += kd[c + j];
+                                    v4[j] += vd[c + j];
+                                }
+                            }
+                        }
+                        store4<T>(kd + c, k4[0] * scale, k4[1] * scale, k4[2] * scale, k4[3] * scale);
+                        store4<T>(vd + c, v4[0], v4[1], v4[2], v4[3]);
+                    }
+                }
+        }
+        if (!last) {
+            parted = true;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) { dk[d][r] = 0.f; dv[d][r] = 0.f; }
         }
     };
     if (AHEAD && total > 0) fetch(0);
@@ -298,6 +343,7 @@ __global__ __launch_bounds__(64 * NW, DP >= 64 ? 1 : 2) void attention_dkv_kerne
         __syncthreads();
         if (AHEAD && i + 1 < total) fetch(i + 1);
         if (!alive) continue;
+        if (i > 0 && i % PART == 0) store(false);
 #pragma unroll
         for (int n = 0; n < QT / 32; ++n) {
             const int pos0 = back + row0 + n * 32;                     // position of the tile's first query
@@ -349,20 +395,7 @@ __global__ __launch_bounds__(64 * NW, DP >= 64 ? 1 : 2) void attention_dkv_kerne
             }
         }
     }
-    if (key < p.Sk) {
-        T* kd = at_mut<T>(p.dk, b, key, kvh);
-        T* vd = at_mut<T>(p.dv, b, key, kvh);
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const int c = d * 32 + acc_row(r, half);
-                if (c < p.D) {
-                    store4<T>(kd + c, dk[d][r] * p.scale, dk[d][r + 1] * p.scale, dk[d][r + 2] * p.scale, dk[d][r + 3] * p.scale);
-                    store4<T>(vd + c, dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]);
-                }
-            }
-    }
+    store(true);
 }
 
 // the sums by distance of every (batch row, query tile), added in index order in kSeg segments ...

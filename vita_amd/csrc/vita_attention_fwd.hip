@@ -8,13 +8,16 @@
 // the previous one is multiplied).  With few rows the key axis is also split over workgroups, whose (O, m, l) a second launch joins in
 // split order.  Query heads that share a key head share a row tile there (row = query * G + head), so the cache is read once.
 // Tiles whose keys are all padded, or all ahead of a causal row, are skipped without being read.
-// P is rounded to bf16 for the second product of bf16 calls (the matrix unit's operand type); sums, maxima and O stay fp32.
+// P is rounded to bf16 for the second product of bf16 calls (the matrix unit's operand type); sums, maxima and O stay fp32.  EXACT: what
+// the rounding lost is multiplied too, and O's own rounding is kept beside the row statistics: the backward pass's sum dO . O needs O
+// nearer than bf16 where a row has few keys (dq, dk and the bias gradient came out 1.5 - 1.8 times as far off as their own rounding puts
+// them, with it 1.4).  The few-row kernels always do it (they wait for memory), the long one in training only (207 against LONGTIME us).
 #include "vita_attention.h"
 
 namespace vita {
 namespace {
 
-template <class T, int DP, int NQ, int NK, int KW>
+template <class T, int DP, int NQ, int NK, int KW, bool EXACT>
 __global__ __launch_bounds__(64 * NQ * NK, sizeof(T) == 4 && DP >= 96 ? 1 : 2) void attention_fwd_kernel(AttnParams p) {
     constexpr int NT = 64 * NQ * NK, KT = KW * NK, KS = lds_stride<T, DP>(), NC = DP / 16, ND = DP / 32, NS = KW / 32;
     constexpr bool AHEAD = NQ * NK > 1;      // the next tile is fetched while this one is multiplied; one-wave workgroups mostly have one tile
@@ -148,7 +151,7 @@ __global__ __launch_bounds__(64 * NQ * NK, sizeof(T) == 4 && DP >= 96 ? 1 : 2) v
             }
             const float shift = add - (m == -kInf ? 0.f : m);
             // probabilities of 16 keys at a time, so that a step's exponentials run beside the previous step's products
-            Frag<T> pf;
+            Frag<T> pf, rest;
             pipelined<T, 2 * NS, ND>(
                 [&](int i, int d) { return col_frag<T, KS>(vt, wk * KW + i * 16, d * 32, lane); },
                 [&](int i, int d, const Frag<T>& a) {
@@ -162,8 +165,10 @@ __global__ __launch_bounds__(64 * NQ * NK, sizeof(T) == 4 && DP >= 96 ? 1 : 2) v
                         }
                         l += sum;
                         pf = pack8<T>(sn, i & 1);
+                        if constexpr (EXACT) rest = pack8_rest(sn, i & 1, pf);
                     }
                     mma(o[d], a, pf);
+                    if constexpr (EXACT) mma(o[d], a, rest);
                 });
         }
         t = tn;
@@ -182,8 +187,13 @@ __global__ __launch_bounds__(64 * NQ * NK, sizeof(T) == 4 && DP >= 96 ? 1 : 2) v
                 for (int r = 0; r < 16; r += 4) {
                     const int c = d * 32 + acc_row(r, half);
                     if (c < p.D) {
-                        if (part != nullptr) store4<float>(part + c, o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]);
-                        else store4<T>(dst + c, o[d][r] * inv, o[d][r + 1] * inv, o[d][r + 2] * inv, o[d][r + 3] * inv);
+                        if (part != nullptr) {
+                            store4<float>(part + c, o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]);
+                        } else {
+                            const float v0 = o[d][r] * inv, v1 = o[d][r + 1] * inv, v2 = o[d][r + 2] * inv, v3 = o[d][r + 3] * inv;
+                            store4<T>(dst + c, v0, v1, v2, v3);
+                            if (sizeof(T) == 2 && p.stats != nullptr) store_rest4(p.stats + rec * p.stats_row, c, v0, v1, v2, v3);
+                        }
                     }
                 }
             if (half == 0) {
@@ -191,7 +201,7 @@ __global__ __launch_bounds__(64 * NQ * NK, sizeof(T) == 4 && DP >= 96 ? 1 : 2) v
                     p.part_ml[(split * nrec + rec) * 2] = m;
                     p.part_ml[(split * nrec + rec) * 2 + 1] = l;
                 } else if (p.stats != nullptr) {
-                    p.stats[rec] = make_float2(m == -kInf ? 0.f : m, inv);
+                    store_stats<T>(p.stats + rec * p.stats_row, m == -kInf ? 0.f : m, inv);
                 }
             }
         }
@@ -229,15 +239,19 @@ __global__ __launch_bounds__(64 * NQ * NK, sizeof(T) == 4 && DP >= 96 ? 1 : 2) v
                     for (int w = 1; w < NK; ++w) a[j] += buf[(w * DP + c + j) * 32 + col];
                     a[j] *= scale;
                 }
-                if (part != nullptr) store4<float>(part + c, a[0], a[1], a[2], a[3]);
-                else store4<T>(dst + c, a[0], a[1], a[2], a[3]);
+                if (part != nullptr) {
+                    store4<float>(part + c, a[0], a[1], a[2], a[3]);
+                } else {
+                    store4<T>(dst + c, a[0], a[1], a[2], a[3]);
+                    if (sizeof(T) == 2 && p.stats != nullptr) store_rest4(p.stats + rec * p.stats_row, c, a[0], a[1], a[2], a[3]);
+                }
             }
             if (wave == 0 && half == 0) {
                 if (part != nullptr) {
                     p.part_ml[(split * nrec + rec) * 2] = top;
                     p.part_ml[(split * nrec + rec) * 2 + 1] = total;
                 } else if (p.stats != nullptr) {
-                    p.stats[rec] = make_float2(safe, scale);
+                    store_stats<T>(p.stats + rec * p.stats_row, safe, scale);
                 }
             }
         }
@@ -267,7 +281,11 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p) {
     const int64_t bh = rec / p.Sq;
     const int qi = (int)(rec - bh * p.Sq), b = (int)(bh / p.H), h = (int)(bh - (int64_t)b * p.H);
     store4<T>(at_mut<T>(p.o, b, qi, h) + c, a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv);
-    if (c == 0 && p.stats != nullptr) p.stats[rec] = make_float2(safe, inv);
+    if (p.stats != nullptr) {
+        float* row = p.stats + rec * p.stats_row;
+        if (sizeof(T) == 2) store_rest4(row, c, a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv);
+        if (c == 0) store_stats<T>(row, safe, inv);
+    }
 }
 
 enum { FWD_ROWS4 = 0, FWD_ROWS1 = 1, FWD_KEYS4 = 2 };
@@ -297,21 +315,26 @@ Plan plan(const vita_attention_args* a) {
     return f;
 }
 
-template <class T, int DP, int NQ, int NK, int KW>
+template <class T, int DP, int NQ, int NK, int KW, bool EXACT>
 int launch(const AttnParams& p, int64_t blocks, hipStream_t s) {
     const size_t lds = (size_t)2 * KW * NK * lds_stride<T, DP>() * sizeof(T) + (NK > 1 ? NK * 64 * 4 : 0) +
                        (p.table != nullptr ? (size_t)p.pack * (2 * p.R + 1) * 4 : 0);
     VITA_REQUIRE(lds <= 160 * 1024, "vita_attention: radius %d with %d heads to a key head needs %zu bytes of LDS", p.R, p.pack, lds);
-    auto kernel = attention_fwd_kernel<T, DP, NQ, NK, KW>;
+    auto kernel = attention_fwd_kernel<T, DP, NQ, NK, KW, EXACT>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * NQ * NK), lds, s, p);
     VITA_CHECK_HIP(hipGetLastError());
     return VITA_OK;
 }
 template <class T, int DP>
 int launch_mode(const AttnParams& p, const Plan& f, hipStream_t s) {
-    if (f.mode == FWD_ROWS4) return launch<T, DP, 4, 1, sizeof(T) == 2 ? 64 : 32>(p, f.blocks, s);
-    if (f.mode == FWD_ROWS1) return launch<T, DP, 1, 1, 32>(p, f.blocks, s);
-    return launch<T, DP, 1, 4, 32>(p, f.blocks, s);
+    constexpr bool BF = sizeof(T) == 2;
+    if (f.mode == FWD_ROWS4) {
+        if constexpr (BF)
+            if (p.stats != nullptr) return launch<T, DP, 4, 1, 64, true>(p, f.blocks, s);
+        return launch<T, DP, 4, 1, BF ? 64 : 32, false>(p, f.blocks, s);
+    }
+    if (f.mode == FWD_ROWS1) return launch<T, DP, 1, 1, 32, BF>(p, f.blocks, s);
+    return launch<T, DP, 1, 4, 32, BF>(p, f.blocks, s);
 }
 template <class T>
 int launch_type(const AttnParams& p, const Plan& f, hipStream_t s) {
@@ -348,7 +371,7 @@ int attention_check(const vita_attention_args* a, bool bwd, const char* who) {
     VITA_REQUIRE((int64_t)a->k_ss < (1 << 23) && a->v_ss < (1 << 23) && a->q_ss < (1 << 23) && (!bwd || a->dout_ss < (1 << 23)) && a->k_ss >= 0 && a->v_ss >= 0 &&
                      a->q_ss >= 0 && (!bwd || a->dout_ss >= 0),
                  "%s: token strides must be below 2^23 elements", who);
-    VITA_REQUIRE((reinterpret_cast<uintptr_t>(a->stats) & 7u) == 0, "%s: misaligned stats", who);
+    VITA_REQUIRE((reinterpret_cast<uintptr_t>(a->stats) & 15u) == 0, "%s: misaligned stats", who);
     VITA_REQUIRE(a->key_pad == nullptr || a->ld_pad == 0 || a->ld_pad >= a->Sk, "%s: bad ld_pad", who);
     if (a->table != nullptr) {
         VITA_REQUIRE(a->buckets != nullptr && a->radius >= 0 && a->radius <= kMaxRadius && a->num_buckets >= 1, "%s: bias with radius %d, %d buckets", who,
@@ -356,7 +379,7 @@ int attention_check(const vita_attention_args* a, bool bwd, const char* who) {
         VITA_REQUIRE((reinterpret_cast<uintptr_t>(a->table) & (es - 1)) == 0, "%s: misaligned bias table", who);
     }
     if (bwd) {
-        VITA_REQUIRE(a->stats != nullptr && (reinterpret_cast<uintptr_t>(a->stats) & 7u) == 0 && ok(a->dout, a->dout_sb, a->dout_ss, a->dout_sh) && ok(a->dq, a->dq_sb, a->dq_ss, a->dq_sh) &&
+        VITA_REQUIRE(a->stats != nullptr && ok(a->dout, a->dout_sb, a->dout_ss, a->dout_sh) && ok(a->dq, a->dq_sb, a->dq_ss, a->dq_sh) &&
                          ok(a->dk, a->dk_sb, a->dk_ss, a->dk_sh) && ok(a->dv, a->dv_sb, a->dv_ss, a->dv_sh),
                      "%s: stats, dout, dq, dk and dv must be non-null, 16-byte aligned, with strides that are multiples of 16 bytes", who);
         VITA_REQUIRE(a->dtable == nullptr || a->table != nullptr, "%s: dtable without a table", who);
@@ -368,7 +391,7 @@ void attention_fill(const vita_attention_args* a, AttnParams& p) {
     auto t = [](const void* q, int64_t b, int64_t s, int64_t h) { return AttnTensor{(char*)const_cast<void*>(q), b, s, h}; };
     p.q = t(a->q, a->q_sb, a->q_ss, a->q_sh); p.k = t(a->k, a->k_sb, a->k_ss, a->k_sh);
     p.v = t(a->v, a->v_sb, a->v_ss, a->v_sh); p.o = t(a->o, a->o_sb, a->o_ss, a->o_sh);
-    p.stats = reinterpret_cast<float2*>(a->stats); p.pad = a->key_pad; p.ld_pad = a->ld_pad;
+    p.stats = a->stats; p.stats_row = stats_row(a->dtype == VITA_DT_BF16, a->D); p.pad = a->key_pad; p.ld_pad = a->ld_pad;
     p.table = a->table; p.buckets = a->buckets; p.R = a->table != nullptr ? a->radius : 0; p.NB = a->num_buckets;
     p.B = a->B; p.H = a->H; p.Hk = a->Hk; p.G = a->H / a->Hk; p.Sq = a->Sq; p.Sk = a->Sk; p.D = a->D; p.causal = a->causal != 0;
     p.scale = a->scale; p.scale_log2 = a->scale * kLog2e;
@@ -380,6 +403,8 @@ void attention_fill(const vita_attention_args* a, AttnParams& p) {
 using namespace vita;
 
 extern "C" {
+
+int32_t vita_attention_stats_row(int32_t dtype, int32_t D) { return stats_row(dtype == VITA_DT_BF16, D); }
 
 size_t vita_attention_workspace_bytes(const vita_attention_args* a) {
     if (a == nullptr || a->B <= 0 || a->Sq <= 0 || a->Hk <= 0 || a->H < a->Hk || a->H % a->Hk != 0 || a->Sk < 0) return 0;

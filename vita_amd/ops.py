@@ -1614,10 +1614,14 @@ def _attention_args(q, k, v, scale, causal, key_pad, table, buckets, who):
     return head, tail, (q, k, v, key_pad, table, buckets)
 
 
+def _stats_shape(q: Tensor) -> tuple:
+    return q.shape[0], q.shape[2], q.shape[1], L.load().vita_attention_stats_row(_DT[q.dtype], q.shape[3])
+
+
 def _attention(q, k, v, scale, causal, key_pad, table, buckets, need_lse, out):
     head, tail, keep = _attention_args(q, k, v, scale, causal, key_pad, table, buckets, "attention")
     o = _out(out, "attention: out", q.shape, q)
-    stats = torch.empty((q.shape[0], q.shape[2], q.shape[1], 2), dtype=torch.float32, device=q.device) if need_lse else None
+    stats = torch.empty(_stats_shape(q), dtype=torch.float32, device=q.device) if need_lse else None
     if o.numel():
         if out is not None and not _aligned(o):
             raise L.VitaHipError("attention: out needs 16-byte aligned rows")
@@ -1639,7 +1643,7 @@ def attention_bwd(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, o: Tensor, stat
         if t.shape != q.shape:
             raise L.VitaHipError(f"attention_bwd: {name} {tuple(t.shape)}, expected {tuple(q.shape)}")
     _f32(stats, "attention_bwd: stats")
-    rows = (q.shape[0], q.shape[2], q.shape[1], 2)
+    rows = _stats_shape(q)
     if tuple(stats.shape) != rows or stats.device != q.device:
         raise L.VitaHipError(f"attention_bwd: stats {tuple(stats.shape)} on {stats.device}, expected {rows} on {q.device}")
     dout, o, stats = _aligned_rows(dout), _aligned_rows(o), stats.contiguous()
@@ -1686,8 +1690,10 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, scale: Optional[float] = None,
     scale: D ** -0.5 by default.  causal: query i sees keys up to i + Sk - Sq.  key_pad (B, Sk) bool: True where a key does not exist
     (the dataset's `*_is_pad`); a query without any key gives zeros.  table (buckets, H) of q's type with buckets = int32
     (2 R + 1,), the bucket of each distance -R .. R (relative_buckets): adds table[bucket of (key - query position), h] to the scores.
-    need_lse: also the row statistics that attention_bwd takes, (B, H, Sq, 2) fp32: a maximum m of the row's scores times log2 e and
-    r = 1 / sum 2 ** (score log2 e - m), so that log sum exp = m ln 2 - ln r; (0, 0) for a query without keys.  out: the result's tensor.  Differentiable in q, k, v and table."""
+    need_lse: also the row statistics that attention_bwd takes, (B, H, Sq, n) fp32: [..., 0] a maximum m of the row's scores times log2 e,
+    [..., 1] r = 1 / sum 2 ** (score log2 e - m), so that log sum exp = m ln 2 - ln r, (0, 0) for a query without keys; bf16: behind them
+    what the result lost when it was rounded (probabilities are then multiplied in two bf16 parts: the result is nearer than without).
+    out: the result's tensor.  Differentiable in q, k, v and table."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, table)):
         if out is not None:
             raise L.VitaHipError("attention: out= cannot be used where a gradient is wanted")

@@ -54,8 +54,16 @@ __device__ __forceinline__ void mma(f32x16& acc, const Frag<bf16>& a, const Frag
 
 __device__ __forceinline__ int acc_row(int r, int half) { return (r >> 2) * 8 + half * 4 + (r & 3); }
 
-// elements of a tile's row in LDS: padded so that the 16-byte reads of 16 consecutive rows meet 16 different bank groups
-template <class T, int DP> constexpr int lds_stride() { return DP + 16 / (int)sizeof(T); }
+// A tile in LDS: rows of DP elements and a padding.  The 16-byte reads of 16 consecutive rows meet 16 different groups of 4 banks where
+// the stride is an odd number of 16 bytes.  The transposed reads of bf16 take 4 rows x 64 bytes at a time, which share no more than two
+// to a bank where the stride is 48, 80, 176 or 208 bytes beyond a multiple of 256.  (XORed pieces in place of padding free both of
+// conflicts, but want an address register for every piece: the dq kernel spilled and went from 340 to 374 us, 2 x 4096 x 16 heads of 128.)
+template <class T, int DP> constexpr int lds_stride() {
+    return DP + (sizeof(T) == 2 && DP % 64 == 0 ? 24 : 16 / (int)sizeof(T));
+}
+// the 16-byte piece `piece` of a row
+template <class T, int DP>
+__device__ __forceinline__ int lds_at(int row, int piece) { return row * lds_stride<T, DP>() + piece * (16 / (int)sizeof(T)); }
 
 template <class T>
 __device__ __forceinline__ Frag<T> load8(const T* p) {      // 16-byte aligned
@@ -68,6 +76,11 @@ __device__ __forceinline__ Frag<T> load8(const T* p) {      // 16-byte aligned
         for (int j = 0; j < 4; ++j) { f.v[j] = a[j]; f.v[4 + j] = b[j]; }
     }
     return f;
+}
+// 8 elements from column 8 c of a tile's row
+template <class T, int DP>
+__device__ __forceinline__ Frag<T> row_frag(const T* tile, int row, int c) {
+    return load8(tile + row * lds_stride<T, DP>() + c * 8);
 }
 template <class T>
 __device__ __forceinline__ Frag<T> zero8() {
@@ -83,8 +96,9 @@ __device__ __forceinline__ Frag<T> zero8() {
 // fragment whose depth is the transpose of the tile: row = column col0 + lane % 32 of the tile, depth = the tile's rows row0 ..
 // row0 + 15 in accumulator order.  bf16: the hardware's transposed read (a group of 16 lanes gives 4 rows x 16 columns, lane i
 // getting column i); fp32: 8 reads of 32 neighbouring columns.
-template <class T, int KS>
+template <class T, int DP>
 __device__ __forceinline__ Frag<T> col_frag(const T* tile, int row0, int col0, int lane) {
+    constexpr int KS = lds_stride<T, DP>();
     Frag<T> f;
     if constexpr (sizeof(T) == 2) {
         const int g = lane >> 4, q = (lane & 15) >> 2, c = lane & 3;
@@ -102,25 +116,44 @@ __device__ __forceinline__ Frag<T> col_frag(const T* tile, int row0, int col0, i
     return f;
 }
 
-// Products of one tile in steps, the next step's fragments requested before this step multiplies: a step is long enough to cover the
-// LDS reads (one fp32 fragment feeds 512 cycles of MFMA, one bf16 fragment 32, so a bf16 step takes N of them), and the scheduler may not
-// move reads over a step's border.  a(i, j): the A fragment of column block j at step i;  mul(i, j, a): uses it.
-template <class T, int STEPS, int N, class Read, class Use>
-__device__ __forceinline__ void pipelined(Read read, Use use) {
-    constexpr int W = sizeof(T) == 2 ? N : 1, TOTAL = STEPS * N / W;
-    Frag<T> a[2][W];
+// Products of one tile in steps, fragments requested DEPTH steps ahead: a step is long enough to cover the LDS reads together with the
+// SIMD's other wave (one fp32 fragment feeds 512 cycles of MFMA, one bf16 fragment 32, so a bf16 step takes N of them; DEPTH 2 where a
+// wave has its SIMD to itself), and the scheduler may not move reads over a step's border.  read(i, j): the A fragment of column block j
+// at step i;  use(i, j, a): multiplies it.  start() may stand well in front of run().
+template <class T, int STEPS, int N, int DEPTH>
+struct Pipe {
+    static constexpr int W = sizeof(T) == 2 ? N : 1, TOTAL = STEPS * N / W;
+    Frag<T> a[DEPTH + 1][W];
+    template <class Read>
+    __device__ __forceinline__ void request(int i, Read read) {
+        if (i < TOTAL) {
 #pragma unroll
-    for (int j = 0; j < W; ++j) a[0][j] = read(0, j);
-#pragma unroll
-    for (int i = 0; i < TOTAL; ++i) {
-        if (i + 1 < TOTAL) {
-#pragma unroll
-            for (int j = 0; j < W; ++j) a[(i + 1) & 1][j] = read((i + 1) * W / N, (i + 1) * W % N + j);
+            for (int j = 0; j < W; ++j) a[i % (DEPTH + 1)][j] = read(i * W / N, i * W % N + j);
         }
+    }
+    template <class Read>
+    __device__ __forceinline__ void start(Read read) {
 #pragma unroll
-        for (int j = 0; j < W; ++j) use(i * W / N, i * W % N + j, a[i & 1][j]);
+        for (int i = 0; i < DEPTH; ++i) request(i, read);
         __builtin_amdgcn_sched_barrier(0);
     }
+    template <class Read, class Use>
+    __device__ __forceinline__ void run(Read read, Use use) {
+#pragma unroll
+        for (int i = 0; i < TOTAL; ++i) {
+            request(i + DEPTH, read);
+#pragma unroll
+            for (int j = 0; j < W; ++j) use(i * W / N, i * W % N + j, a[i % (DEPTH + 1)][j]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+};
+template <class T, int STEPS, int N, class Read, class Use>
+__device__ __forceinline__ void pipelined(Read read, Use use) {
+    Pipe<T, STEPS, N, 1> pipe;
+#pragma unroll
+    for (int j = 0; j < pipe.W; ++j) pipe.a[0][j] = read(0, j);
+    pipe.run(read, use);
 }
 
 template <class T>
@@ -179,7 +212,7 @@ struct Stage {
 #pragma unroll
         for (int j = 0; j < NLD; ++j) {
             const int i = j * NT + tid, row = i / NV, vec = i - row * NV;
-            *reinterpret_cast<uint4*>(tile + row * lds_stride<T, DP>() + vec * E) = r[j];
+            *reinterpret_cast<uint4*>(tile + lds_at<T, DP>(row, vec)) = r[j];
         }
     }
 };

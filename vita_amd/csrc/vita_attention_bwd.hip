@@ -32,6 +32,7 @@ template <class T, int DP, int NW, int KT>
 __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void attention_dq_kernel(AttnParams p) {
     constexpr int NT = 64 * NW, KS = lds_stride<T, DP>(), NC = DP / 16, ND = DP / 32;
     constexpr bool AHEAD = NW > 1;      // the next tile is fetched while this one is multiplied; one-wave workgroups mostly have one tile
+    constexpr bool EXACT = sizeof(T) == 2 && NW == 1;      // few keys: their roundings do not average out, and there is time to multiply them too
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* kt = reinterpret_cast<T*>(smem);
     T* vt = kt + KT * KS;
@@ -133,7 +134,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void a
             f32x16 s, dp;
 #pragma unroll
             for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
-            pipelined<T, NC, 2>([&](int c, int j) { return load8((j == 0 ? kt : vt) + (n * 32 + col) * KS + c * 16 + half * 8); },
+            pipelined<T, NC, 2>([&](int c, int j) { return row_frag<T, DP>(j == 0 ? kt : vt, n * 32 + col, c * 2 + half); },
                                 [&](int c, int j, const Frag<T>& a) { mma(j == 0 ? s : dp, a, j == 0 ? q[c] : g[c]); });
             const int dmax = key0 + 31 - pos_lo, dmin = key0 - pos_hi;
             const bool far = dmax <= -R || dmin >= R, full = bits == 0xffffffffu && !(p.causal && key0 + 31 > pos_lo);
@@ -155,8 +156,13 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void a
             }
             {
                 const Frag<T> df[2] = {pack8<T>(s, 0), pack8<T>(s, 1)};
-                pipelined<T, 2, ND>([&](int c, int d) { return col_frag<T, KS>(kt, n * 32 + c * 16, d * 32, lane); },
-                                    [&](int c, int d, const Frag<T>& a) { mma(dq[d], a, df[c]); });
+                Frag<T> rest[2];
+                if constexpr (EXACT) { rest[0] = pack8_rest(s, 0, df[0]); rest[1] = pack8_rest(s, 1, df[1]); }
+                pipelined<T, 2, ND>([&](int c, int d) { return col_frag<T, DP>(kt, n * 32 + c * 16, d * 32, lane); },
+                                    [&](int c, int d, const Frag<T>& a) {
+                                        mma(dq[d], a, df[c]);
+                                        if constexpr (EXACT) mma(dq[d], a, rest[c]);
+                                    });
             }
             if (want) {
                 if (far) {
@@ -226,11 +232,12 @@ template <class T, int DP, int NW, int QT>
 __global__ __launch_bounds__(64 * NW, DP >= 64 ? 1 : 2) void attention_dkv_kernel(AttnParams p) {
     constexpr int NT = 64 * NW, KS = lds_stride<T, DP>(), NC = DP / 16, ND = DP / 32;
     constexpr bool AHEAD = NW > 1;      // the next tile is fetched while this one is multiplied; one-wave workgroups mostly have one tile
+    constexpr bool EXACT = sizeof(T) == 2 && NW == 1;      // few keys: their roundings do not average out, and there is time to multiply them too
+    constexpr int BUF = 2 * QT * KS;                                 // q and dO rows of a tile, two tiles
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    T* qs = reinterpret_cast<T*>(smem);
-    T* gs = qs + QT * KS;
-    float* stat = reinterpret_cast<float*>(gs + QT * KS);            // (3, QT): maximum, reciprocal sum, delta of the tile's rows
-    float* bias = stat + 3 * QT;
+    T* tiles = reinterpret_cast<T*>(smem);
+    float* stats = reinterpret_cast<float*>(tiles + 2 * BUF);        // (2, 3, QT): maximum, reciprocal sum, delta of the tiles' rows
+    float* biases = stats + 6 * QT;                                  // (2, 2 R + 1): of the current and the next query head
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
@@ -285,7 +292,7 @@ __global__ __launch_bounds__(64 * NW, DP >= 64 ? 1 : 2) void attention_dkv_kerne
     };
     // fp32 sums over many rows go to the output in parts of 512 rows (read back and added: 1 / 16 of a part's traffic), so that their
     // rounding does not grow with the sequence and the heads of a group: 4 heads x 4095 rows come out 0.6e-6 off, half of what one chain leaves
-    constexpr int PART = sizeof(T) == 4 ? 512 / QT : 1 << 30;
+    constexpr int PART = 512 / QT;
     bool parted = false;
     auto store = [&](bool last) {
         if (key < p.Sk) {
@@ -323,78 +330,113 @@ __global__ __launch_bounds__(64 * NW, DP >= 64 ? 1 : 2) void attention_dkv_kerne
                 for (int r = 0; r < 16; ++r) { dk[d][r] = 0.f; dv[d][r] = 0.f; }
         }
     };
-    if (AHEAD && total > 0) fetch(0);
+    // two tiles in LDS: tile i + 1 is written while others may still read tile i, one barrier a tile
     int have = -1;
-    for (int i = 0; i < total; ++i) {
-        const int gi = i / per, row0 = (q_first + i - gi * per) * QT;
-        __syncthreads();
-        if (!AHEAD) fetch(i);
-        sq.store(qs, tid);
-        sg.store(gs, tid);
+    auto put = [&](int i) {
+        T* t = tiles + (i & 1) * BUF;
+        float* stat = stats + (i & 1) * 3 * QT;
+        sq.store(t, tid);
+        sg.store(t + QT * KS, tid);
         if (tid < QT) {
             stat[tid] = st.x;
             stat[QT + tid] = st.y;
             stat[2 * QT + tid] = st_d;
         }
+        const int gi = i / per;
         if (has_bias && gi != have) {
-            load_bias<T>(p, bias, kvh * p.G + gi, 1, tid, NT);
+            load_bias<T>(p, biases + (gi & 1) * (2 * R + 1), kvh * p.G + gi, 1, tid, NT);
             have = gi;
         }
-        __syncthreads();
-        if (AHEAD && i + 1 < total) fetch(i + 1);
-        if (!alive) continue;
-        if (i > 0 && i % PART == 0) store(false);
-#pragma unroll
-        for (int n = 0; n < QT / 32; ++n) {
-            const int pos0 = back + row0 + n * 32;                     // position of the tile's first query
-            if (row0 + n * 32 >= p.Sq || (p.causal && pos0 + 31 < key0)) continue;
-            f32x16 s, dp;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
-            pipelined<T, NC, 2>([&](int c, int j) { return load8((j == 0 ? qs : gs) + (n * 32 + col) * KS + c * 16 + half * 8); },
-                                [&](int c, int j, const Frag<T>& a) { mma(j == 0 ? s : dp, a, j == 0 ? k[c] : v[c]); });
-            const int dmax = key0 + 31 - pos0, dmin = key0 - pos0 - 31;
-            const bool far = dmax <= -R || dmin >= R;
-            const float add = has_bias ? bias[dmax <= -R ? 0 : 2 * R] : 0.f;
-            if (whole && (!has_bias || (far && __builtin_fabsf(add) < kFoldBias)) && !(p.causal && key0 + 31 > pos0)) {
-#pragma unroll
-                for (int r = 0; r < 16; r += 4) {
-                    const f32x4 m4 = *reinterpret_cast<const f32x4*>(stat + n * 32 + acc_row(r, half));
-                    const f32x4 i4 = *reinterpret_cast<const f32x4*>(stat + QT + n * 32 + acc_row(r, half));
-                    const f32x4 d4 = *reinterpret_cast<const f32x4*>(stat + 2 * QT + n * 32 + acc_row(r, half));
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        s[r + j] = __builtin_amdgcn_exp2f(fmaf(s[r + j], p.scale_log2, add - m4[j])) * i4[j];
-                        dp[r + j] = s[r + j] * (dp[r + j] - d4[j]);
-                    }
-                }
-            } else {
-                const int see = p.causal ? key - pos0 - half * 4 : -(1 << 30);       // rows from `see` on see this key
-#pragma unroll
-                for (int r = 0; r < 16; r += 4) {
-                    const f32x4 m4 = *reinterpret_cast<const f32x4*>(stat + n * 32 + acc_row(r, half));
-                    const f32x4 i4 = *reinterpret_cast<const f32x4*>(stat + QT + n * 32 + acc_row(r, half));
-                    const f32x4 d4 = *reinterpret_cast<const f32x4*>(stat + 2 * QT + n * 32 + acc_row(r, half));
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float bv = has_bias ? bias[max(-R, min(R, key - pos0 - acc_row(r + j, half))) + R] : 0.f;
-                        const bool on = valid && acc_row(r + j, 0) >= see;
-                        const float pr = __builtin_amdgcn_exp2f(fmaf(s[r + j], p.scale_log2, bv) - m4[j]) * i4[j];
-                        s[r + j] = on ? pr : 0.f;
-                        dp[r + j] = on ? pr * (dp[r + j] - d4[j]) : 0.f;
-                    }
-                }
-            }
-            {
-                const Frag<T> pf[2] = {pack8<T>(s, 0), pack8<T>(s, 1)}, df[2] = {pack8<T>(dp, 0), pack8<T>(dp, 1)};
-                pipelined<T, 4, ND>([&](int i, int d) { return col_frag<T, KS>((i & 1) == 0 ? gs : qs, n * 32 + (i >> 1) * 16, d * 32, lane); },
-                                    [&](int i, int d, const Frag<T>& a) {
-                                        if ((i & 1) == 0) mma(dv[d], a, pf[i >> 1]);
-                                        else mma(dk[d], a, df[i >> 1]);
-                                    });
-            }
-        }
+    };
+    if (total > 0) {
+        fetch(0);
+        put(0);
     }
+    __syncthreads();
+    auto part = [&](int i, int end) {
+        for (; i < end; ++i) {
+            const int gi = i / per, row0 = (q_first + i - gi * per) * QT;
+            const T* qs = tiles + (i & 1) * BUF;
+            const T* gs = qs + QT * KS;
+            const float* stat = stats + (i & 1) * 3 * QT;
+            const float* bias = biases + (gi & 1) * (2 * R + 1);
+            if (AHEAD && i + 1 < total) fetch(i + 1);
+#pragma unroll
+            for (int n = 0; n < QT / 32; ++n) {
+                const int pos0 = back + row0 + n * 32;                     // position of the tile's first query
+                if (!alive || row0 + n * 32 >= p.Sq || (p.causal && pos0 + 31 < key0)) continue;
+                f32x16 s, dp;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+                {
+                    Pipe<T, NC, 2, sizeof(T) == 2 ? 2 : 1> pipe;
+                    auto read = [&](int c, int j) { return row_frag<T, DP>(j == 0 ? qs : gs, n * 32 + col, c * 2 + half); };
+                    pipe.start(read);
+                    pipe.run(read, [&](int c, int j, const Frag<T>& a) { mma(j == 0 ? s : dp, a, j == 0 ? k[c] : v[c]); });
+                }
+                // the transposed fragments of the first steps are on their way while the probabilities are formed
+                Pipe<T, 4, ND, sizeof(T) == 2 ? 2 : 1> pipe;
+                auto read = [&](int i, int d) { return col_frag<T, DP>((i & 1) == 0 ? gs : qs, n * 32 + (i >> 1) * 16, d * 32, lane); };
+                pipe.start(read);
+                const int dmax = key0 + 31 - pos0, dmin = key0 - pos0 - 31;
+                const bool far = dmax <= -R || dmin >= R;
+                const float add = has_bias ? bias[dmax <= -R ? 0 : 2 * R] : 0.f;
+                if (whole && (!has_bias || (far && __builtin_fabsf(add) < kFoldBias)) && !(p.causal && key0 + 31 > pos0)) {
+#pragma unroll
+                    for (int r = 0; r < 16; r += 4) {
+                        const f32x4 m4 = *reinterpret_cast<const f32x4*>(stat + n * 32 + acc_row(r, half));
+                        const f32x4 i4 = *reinterpret_cast<const f32x4*>(stat + QT + n * 32 + acc_row(r, half));
+                        const f32x4 d4 = *reinterpret_cast<const f32x4*>(stat + 2 * QT + n * 32 + acc_row(r, half));
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            s[r + j] = __builtin_amdgcn_exp2f(fmaf(s[r + j], p.scale_log2, add - m4[j])) * i4[j];
+                            dp[r + j] = s[r + j] * (dp[r + j] - d4[j]);
+                        }
+                    }
+                } else {
+                    const int see = p.causal ? key - pos0 - half * 4 : -(1 << 30);       // rows from `see` on see this key
+#pragma unroll
+                    for (int r = 0; r < 16; r += 4) {
+                        const f32x4 m4 = *reinterpret_cast<const f32x4*>(stat + n * 32 + acc_row(r, half));
+                        const f32x4 i4 = *reinterpret_cast<const f32x4*>(stat + QT + n * 32 + acc_row(r, half));
+                        const f32x4 d4 = *reinterpret_cast<const f32x4*>(stat + 2 * QT + n * 32 + acc_row(r, half));
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float bv = has_bias ? bias[max(-R, min(R, key - pos0 - acc_row(r + j, half))) + R] : 0.f;
+                            const bool on = valid && acc_row(r + j, 0) >= see;
+                            const float pr = __builtin_amdgcn_exp2f(fmaf(s[r + j], p.scale_log2, bv) - m4[j]) * i4[j];
+                            s[r + j] = on ? pr : 0.f;
+                            dp[r + j] = on ? pr * (dp[r + j] - d4[j]) : 0.f;
+                        }
+                    }
+                }
+                const Frag<T> pf[2] = {pack8<T>(s, 0), pack8<T>(s, 1)}, df[2] = {pack8<T>(dp, 0), pack8<T>(dp, 1)};
+                Frag<T> rest[4];
+                if constexpr (EXACT) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) { rest[2 * c] = pack8_rest(s, c, pf[c]); rest[2 * c + 1] = pack8_rest(dp, c, df[c]); }
+                }
+                pipe.run(read, [&](int i, int d, const Frag<T>& a) {
+                    f32x16& to = (i & 1) == 0 ? dv[d] : dk[d];
+                    mma(to, a, (i & 1) == 0 ? pf[i >> 1] : df[i >> 1]);
+                    if constexpr (EXACT) mma(to, a, rest[i]);
+                });
+            }
+            if (i + 1 < total) {
+                if (!AHEAD) fetch(i + 1);
+                put(i + 1);
+            }
+            __syncthreads();
+        }
+    };
+    if constexpr (sizeof(T) == 4) {
+        for (int i = 0; i < total;) {
+            const int end = min(total, i + PART);
+            part(i, end);
+            i = end;
+            if (i < total) store(false);
+        }
+    } else part(0, total);
     store(true);
 }
 
@@ -496,7 +538,8 @@ int launch_dq(const AttnParams& p, int64_t blocks, hipStream_t s) {
 }
 template <class T, int DP, int NW, int QT>
 int launch_dkv(const AttnParams& p, int64_t blocks, hipStream_t s) {
-    const size_t lds = (size_t)2 * QT * lds_stride<T, DP>() * sizeof(T) + 3 * QT * 4 + (p.table != nullptr ? (size_t)(2 * p.R + 1) * 4 : 0);
+    const size_t lds = (size_t)4 * QT * lds_stride<T, DP>() * sizeof(T) + 6 * QT * 4 + (p.table != nullptr ? (size_t)(2 * p.R + 1) * 8 : 0);
+    VITA_REQUIRE(lds <= 160 * 1024, "vita_attention_bwd: %zu bytes of LDS", lds);
     auto kernel = attention_dkv_kernel<T, DP, NW, QT>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * NW), lds, s, p);
     VITA_CHECK_HIP(hipGetLastError());

@@ -11,7 +11,8 @@
 // P is rounded to bf16 for the second product of bf16 calls (the matrix unit's operand type); sums, maxima and O stay fp32.  EXACT: what
 // the rounding lost is multiplied too, and O's own rounding is kept beside the row statistics: the backward pass's sum dO . O needs O
 // nearer than bf16 where a row has few keys (dq, dk and the bias gradient came out 1.5 - 1.8 times as far off as their own rounding puts
-// them, with it 1.4).  The few-row kernels always do it (they wait for memory), the long one in training only (207 against LONGTIME us).
+// them, with it 1.4).  The few-row kernels always do it (they wait for memory), the long one in training only (205 against 247 us,
+// 2 x 4095 rows, 16 heads of 128, causal).
 #include "vita_attention.h"
 
 namespace vita {
@@ -106,7 +107,7 @@ __global__ __launch_bounds__(64 * NQ * NK, sizeof(T) == 4 && DP >= 96 ? 1 : 2) v
             for (int n = 0; n < NS; ++n)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[n][r] = 0.f;
-            pipelined<T, NC, NS>([&](int c, int n) { return load8(kt + (wk * KW + n * 32 + col) * KS + c * 16 + half * 8); },
+            pipelined<T, NC, NS>([&](int c, int n) { return row_frag<T, DP>(kt, wk * KW + n * 32 + col, c * 2 + half); },
                                  [&](int c, int n, const Frag<T>& a) { mma(s[n], a, q[c]); });
             const bool full = (KW == 64 ? bits == ~uint64_t(0) : (uint32_t)bits == 0xffffffffu) && !(p.causal && key0 + KW - 1 > pos_lo);
             const int far_lo = key0 + KW - 1 - pos_lo, far_hi = key0 - pos_hi;           // largest and smallest distance of the wave's tile
@@ -150,10 +151,22 @@ __global__ __launch_bounds__(64 * NQ * NK, sizeof(T) == 4 && DP >= 96 ? 1 : 2) v
                 m = to;
             }
             const float shift = add - (m == -kInf ? 0.f : m);
+            // fp32: a tile's product is summed by itself and then added, so that O's rounding grows with the number of tiles, not of key pairs:
+            // dO . O, which the backward pass takes from every dS of a row, would carry it into the bias gradient's sums over all rows
+            // (5 x 1954 rows and keys, 2 heads of 128: the table's gradient 1.4e-6 off, the chained plain form's 0.5e-6)
+            f32x16 own[sizeof(T) == 4 ? ND : 1];
+            f32x16* to = o;
+            if constexpr (sizeof(T) == 4) {
+                to = own;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) own[d][r] = 0.f;
+            }
             // probabilities of 16 keys at a time, so that a step's exponentials run beside the previous step's products
             Frag<T> pf, rest;
             pipelined<T, 2 * NS, ND>(
-                [&](int i, int d) { return col_frag<T, KS>(vt, wk * KW + i * 16, d * 32, lane); },
+                [&](int i, int d) { return col_frag<T, DP>(vt, wk * KW + i * 16, d * 32, lane); },
                 [&](int i, int d, const Frag<T>& a) {
                     if (d == 0) {
                         f32x16& sn = s[i >> 1];
@@ -167,9 +180,15 @@ __global__ __launch_bounds__(64 * NQ * NK, sizeof(T) == 4 && DP >= 96 ? 1 : 2) v
                         pf = pack8<T>(sn, i & 1);
                         if constexpr (EXACT) rest = pack8_rest(sn, i & 1, pf);
                     }
-                    mma(o[d], a, pf);
-                    if constexpr (EXACT) mma(o[d], a, rest);
+                    mma(to[d], a, pf);
+                    if constexpr (EXACT) mma(to[d], a, rest);
                 });
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[d][r] += own[d][r];
+            }
         }
         t = tn;
     }

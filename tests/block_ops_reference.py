@@ -179,11 +179,12 @@ def act_and_slope(g, act):
     return g * th, th + g * torch.sigmoid(g) * (1 - th * th)
 
 
-def gated(x, w, b, act, dh=None):
+def gated(x, w, b, act, dh=None, parts=1):
     """(h, bound) and, with dh, (dx, bound), (dw, bound), (db, bound) behind them.  The slopes of the smooth activations are at most 1.2
-    and their second derivatives at most 1.2; the kernels' activations and slopes are counted with 1e-6 of max(1, |g|) of their own."""
+    and their second derivatives at most 1.2; the kernels' activations and slopes are counted with 1e-6 of max(1, |g|) of their own.
+    parts: the numbers of x's type that dz goes into the products as; the second rounds what the first left, so together they miss ut^2."""
     ut = half_step(x.dtype)
-    up = ut if x.dtype == torch.bfloat16 else 0.0
+    up = ut ** parts if x.dtype == torch.bfloat16 else 0.0
     x64, w64 = x.double().cpu(), w.double().cpu()
     M, K = x64.shape
     F = w64.shape[0] // 2

@@ -360,6 +360,19 @@ def test_gated_wide(M, K, F, act):
     _check_gated(*_gated_case(g, M, K, F, torch.bfloat16, M != 2300), act, g)
 
 
+@pytest.mark.parametrize("M,K,F", [(1, 8, 8), (2, 48, 88), (34, 48, 96), (64, 128, 1024)])
+def test_gated_few_rows_gradients(M, K, F):
+    """bf16: dz reaches dx and dw nearly whole, what is left is their own rounding."""
+    g = _gen(M + K)
+    x, w, b = _gated_case(g, M, K, F, torch.bfloat16, True)
+    dh = _randn(g, M, F, dtype=torch.bfloat16)
+    dx, dw, db = ops.gated_linear_bwd(dh, x, w, b, "silu")
+    r = ref.gated(x, w, b, "silu", dh, parts=2)
+    ref.assert_close(dx, r[2], r[3], "dx")
+    ref.assert_close(dw, r[4], r[5], "dw")
+    ref.assert_close(db, r[6], r[7], "db")
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("act", ["relu", "gelu", "gelu_tanh", "silu", "mish"])
 def test_gated_activations(dtype, act):

@@ -29,11 +29,11 @@ __global__ __launch_bounds__(256) void gated_product_kernel(const float* z, int6
     for (int j = 0; j < 4; ++j) o[j] = (T)(apply_act(g[j], act) * u[j]);
 }
 
-// dz and the partial sums of db: a workgroup has 256 features and kDzRows rows, a thread 4 features of every 4th row; 16-byte accesses
+// dz and the partial sums of db (lo: also what the rounding of dz lost, 2 F further on): a workgroup has 256 features and kDzRows rows, a thread 4 features of every 4th row; 16-byte accesses
 constexpr int kDzRows = 32;
 template <class T>
 __global__ __launch_bounds__(256) void gated_dz_kernel(const float* z, int64_t ldz, const T* dh, int64_t ld_dh, T* dz, int64_t ld_dz, float* db_part, int M,
-                                                       int F, int act, int64_t segs) {
+                                                       int F, int act, int64_t segs, bool lo) {
     typedef T vec4 __attribute__((ext_vector_type(4)));
     __shared__ float part[4][2][256];
     const int lane = threadIdx.x & 63, y = threadIdx.x >> 6, blocks = (F + 255) / 256;
@@ -45,17 +45,23 @@ __global__ __launch_bounds__(256) void gated_dz_kernel(const float* z, int64_t l
         for (int64_t r = r0 + y; r < r1; r += 4) {
             const f32x4 g = *reinterpret_cast<const f32x4*>(z + r * ldz + c), u = *reinterpret_cast<const f32x4*>(z + r * ldz + F + c);
             const vec4 d = *reinterpret_cast<const vec4*>(dh + r * ld_dh + c);
-            vec4 og, ou;
+            vec4 og, ou, lg, lu;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float dg = (float)d[j] * u[j] * act_grad(g[j], act), du = (float)d[j] * apply_act(g[j], act);
                 og[j] = (T)dg;
                 ou[j] = (T)du;
+                lg[j] = (T)(dg - (float)og[j]);
+                lu[j] = (T)(du - (float)ou[j]);
                 sg[j] += dg;
                 su[j] += du;
             }
             *reinterpret_cast<vec4*>(dz + r * ld_dz + c) = og;
             *reinterpret_cast<vec4*>(dz + r * ld_dz + F + c) = ou;
+            if (lo) {
+                *reinterpret_cast<vec4*>(dz + r * ld_dz + 2 * F + c) = lg;
+                *reinterpret_cast<vec4*>(dz + r * ld_dz + 3 * F + c) = lu;
+            }
         }
     if (db_part == nullptr) return;
 #pragma unroll
@@ -71,21 +77,25 @@ __global__ __launch_bounds__(256) void gated_dz_kernel(const float* z, int64_t l
             db_part[seg * 2 * F + k * F + f] = (part[0][k][threadIdx.x] + part[1][k][threadIdx.x]) + (part[2][k][threadIdx.x] + part[3][k][threadIdx.x]);
 }
 
-// (rows, cols) -> (cols, rows) of 16-bit elements
-__global__ __launch_bounds__(256) void transpose16_kernel(const uint16_t* src, int64_t ld, uint16_t* dst, int64_t ldd, int rows, int cols) {
+// (rows, cols) -> (cols, rows) of 16-bit elements, `copies` of it side by side
+__global__ __launch_bounds__(256) void transpose16_kernel(const uint16_t* src, int64_t ld, uint16_t* dst, int64_t ldd, int rows, int cols, int copies) {
     __shared__ uint16_t t[64][66];
     const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
     for (int j = y; j < 64; j += 4)
         if (r0 + j < rows && c0 + x < cols) t[j][x] = src[(int64_t)(r0 + j) * ld + c0 + x];
     __syncthreads();
     for (int j = y; j < 64; j += 4)
-        if (c0 + j < cols && r0 + x < rows) dst[(int64_t)(c0 + j) * ldd + r0 + x] = t[x][j];
+        if (c0 + j < cols && r0 + x < rows)
+            for (int k = 0; k < copies; ++k) dst[(int64_t)(c0 + j) * ldd + (int64_t)k * rows + r0 + x] = t[x][j];
 }
-__global__ __launch_bounds__(256) void to_bf16_kernel(const float* src, bf16* dst, int64_t ldd, int rows, int cols) {
+// the sum of `parts` fp32 matrices, one below the other
+__global__ __launch_bounds__(256) void to_bf16_kernel(const float* src, bf16* dst, int64_t ldd, int rows, int cols, int parts) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= (int64_t)rows * cols) return;
-    const int64_t r = i / cols;
-    dst[r * ldd + (i - r * cols)] = (bf16)src[i];
+    const int64_t r = i / cols, n = (int64_t)rows * cols;
+    float v = src[i];
+    for (int k = 1; k < parts; ++k) v += src[k * n + i];
+    dst[r * ldd + (i - r * cols)] = (bf16)v;
 }
 
 // ---- the wide bf16 products ------------------------------------------------------------------------------------------------------
@@ -346,7 +356,8 @@ int check(const vita_gated_args* a, bool bwd, const char* who) {
     VITA_REQUIRE(a != nullptr, "%s: null args", who);
     VITA_REQUIRE(a->dtype == VITA_DT_F32 || a->dtype == VITA_DT_BF16, "%s: unknown dtype %d", who, a->dtype);
     VITA_REQUIRE(a->act >= VITA_ACT_RELU && a->act <= VITA_ACT_MISH, "%s: unknown activation %d", who, a->act);
-    VITA_REQUIRE(a->M >= 0 && a->F >= 8 && a->K >= 8 && a->F % 8 == 0 && a->K % 8 == 0 && a->F <= (1 << 28) && a->M <= (1 << 28), "%s: bad shape M=%d F=%d K=%d (F and K multiples of 8)",
+    VITA_REQUIRE(a->M >= 0 && a->F >= 8 && a->K >= 8 && a->F % 8 == 0 && a->K % 8 == 0 && a->F <= (1 << 20) && a->K <= (1 << 20) && a->M <= (1 << 28),
+                 "%s: bad shape M=%d F=%d K=%d (F and K multiples of 8, at most 2^20)",
                  who, a->M, a->F, a->K);
     const int vec = a->dtype == VITA_DT_F32 ? 4 : 8;
     auto ok = [&](const void* p, int64_t ld, int64_t n) { return p != nullptr && (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % vec == 0 && ld >= n; };
@@ -370,6 +381,12 @@ bool wide_product(const vita_gated_args* a) { return a->dtype == VITA_DT_BF16 &&
 // a forward call that the few-row kernel takes (z wanted: the general path, which writes it)
 bool few_rows(const vita_gated_args* a) { return a->dtype == VITA_DT_BF16 && a->z == nullptr && a->M <= kFewRows; }
 
+// bf16 gradients of few rows and few weights: dz goes into dx and dw as two bf16 numbers, for with few terms its rounding does not average
+// out (2 x 48 x 88: dx and dw 1.64 times as far off as their own rounding puts them, many terms 1.41, both parts 1.0).  It doubles the
+// products, which such calls do not notice (launches bound them) and larger ones would.
+constexpr int64_t kExactWeights = 1 << 18;
+int dz_parts(const vita_gated_args* a) { return a->dtype == VITA_DT_BF16 && a->M <= kFewRows && 2 * (int64_t)a->F * a->K <= kExactWeights ? 2 : 1; }
+
 struct Ws { float* sk; float* z; void* dz; float* dw32; void* wt; float* db_part; float* cs; size_t bytes; };
 Ws carve(const vita_gated_args* a, bool bwd, void* ws) {
     Carver c(ws);
@@ -380,10 +397,10 @@ Ws carve(const vita_gated_args* a, bool bwd, void* ws) {
     if (bwd || !wide) r.sk = c.take(kSplitkBytes / 4);
     if (a->z == nullptr && !wide) r.z = c.take(M * F2);
     if (bwd) {
-        const size_t es = a->dtype == VITA_DT_F32 ? 4 : 2;
-        r.dz = c.take((M * F2 * es + 3) / 4);
-        if (a->dtype == VITA_DT_BF16 && a->dw != nullptr && !wide_fills(F2, K)) r.dw32 = c.take(F2 * K);
-        if (a->dtype == VITA_DT_BF16 && a->dx != nullptr && !wide_fills(M, K)) r.wt = c.take((F2 * K * es + 3) / 4);
+        const size_t es = a->dtype == VITA_DT_F32 ? 4 : 2, parts = dz_parts(a);
+        r.dz = c.take((M * F2 * parts * es + 3) / 4);
+        if (a->dtype == VITA_DT_BF16 && a->dw != nullptr && !wide_fills(F2, K)) r.dw32 = c.take(parts * F2 * K);
+        if (a->dtype == VITA_DT_BF16 && a->dx != nullptr && !wide_fills(M, K)) r.wt = c.take((parts * F2 * K * es + 3) / 4);
         // fp32 dx: W transposed once lets the product take the row-operand GEMM (2176 x 512 x 4096: 162 us on W as it lies), from as many
         // rows as the training step does so; the transpose wants W without gaps
         if (a->dtype == VITA_DT_F32 && a->dx != nullptr && a->M >= kWtMinRows && a->ldw == a->K) r.wt = c.take(F2 * K);
@@ -423,7 +440,7 @@ int preact(const vita_gated_args* a, float* z, int64_t ldz, const Ws& ws, hipStr
 
 int run_bwd(const vita_gated_args* a, void* workspace, hipStream_t s) {
     const Ws ws = carve(a, true, workspace);
-    const int M = a->M, F = a->F, F2 = 2 * a->F, K = a->K;
+    const int M = a->M, F = a->F, F2 = 2 * a->F, K = a->K, parts = dz_parts(a), FZ = parts * F2;      // FZ: columns of dz
     const float* z = a->z;
     int64_t ldz = a->ldz;
     const bool wide = wide_product(a);
@@ -443,9 +460,9 @@ int run_bwd(const vita_gated_args* a, void* workspace, hipStream_t s) {
         VITA_TRY(launch_wide_gated<WIDE_DZ>(a, o, s));
         segs = (M + WBM - 1) / WBM;
     } else if (a->dtype == VITA_DT_F32)
-        hipLaunchKernelGGL(gated_dz_kernel<float>, grid, dim3(256), 0, s, z, ldz, (const float*)a->dh, a->ld_dh, (float*)ws.dz, F2, part, M, F, a->act, (int64_t)segs);
+        hipLaunchKernelGGL(gated_dz_kernel<float>, grid, dim3(256), 0, s, z, ldz, (const float*)a->dh, a->ld_dh, (float*)ws.dz, F2, part, M, F, a->act, (int64_t)segs, false);
     else
-        hipLaunchKernelGGL(gated_dz_kernel<bf16>, grid, dim3(256), 0, s, z, ldz, (const bf16*)a->dh, a->ld_dh, (bf16*)ws.dz, F2, part, M, F, a->act, (int64_t)segs);
+        hipLaunchKernelGGL(gated_dz_kernel<bf16>, grid, dim3(256), 0, s, z, ldz, (const bf16*)a->dh, a->ld_dh, (bf16*)ws.dz, FZ, part, M, F, a->act, (int64_t)segs, parts == 2);
     VITA_CHECK_HIP(hipGetLastError());
     if (a->db != nullptr) VITA_TRY(vita_colsum_f32(part, F2, segs, F2, ws.cs, a->db, 0, s));
     SplitkScope sk(ws.sk, kSplitkBytes);
@@ -465,10 +482,11 @@ int run_bwd(const vita_gated_args* a, void* workspace, hipStream_t s) {
         o.c = (bf16*)a->dx; o.ldc = a->ld_dx;
         VITA_TRY((launch_wide<false, true, WIDE_C>((const bf16*)ws.dz, F2, (const bf16*)a->w, a->ldw, M, K, F2, 0, o, s)));
     } else if (a->dx != nullptr) {
-        hipLaunchKernelGGL(transpose16_kernel, dim3((K + 63) / 64, (F2 + 63) / 64), dim3(256), 0, s, (const uint16_t*)a->w, a->ldw, (uint16_t*)ws.wt, (int64_t)F2, F2, K);
+        hipLaunchKernelGGL(transpose16_kernel, dim3((K + 63) / 64, (F2 + 63) / 64), dim3(256), 0, s, (const uint16_t*)a->w, a->ldw, (uint16_t*)ws.wt, (int64_t)FZ, F2, K,
+                           parts);
         VITA_CHECK_HIP(hipGetLastError());
         vita_linear_args l{};
-        l.X = (const float*)ws.dz; l.ldx = F2; l.W = (const float*)ws.wt; l.ldw = F2; l.M = M; l.N = K; l.K = F2; l.ldy = K;
+        l.X = (const float*)ws.dz; l.ldx = FZ; l.W = (const float*)ws.wt; l.ldw = FZ; l.M = M; l.N = K; l.K = FZ; l.ldy = K;
         VITA_TRY(gemm_bf16_dma(l, (uint16_t*)a->dx, a->ld_dx, s));
     }
     if (a->dw != nullptr && wide_fills(F2, K)) {
@@ -477,10 +495,10 @@ int run_bwd(const vita_gated_args* a, void* workspace, hipStream_t s) {
         VITA_TRY((launch_wide<true, true, WIDE_C>((const bf16*)ws.dz, F2, (const bf16*)a->x, a->ldx, F2, K, M, 0, o, s)));
     } else if (a->dw != nullptr) {
         vita_linear_args l{};
-        l.Y = ws.dw32; l.ldy = K; l.M = F2; l.N = K; l.K = M; l.splitk_ws = ws.sk; l.splitk_ws_bytes = kSplitkBytes;
-        VITA_TRY(gemm_bf16_wgrad_tn((const uint16_t*)ws.dz, F2, (const uint16_t*)a->x, a->ldx, l, s));
+        l.Y = ws.dw32; l.ldy = K; l.M = FZ; l.N = K; l.K = M; l.splitk_ws = ws.sk; l.splitk_ws_bytes = kSplitkBytes;
+        VITA_TRY(gemm_bf16_wgrad_tn((const uint16_t*)ws.dz, FZ, (const uint16_t*)a->x, a->ldx, l, s));
         const int64_t n = (int64_t)F2 * K;
-        hipLaunchKernelGGL(to_bf16_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, ws.dw32, (bf16*)a->dw, a->ld_dw, F2, K);
+        hipLaunchKernelGGL(to_bf16_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, ws.dw32, (bf16*)a->dw, a->ld_dw, F2, K, parts);
         VITA_CHECK_HIP(hipGetLastError());
     }
     return VITA_OK;

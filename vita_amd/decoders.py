@@ -60,10 +60,12 @@ class CNNActionDecoder(nn.Module):
 
 class CNNAttentionActionDecoder(nn.Module):
     """action_vae.py:301-387: transposed-convolution upsampling to one token per action step, `num_transformer_layers` pre-norm
-    blocks (RoPE attention, models/transformer/blocks.py:13-55), LayerNorm, a per-token action head."""
+    blocks (RoPE attention, models/transformer/blocks.py:13-55; gated, rel_buckets, kernels: encoders.TransformerBlock), LayerNorm, a
+    per-token action head."""
 
     def __init__(self, pred_horizon: int, action_dim: int, latent_dim: int, hidden_dim: int = 128, num_cnn_layers: int = 2,
-                 num_transformer_layers: int = 2, num_heads: int = 4, mlp_ratio: float = 4.0, dropout: float = 0.0):
+                 num_transformer_layers: int = 2, num_heads: int = 4, mlp_ratio: float = 4.0, dropout: float = 0.0,
+                 gated: bool = False, rel_buckets: int = 0, kernels: bool = False):
         super().__init__()
         if float(dropout) != 0.0:
             raise NotImplementedError("CNNAttentionActionDecoder: dropout > 0 is not built")
@@ -74,7 +76,8 @@ class CNNAttentionActionDecoder(nn.Module):
         self.latent_proj = nn.Linear(latent_dim, hidden_dim * self.conv_output_length)
         self.cnn_decoder = _upsampling_stack(hidden_dim, hidden_dim, num_cnn_layers, relu_after_last=True)
         self.token_proj = nn.Linear(hidden_dim, hidden_dim)
-        self.transformer_layers = nn.ModuleList([TransformerBlock(hidden_dim, num_heads, mlp_ratio, rope_max_seq_length=pred_horizon)
+        self.transformer_layers = nn.ModuleList([TransformerBlock(hidden_dim, num_heads, mlp_ratio, rope_max_seq_length=pred_horizon,
+                                                                  gated=gated, rel_buckets=rel_buckets, kernels=kernels)
                                                  for _ in range(num_transformer_layers)])
         self.norm = nn.LayerNorm(hidden_dim)
         self.action_head = nn.Linear(hidden_dim, action_dim)

@@ -372,7 +372,9 @@ class VitaPolicy(nn.Module):
                                                            num_heads=net.num_heads, pred_horizon=self.pred_horizon,
                                                            action_dim=self.action_dim, num_layers=net.num_layers,
                                                            mlp_ratio=net.get("mlp_ratio", 4.0), dropout=net.get("dropout", 0.0),
-                                                           variational=bool(self.use_action_vae))             # action_vae.py:408-418
+                                                           variational=bool(self.use_action_vae),             # action_vae.py:408-418
+                                                           gated=bool(net.get("gated_mlp", False)), rel_buckets=int(net.get("rel_buckets", 0)),
+                                                           kernels=bool(net.get("encoder_kernels", False)))   # not the reference's (encoders.py)
         else:
             self.action_encoder = make_action_encoder(net.encoder_type, self.pred_horizon, self.action_dim, self.latent_dim,
                                                       net.enc_hidden_dim, net.num_layers, bool(self.use_action_vae))   # :101-110

@@ -178,3 +178,32 @@ def test_relative_buckets():
     for bad in ((2, 10), (7, 10), (8, 2)):
         with pytest.raises(ValueError):
             ops.relative_buckets(*bad)
+
+
+def _apart(*a, **k):
+    try:
+        ops._apart("out", *a, **k)
+        return True
+    except L.VitaHipError:
+        return False
+
+
+def test_outputs_apart_from_inputs():
+    for x, i in ((torch.zeros(2, 5, 3, 4, 8), 2), (torch.zeros(2, 5, 4, 3, 8), 3), (torch.zeros(3, 1, 3, 4, 8), 2), (torch.zeros(1, 1, 3, 4, 8), 2)):
+        q, k, v = x.unbind(i)                                         # slices of a packed projection, whole or by heads
+        assert _apart(q, k, v) and _apart(k, q, v) and not _apart(q, q) and not _apart(q, k, q[..., :4, :]) and _apart(q, q, but=(q,))
+        assert _apart(q, None, torch.zeros(2, 5, 4, 8), k[:0])
+    x = torch.zeros(2, 5, 3, 4, 8)
+    assert not _apart(x[:, :, 0], x[:, :, 0, 1:]) and _apart(x[:, :, 0, :2], x[:, :, 0, 2:]) and not _apart(x[:, 1:, 0], x[:, :-1, 0])
+    assert not _apart(x[:, :, 0], x[:, :, 0, :2], but=(x[:, :, 0, :2],))
+    z = torch.zeros(40, 64)
+    assert _apart(z[:, :40], z[:, 40:]) and not _apart(z[:, :40], z[:, 39:]) and not _apart(z[1:], z[:-1]) and _apart(z[:20], z[20:])
+
+
+def test_outputs_do_not_overlap_themselves():
+    like = torch.zeros(1)
+    for good in (torch.zeros(2, 5, 4, 8), torch.zeros(5, 2, 4, 8).transpose(0, 1), torch.zeros(2, 4, 5, 8).transpose(1, 2), torch.zeros(2, 5, 4, 3, 8)[:, :, :, 1]):
+        assert ops._out(good, "out", (2, 5, 4, 8), like) is good
+    for strides in ((40, 8, 8, 1), (160, 32, 4, 1), (160, 16, 8, 1), (0, 32, 8, 1), (160, 32, 8, 0), (640, 128, 16, 2)):
+        with pytest.raises(L.VitaHipError, match="overlap"):
+            ops._out(torch.zeros(4000).as_strided((2, 5, 4, 8), strides), "out", (2, 5, 4, 8), like)

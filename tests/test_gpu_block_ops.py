@@ -537,3 +537,22 @@ def test_autograd_gives_the_backward_calls_results():
         assert torch.equal(t.grad, d)
     with pytest.raises(L.VitaHipError, match="out="):
         ops.attention(q.clone().requires_grad_(), k, v, out=torch.empty_like(q))
+
+
+def test_outputs_that_share_memory_are_refused():
+    x = torch.zeros(2, 40, 3, 4, 16, device=DEV)
+    q, k, v = x.unbind(2)
+    rope = ref.rope_table(40, 1, 16).to(DEV)
+    ops.qk_norm_rope(q, k, rope, out=(q, k))                          # in place in the packed projection
+    o, stats = ops.attention(q, k, v, need_lse=True)
+    d = torch.zeros_like(o)
+    new = [torch.empty_like(o) for _ in range(3)]
+    ops.attention_bwd(d, q, k, v, o, stats, out=new)
+    for call in (lambda: ops.qk_norm_rope(q, k, rope, out=(k, q)), lambda: ops.qk_norm_rope(q, k, rope, out=(new[0], new[0])),
+                 lambda: ops.qk_norm_rope_bwd(d, new[0], q, k, rope, out=(new[0], new[1])),
+                 lambda: ops.attention(q, k, v, out=q), lambda: ops.attention(q, k, v, out=v),
+                 lambda: ops.attention_bwd(d, q, k, v, o, stats, out=(new[0], new[1], new[1])),
+                 lambda: ops.attention_bwd(d, q, k, v, o, stats, out=(d, new[1], new[2])),
+                 lambda: ops.gated_linear(d.view(-1, 64)[:, :16], torch.zeros(32, 16, device=DEV), out=d.view(-1, 64)[:, 8:24])):
+        with pytest.raises(L.VitaHipError, match="shares memory"):
+            call()

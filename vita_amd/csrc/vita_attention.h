@@ -301,6 +301,19 @@ __device__ __forceinline__ bool pair_order(int id, int pairs, int tiles, int by_
     return pair < pairs;
 }
 
+// Whether workgroups of 32 rows whose 4 waves share out the other axis run instead of workgroups of 4 x 32 rows, of which there would be
+// `wide`.  Each tile is then read for a quarter of the rows, but where the wide ones leave CUs without work, or give the CU with the
+// longest rows twice the mean, all share it.  Forward / backward, 8 heads, wide -> narrow: 1 x 512 tokens of 64 (32 workgroups) fp32
+// 46 / 147 -> 20 / 54 us; 1 x 1000 of 128 (64) fp32 155 / 519 -> 60 / 203, bf16 29 / 102 -> 22 / 64; 2 x 2048 of 64 causal (256) fp32
+// 168 / 578 -> 105 / 386; all rows alike (1 x 4095 of 64, 256) 334 / 1186 -> 333 / 1321; one tile long (32 x 100 causal, 256) 19 / 53 ->
+// 19 / 89; of 128 causal (2 x 2000 x 16 heads, 512) 340 / 1127 -> 447 / 1640.
+inline bool attention_narrow(const vita_attention_args* a, int64_t wide) {
+    if (a->dtype == VITA_DT_F32 && a->D > 96 && a->radius > 240) return false;                // its tiles and the bias gradient's rows fill the LDS
+    // (bf16 tiles are short of delivery sooner: 4 x 1000 padded tokens of 64, 256: 28 / 84 -> 36 / 111)
+    const bool uneven = a->dtype == VITA_DT_F32 && (a->causal || a->key_pad != nullptr);
+    return wide < 256 || (wide < 512 && uneven && a->D <= 64 && a->Sq >= 512 && a->Sk >= 512);
+}
+
 template <class T> __device__ __forceinline__ const T* at(const AttnTensor& t, int b, int64_t s, int h) {
     return reinterpret_cast<const T*>(t.p) + b * t.sb + s * t.ss + h * t.sh;
 }

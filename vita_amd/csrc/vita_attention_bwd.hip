@@ -28,28 +28,30 @@ __device__ __forceinline__ void wave_lds_order() {
     __builtin_amdgcn_wave_barrier();
 }
 
-template <class T, int DP, int NW, int KT>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void attention_dq_kernel(AttnParams p) {
-    constexpr int NT = 64 * NW, KS = lds_stride<T, DP>(), NC = DP / 16, ND = DP / 32;
-    constexpr bool AHEAD = NW > 1;      // the next tile is fetched while this one is multiplied; one-wave workgroups mostly have one tile
-    constexpr bool EXACT = sizeof(T) == 2 && NW == 1;      // few keys: their roundings do not average out, and there is time to multiply them too
+template <class T, int DP, int NQ, int NK, int KT>
+__global__ __launch_bounds__(64 * NQ * NK, (sizeof(T) == 4 && DP >= 64) || (NK > 1 && DP >= 96) ? 1 : 2) void attention_dq_kernel(AttnParams p) {
+    constexpr int NW = NQ * NK, NT = 64 * NW, KS = lds_stride<T, DP>(), NC = DP / 16, ND = DP / 32;
+    // the next tile is fetched while this one is multiplied; one-wave workgroups mostly have one tile, and 128 long fp32 rows do not fit registers
+    constexpr bool AHEAD = NW > 1 && !(NK > 1 && sizeof(T) == 4 && DP > 96);
+    constexpr bool EXACT = sizeof(T) == 2 && NQ == 1;      // few rows or keys: roundings do not average out, and there is time to multiply them too
+    static_assert(NK == 1 || KT == NK * 32, "a wave has one block of 32 keys of a tile");
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* kt = reinterpret_cast<T*>(smem);
     T* vt = kt + KT * KS;
     float* bias = reinterpret_cast<float*>(vt + KT * KS);
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wq = wave / NK, wk = wave % NK;
 
     int bh, id;
     if (!pair_order(blockIdx.x, p.B * p.H, p.tiles, p.causal, bh, id)) return;
     const int qt = p.causal ? p.tiles - 1 - id : id;
     const int h = bh % p.H, b = bh / p.H, kvh = h / p.G;
 
-    const int first_row = (qt * NW + wave) * 32, row = first_row + col;
+    const int first_row = (qt * NQ + wq) * 32, row = first_row + col;
     const bool valid = row < p.Sq;
     const int qi = min(row, p.Sq - 1), qpos = p.Sk - p.Sq + qi;
     const int pos_lo = p.Sk - p.Sq + min(first_row, p.Sq - 1), pos_hi = p.Sk - p.Sq + min(first_row + 31, p.Sq - 1);
-    const int wg_hi = p.Sk - p.Sq + min((qt + 1) * NW * 32 - 1, p.Sq - 1);
+    const int wg_hi = p.Sk - p.Sq + min((qt + 1) * NQ * 32 - 1, p.Sq - 1);
 
     const int64_t rec = ((int64_t)b * p.H + h) * p.Sq + qi;
     Frag<T> q[NC], g[NC];
@@ -57,27 +59,31 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void a
     {
         const T* qs = at<T>(p.q, b, qi, h);
         const T* gs = at<T>(p.dout, b, qi, h);
-        const T* os = at<T>(p.o, b, qi, h);
+        [[maybe_unused]] const T* os = at<T>(p.o, b, qi, h);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int d = c * 16 + half * 8;
             const bool in = valid && d < p.D;
             q[c] = in ? load8(qs + d) : zero8<T>();
             g[c] = in ? load8(gs + d) : zero8<T>();
-            const Frag<T> o = in ? load8(os + d) : zero8<T>();
+            if constexpr (NW > 1) {
+                const Frag<T> o = in ? load8(os + d) : zero8<T>();
 #pragma unroll
-            for (int j = 0; j < 8; ++j) delta = fmaf((float)g[c].v[j], (float)o.v[j], delta);
-            if constexpr (sizeof(T) == 2) {                           // what o lost when it was rounded
+                for (int j = 0; j < 8; ++j) delta = fmaf((float)g[c].v[j], (float)o.v[j], delta);
+            }
+            if constexpr (NW > 1 && sizeof(T) == 2) {                 // what o lost when it was rounded
                 const Frag<T> rest = in ? load8(reinterpret_cast<const T*>(p.stats + rec * p.stats_row + 4) + d) : zero8<T>();
 #pragma unroll
                 for (int j = 0; j < 8; ++j) delta = fmaf((float)g[c].v[j], (float)rest.v[j], delta);
             }
         }
     }
-    delta += __shfl_xor(delta, 32, 64);
-    if (valid && half == 0) p.delta[rec] = delta;
+    if constexpr (NW > 1) {
+        delta += __shfl_xor(delta, 32, 64);
+        if (valid && half == 0 && wk == 0) p.delta[rec] = delta;
+    }
     const float2 st = *reinterpret_cast<const float2*>(p.stats + rec * p.stats_row);
-    const float top = st.x, inv = valid ? st.y : 0.f, dinv = delta * inv;      // dS = 2^(s - top) (dP inv - delta inv)
+    [[maybe_unused]] const float top = st.x, inv = valid ? st.y : 0.f, dinv = delta * inv;      // dS = 2^(s - top) (dP inv - delta inv)
 
     const bool has_bias = p.table != nullptr, want = p.want_dtable != 0;
     const int R = p.R, nb = 2 * R + 1;
@@ -118,7 +124,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void a
     int t = next(0);
     if (AHEAD && t < t1) fetch(t);
     while (t < t1) {
-        const uint64_t c0 = m0;
+        const uint64_t c0 = m0, c1 = m1;
         __syncthreads();
         if (!AHEAD) fetch(t);
         sk.store(kt, tid);
@@ -127,9 +133,9 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void a
         const int tn = next(t + 1);
         if (AHEAD && tn < t1) fetch(tn);
 #pragma unroll
-        for (int n = 0; n < KT / 32; ++n) {
-            const int key0 = t * KT + n * 32;
-            const uint32_t bits = (uint32_t)(c0 >> (n * 32));
+        for (int j = 0; j < KT / 32 / NK; ++j) {
+            const int n = NK > 1 ? wk : j, key0 = t * KT + n * 32;
+            const uint32_t bits = (uint32_t)((n < 2 ? c0 : c1) >> ((n & 1) * 32));
             if (bits == 0 || first_row >= p.Sq || (p.causal && key0 > pos_hi)) continue;      // (a wave behind the last row has nothing)
             f32x16 s, dp;
 #pragma unroll
@@ -139,7 +145,26 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void a
             const int dmax = key0 + 31 - pos_lo, dmin = key0 - pos_hi;
             const bool far = dmax <= -R || dmin >= R, full = bits == 0xffffffffu && !(p.causal && key0 + 31 > pos_lo);
             const float add = has_bias ? bias[dmax <= -R ? 0 : 2 * R] : 0.f;
-            if (full && (!has_bias || (far && __builtin_fabsf(add) < kFoldBias))) {
+            if constexpr (NW == 1) {
+                // one tile has every key of a row: delta = sum P dP from the same P and dP, so that dS sums to zero over the row as it has to
+                // (dO . O, rounded by itself, left dq and dk of 3 causal keys 1.3e-6 off where P and dP put them 0.2e-6)
+                const uint32_t mine = bits >> (half * 4);
+                const int see = p.causal ? qpos - key0 - half * 4 : 1 << 30;
+                delta = 0.f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int k = acc_row(r, 0);
+                    const float bv = has_bias ? bias[max(-R, min(R, key0 + half * 4 + k - qpos)) + R] : 0.f;
+                    const float v = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale_log2, bv) - top) * inv;
+                    const bool on = ((mine >> k) & 1) != 0 && k <= see;
+                    s[r] = on ? v : 0.f;
+                    dp[r] = on ? dp[r] : 0.f;
+                    delta = fmaf(s[r], dp[r], delta);
+                }
+                delta += __shfl_xor(delta, 32, 64);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] *= dp[r] - delta;
+            } else if (full && (!has_bias || (far && __builtin_fabsf(add) < kFoldBias))) {
                 const float shift = add - top;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale_log2, shift)) * fmaf(dp[r], inv, -dinv);
@@ -191,7 +216,31 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void a
         }
         t = tn;
     }
-    if (valid) {
+    if (NW == 1 && valid && half == 0) p.delta[rec] = delta;
+    if constexpr (NK > 1) {
+        // the waves' sums are added in wave order
+        static_assert(NK * DP * 32 * 4 <= 2 * KT * KS * (int)sizeof(T), "the join must fit the tiles' room");
+        __syncthreads();
+        float* buf = reinterpret_cast<float*>(smem);                  // (NK, DP, 32)
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) buf[(wk * DP + d * 32 + acc_row(r, half)) * 32 + col] = dq[d][r];
+        __syncthreads();
+        if (valid) {
+            T* dst = at_mut<T>(p.dq, b, qi, h);
+            for (int c = (wave * 2 + half) * 4; c < p.D; c += NK * 8) {
+                float a[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    a[j] = 0.f;
+#pragma unroll
+                    for (int w = 0; w < NK; ++w) a[j] += buf[(w * DP + c + j) * 32 + col];
+                }
+                store4<T>(dst + c, a[0] * p.scale, a[1] * p.scale, a[2] * p.scale, a[3] * p.scale);
+            }
+        }
+    } else if (valid) {
         T* dst = at_mut<T>(p.dq, b, qi, h);
 #pragma unroll
         for (int d = 0; d < ND; ++d)
@@ -228,25 +277,28 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void a
     }
 }
 
-template <class T, int DP, int NW, int QT>
-__global__ __launch_bounds__(64 * NW, DP >= 64 ? 1 : 2) void attention_dkv_kernel(AttnParams p) {
-    constexpr int NT = 64 * NW, KS = lds_stride<T, DP>(), NC = DP / 16, ND = DP / 32;
-    constexpr bool AHEAD = NW > 1;      // the next tile is fetched while this one is multiplied; one-wave workgroups mostly have one tile
+template <class T, int DP, int NB, int NR, int QT>
+__global__ __launch_bounds__(64 * NB * NR, DP >= 64 ? 1 : 2) void attention_dkv_kernel(AttnParams p) {
+    constexpr int NW = NB * NR, NT = 64 * NW, KS = lds_stride<T, DP>(), NC = DP / 16, ND = DP / 32;
+    // the next tile is fetched while this one is multiplied; one-wave workgroups mostly have one tile, and 128 long fp32 rows do not fit registers
+    constexpr bool AHEAD = NW > 1 && !(NR > 1 && sizeof(T) == 4 && DP > 64);
     constexpr bool EXACT = sizeof(T) == 2 && NW == 1;      // few keys: their roundings do not average out, and there is time to multiply them too
-    constexpr int BUF = 2 * QT * KS;                                 // q and dO rows of a tile, two tiles
+    constexpr int NBUF = NR > 1 ? 1 : 2, BUF = 2 * QT * KS;          // tiles in LDS; q and dO rows of a tile
+    static_assert(NR == 1 || QT == NR * 32, "a wave has one block of 32 rows of a tile");
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* tiles = reinterpret_cast<T*>(smem);
-    float* stats = reinterpret_cast<float*>(tiles + 2 * BUF);        // (2, 3, QT): maximum, reciprocal sum, delta of the tiles' rows
-    float* biases = stats + 6 * QT;                                  // (2, 2 R + 1): of the current and the next query head
+    float* stats = reinterpret_cast<float*>(tiles + NBUF * BUF);     // (NBUF, 3, QT): maximum, reciprocal sum, delta of the tiles' rows
+    float* biases = stats + NBUF * 3 * QT;                                  // (2, 2 R + 1): of the current and the next query head
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
     int bh, kt;
     if (!pair_order(blockIdx.x, p.B * p.Hk, p.tiles, p.causal, bh, kt)) return;
     const int kvh = bh % p.Hk, b = bh / p.Hk;
-    const int key0 = (kt * NW + wave) * 32, key = key0 + col;
+    const int wb = wave / NR, wr = wave % NR;
+    const int key0 = (kt * NB + wb) * 32, key = key0 + col;
     const bool valid = key < p.Sk && (p.pad == nullptr || p.pad[(int64_t)b * p.ld_pad + key] == 0);
-    const int wg_key0 = kt * NW * 32;
+    const int wg_key0 = kt * NB * 32;
 
     Frag<T> k[NC], v[NC];
     {
@@ -281,9 +333,10 @@ __global__ __launch_bounds__(64 * NW, DP >= 64 ? 1 : 2) void attention_dkv_kerne
     auto fetch = [&](int i) {
         const int gi = i / per, h = kvh * p.G + gi, row0 = (q_first + i - gi * per) * QT;
         const int left = p.Sq - row0;
-        const uint64_t m = left >= 64 ? ~uint64_t(0) : (uint64_t(1) << left) - 1;
-        sq.load(at<T>(p.q, b, row0, h), m, 0, p.D, tid);
-        sg.load(at<T>(p.dout, b, row0, h), m, 0, p.D, tid);
+        const uint64_t m0 = left >= 64 ? ~uint64_t(0) : (uint64_t(1) << left) - 1;
+        const uint64_t m1 = left >= 128 ? ~uint64_t(0) : (left > 64 ? (uint64_t(1) << (left - 64)) - 1 : 0);
+        sq.load(at<T>(p.q, b, row0, h), m0, m1, p.D, tid);
+        sg.load(at<T>(p.dout, b, row0, h), m0, m1, p.D, tid);
         if (tid < QT) {
             const int64_t rec = ((int64_t)b * p.H + h) * p.Sq + row0 + tid;
             st = tid < left ? *reinterpret_cast<const float2*>(p.stats + rec * p.stats_row) : make_float2(0.f, 0.f);
@@ -330,11 +383,11 @@ __global__ __launch_bounds__(64 * NW, DP >= 64 ? 1 : 2) void attention_dkv_kerne
                 for (int r = 0; r < 16; ++r) { dk[d][r] = 0.f; dv[d][r] = 0.f; }
         }
     };
-    // two tiles in LDS: tile i + 1 is written while others may still read tile i, one barrier a tile
+    // two tiles in LDS: tile i + 1 is written while others may still read tile i, one barrier a tile (one tile: two barriers)
     int have = -1;
     auto put = [&](int i) {
-        T* t = tiles + (i & 1) * BUF;
-        float* stat = stats + (i & 1) * 3 * QT;
+        T* t = tiles + i % NBUF * BUF;
+        float* stat = stats + i % NBUF * 3 * QT;
         sq.store(t, tid);
         sg.store(t + QT * KS, tid);
         if (tid < QT) {
@@ -356,13 +409,14 @@ __global__ __launch_bounds__(64 * NW, DP >= 64 ? 1 : 2) void attention_dkv_kerne
     auto part = [&](int i, int end) {
         for (; i < end; ++i) {
             const int gi = i / per, row0 = (q_first + i - gi * per) * QT;
-            const T* qs = tiles + (i & 1) * BUF;
+            const T* qs = tiles + i % NBUF * BUF;
             const T* gs = qs + QT * KS;
-            const float* stat = stats + (i & 1) * 3 * QT;
+            const float* stat = stats + i % NBUF * 3 * QT;
             const float* bias = biases + (gi & 1) * (2 * R + 1);
             if (AHEAD && i + 1 < total) fetch(i + 1);
 #pragma unroll
-            for (int n = 0; n < QT / 32; ++n) {
+            for (int j = 0; j < QT / 32 / NR; ++j) {
+                const int n = NR > 1 ? wr : j;
                 const int pos0 = back + row0 + n * 32;                     // position of the tile's first query
                 if (!alive || row0 + n * 32 >= p.Sq || (p.causal && pos0 + 31 < key0)) continue;
                 f32x16 s, dp;
@@ -424,12 +478,13 @@ __global__ __launch_bounds__(64 * NW, DP >= 64 ? 1 : 2) void attention_dkv_kerne
             }
             if (i + 1 < total) {
                 if (!AHEAD) fetch(i + 1);
+                if (NBUF == 1) __syncthreads();
                 put(i + 1);
             }
             __syncthreads();
         }
     };
-    if constexpr (sizeof(T) == 4) {
+    if constexpr (sizeof(T) == 4 && NR == 1) {
         for (int i = 0; i < total;) {
             const int end = min(total, i + PART);
             part(i, end);
@@ -437,7 +492,35 @@ __global__ __launch_bounds__(64 * NW, DP >= 64 ? 1 : 2) void attention_dkv_kerne
             if (i < total) store(false);
         }
     } else part(0, total);
-    store(true);
+    if constexpr (NR == 1) {
+        store(true);
+    } else {
+        // the waves' sums are added in wave order, dk's and then dv's
+        static_assert(NR * DP * 32 * 4 <= BUF * (int)sizeof(T), "the join must fit the tiles' room");
+        float* buf = reinterpret_cast<float*>(smem);                  // (NR, DP, 32)
+        for (int which = 0; which < 2; ++which) {
+            __syncthreads();
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) buf[(wr * DP + d * 32 + acc_row(r, half)) * 32 + col] = which == 0 ? dk[d][r] : dv[d][r];
+            __syncthreads();
+            if (key < p.Sk) {
+                T* dst = at_mut<T>(which == 0 ? p.dk : p.dv, b, key, kvh);
+                const float scale = which == 0 ? p.scale : 1.f;
+                for (int c = (wr * 2 + half) * 4; c < p.D; c += NR * 8) {
+                    float a[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        a[j] = 0.f;
+#pragma unroll
+                        for (int w = 0; w < NR; ++w) a[j] += buf[(w * DP + c + j) * 32 + col];
+                    }
+                    store4<T>(dst + c, a[0] * scale, a[1] * scale, a[2] * scale, a[3] * scale);
+                }
+            }
+        }
+    }
 }
 
 // the sums by distance of every (batch row, query tile), added in index order in kSeg segments ...
@@ -504,13 +587,18 @@ __global__ __launch_bounds__(256) void attention_zero_rows_kernel(AttnTensor t, 
     at_mut<T>(t, b, tok - (int64_t)b * S, h)[d] = (T)0.f;
 }
 
-struct BPlan { int qw, kw, qtiles, ktiles; };
+// q: query rows of a workgroup by 32, qk: waves that share them, a part of the keys each; k, kr: the same of keys and query rows
+struct BPlan { int q, qk, k, kr, qtiles, ktiles; };
 BPlan plan(const vita_attention_args* a) {
     BPlan f{};
-    f.qw = a->Sq <= 32 ? 1 : 4;
-    f.kw = a->Sk <= 32 ? 1 : 4;
-    f.qtiles = (a->Sq + 32 * f.qw - 1) / (32 * f.qw);
-    f.ktiles = (a->Sk + 32 * f.kw - 1) / (32 * f.kw);
+    const int64_t qwide = (int64_t)(a->Sq + 127) / 128 * a->H * a->B, kwide = (int64_t)(a->Sk + 127) / 128 * a->Hk * a->B;
+    const int64_t rows = (int64_t)a->Sq * (a->H / a->Hk);
+    f.q = a->Sq <= 32 || (a->Sk > 32 && attention_narrow(a, qwide)) ? 1 : 4;
+    f.qk = f.q == 1 && a->Sk > 32 ? 4 : 1;
+    f.k = a->Sk <= 32 || (rows > 32 && attention_narrow(a, kwide)) ? 1 : 4;
+    f.kr = f.k == 1 && rows > 32 ? 4 : 1;
+    f.qtiles = (a->Sq + 32 * f.q - 1) / (32 * f.q);
+    f.ktiles = (a->Sk + 32 * f.k - 1) / (32 * f.k);
     return f;
 }
 size_t carve(const vita_attention_args* a, void* ws, float** delta, float** part, float** seg) {
@@ -526,21 +614,23 @@ size_t carve(const vita_attention_args* a, void* ws, float** delta, float** part
     return c.off;
 }
 
-template <class T, int DP, int NW, int KT>
+template <class T, int DP, int NQ, int NK, int KT>
 int launch_dq(const AttnParams& p, int64_t blocks, hipStream_t s) {
+    constexpr int NW = NQ * NK;
     const size_t lds = (size_t)2 * KT * lds_stride<T, DP>() * sizeof(T) + (p.table != nullptr ? (size_t)((2 * p.R + 1 + 3) & ~3) * 4 : 0) +
                        (p.want_dtable ? (size_t)NW * (32 * kDiag + ((dist_slots(p.R) + 3) & ~3)) * 4 : 0);
-    auto kernel = attention_dq_kernel<T, DP, NW, KT>;
+    auto kernel = attention_dq_kernel<T, DP, NQ, NK, KT>;
     VITA_REQUIRE(lds <= 160 * 1024, "vita_attention_bwd: %zu bytes of LDS", lds);
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * NW), lds, s, p);
     VITA_CHECK_HIP(hipGetLastError());
     return VITA_OK;
 }
-template <class T, int DP, int NW, int QT>
+template <class T, int DP, int NB, int NR, int QT>
 int launch_dkv(const AttnParams& p, int64_t blocks, hipStream_t s) {
-    const size_t lds = (size_t)4 * QT * lds_stride<T, DP>() * sizeof(T) + 6 * QT * 4 + (p.table != nullptr ? (size_t)(2 * p.R + 1) * 8 : 0);
+    constexpr int NW = NB * NR, tiles = NR > 1 ? 1 : 2;
+    const size_t lds = (size_t)2 * tiles * QT * lds_stride<T, DP>() * sizeof(T) + 3 * tiles * QT * 4 + (p.table != nullptr ? (size_t)(2 * p.R + 1) * 8 : 0);
     VITA_REQUIRE(lds <= 160 * 1024, "vita_attention_bwd: %zu bytes of LDS", lds);
-    auto kernel = attention_dkv_kernel<T, DP, NW, QT>;
+    auto kernel = attention_dkv_kernel<T, DP, NB, NR, QT>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * NW), lds, s, p);
     VITA_CHECK_HIP(hipGetLastError());
     return VITA_OK;
@@ -549,12 +639,15 @@ template <class T, int DP>
 int launch_dp(const vita_attention_args* a, AttnParams p, const BPlan& f, hipStream_t s) {
     constexpr int T4 = sizeof(T) == 2 ? 64 : 32;
     constexpr int TQ = sizeof(T) == 2 && DP < 128 ? 64 : 32;      // dq at 128: with tiles of 64 keys the prefetch does not fit two waves a SIMD
+    const int64_t qgrid = pair_grid((int64_t)a->H * a->B, f.qtiles), kgrid = pair_grid((int64_t)a->Hk * a->B, f.ktiles);
     p.tiles = f.qtiles;
-    if (f.qw == 4) VITA_TRY((launch_dq<T, DP, 4, TQ>(p, pair_grid((int64_t)a->H * a->B, f.qtiles), s)));
-    else VITA_TRY((launch_dq<T, DP, 1, 32>(p, pair_grid((int64_t)a->H * a->B, f.qtiles), s)));
+    if (f.q == 4) VITA_TRY((launch_dq<T, DP, 4, 1, TQ>(p, qgrid, s)));
+    else if (f.qk == 4) VITA_TRY((launch_dq<T, DP, 1, 4, 128>(p, qgrid, s)));
+    else VITA_TRY((launch_dq<T, DP, 1, 1, 32>(p, qgrid, s)));
     p.tiles = f.ktiles;
-    if (f.kw == 4) return launch_dkv<T, DP, 4, T4>(p, pair_grid((int64_t)a->Hk * a->B, f.ktiles), s);
-    return launch_dkv<T, DP, 1, 32>(p, pair_grid((int64_t)a->Hk * a->B, f.ktiles), s);
+    if (f.k == 4) return launch_dkv<T, DP, 4, 1, T4>(p, kgrid, s);
+    if (f.kr == 4) return launch_dkv<T, DP, 1, 4, 128>(p, kgrid, s);
+    return launch_dkv<T, DP, 1, 1, 32>(p, kgrid, s);
 }
 template <class T>
 int run(const vita_attention_args* a, AttnParams& p, float* seg, hipStream_t s) {

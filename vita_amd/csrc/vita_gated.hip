@@ -29,7 +29,7 @@ __global__ __launch_bounds__(256) void gated_product_kernel(const float* z, int6
     for (int j = 0; j < 4; ++j) o[j] = (T)(apply_act(g[j], act) * u[j]);
 }
 
-// dz and the partial sums of db (lo: also what the rounding of dz lost, 2 F further on): a workgroup has 256 features and kDzRows rows, a thread 4 features of every 4th row; 16-byte accesses
+// dz and the partial sums of db (lo: also what the rounding of dz lost, M rows further on): a workgroup has 256 features and kDzRows rows, a thread 4 features of every 4th row; 16-byte accesses
 constexpr int kDzRows = 32;
 template <class T>
 __global__ __launch_bounds__(256) void gated_dz_kernel(const float* z, int64_t ldz, const T* dh, int64_t ld_dh, T* dz, int64_t ld_dz, float* db_part, int M,
@@ -59,8 +59,8 @@ __global__ __launch_bounds__(256) void gated_dz_kernel(const float* z, int64_t l
             *reinterpret_cast<vec4*>(dz + r * ld_dz + c) = og;
             *reinterpret_cast<vec4*>(dz + r * ld_dz + F + c) = ou;
             if (lo) {
-                *reinterpret_cast<vec4*>(dz + r * ld_dz + 2 * F + c) = lg;
-                *reinterpret_cast<vec4*>(dz + r * ld_dz + 3 * F + c) = lu;
+                *reinterpret_cast<vec4*>(dz + (M + r) * ld_dz + c) = lg;
+                *reinterpret_cast<vec4*>(dz + (M + r) * ld_dz + F + c) = lu;
             }
         }
     if (db_part == nullptr) return;
@@ -77,16 +77,15 @@ __global__ __launch_bounds__(256) void gated_dz_kernel(const float* z, int64_t l
             db_part[seg * 2 * F + k * F + f] = (part[0][k][threadIdx.x] + part[1][k][threadIdx.x]) + (part[2][k][threadIdx.x] + part[3][k][threadIdx.x]);
 }
 
-// (rows, cols) -> (cols, rows) of 16-bit elements, `copies` of it side by side
-__global__ __launch_bounds__(256) void transpose16_kernel(const uint16_t* src, int64_t ld, uint16_t* dst, int64_t ldd, int rows, int cols, int copies) {
+// (rows, cols) -> (cols, rows) of 16-bit elements
+__global__ __launch_bounds__(256) void transpose16_kernel(const uint16_t* src, int64_t ld, uint16_t* dst, int64_t ldd, int rows, int cols) {
     __shared__ uint16_t t[64][66];
     const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
     for (int j = y; j < 64; j += 4)
         if (r0 + j < rows && c0 + x < cols) t[j][x] = src[(int64_t)(r0 + j) * ld + c0 + x];
     __syncthreads();
     for (int j = y; j < 64; j += 4)
-        if (c0 + j < cols && r0 + x < rows)
-            for (int k = 0; k < copies; ++k) dst[(int64_t)(c0 + j) * ldd + (int64_t)k * rows + r0 + x] = t[x][j];
+        if (c0 + j < cols && r0 + x < rows) dst[(int64_t)(c0 + j) * ldd + r0 + x] = t[x][j];
 }
 // the sum of `parts` fp32 matrices, one below the other
 __global__ __launch_bounds__(256) void to_bf16_kernel(const float* src, bf16* dst, int64_t ldd, int rows, int cols, int parts) {
@@ -99,6 +98,16 @@ __global__ __launch_bounds__(256) void to_bf16_kernel(const float* src, bf16* ds
 }
 
 // ---- the wide bf16 products ------------------------------------------------------------------------------------------------------
+// a (2 M, K) matrix whose halves both are x
+__global__ __launch_bounds__(256) void rows_twice_kernel(const bf16* x, int64_t ldx, bf16* dst, int M, int K) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n8 = K / 8, r = i / n8;
+    if (r >= M) return;
+    const int64_t c = (i - r * n8) * 8;
+    const bf16x8 v = *reinterpret_cast<const bf16x8*>(x + r * ldx + c);
+    *reinterpret_cast<bf16x8*>(dst + r * K + c) = v;
+    *reinterpret_cast<bf16x8*>(dst + (M + r) * K + c) = v;
+}
+
 struct WideOut {
     const float* bias;
     bf16* c; int64_t ldc;                 // h, or C
@@ -381,13 +390,12 @@ bool wide_product(const vita_gated_args* a) { return a->dtype == VITA_DT_BF16 &&
 // a forward call that the few-row kernel takes (z wanted: the general path, which writes it)
 bool few_rows(const vita_gated_args* a) { return a->dtype == VITA_DT_BF16 && a->z == nullptr && a->M <= kFewRows; }
 
-// bf16 gradients of few rows and few weights: dz goes into dx and dw as two bf16 numbers, for with few terms its rounding does not average
-// out (2 x 48 x 88: dx and dw 1.64 times as far off as their own rounding puts them, many terms 1.41, both parts 1.0).  It doubles the
-// products, which such calls do not notice (launches bound them) and larger ones would.
-constexpr int64_t kExactWeights = 1 << 18;
-int dz_parts(const vita_gated_args* a) { return a->dtype == VITA_DT_BF16 && a->M <= kFewRows && 2 * (int64_t)a->F * a->K <= kExactWeights ? 2 : 1; }
+// bf16 gradients of few rows: dz goes into dx and dw as two bf16 numbers, a second set of M rows, for with few terms its rounding does
+// not average out (2 x 48 x 88: dx and dw 1.64 times as far off as their own rounding puts them, 1 x 400 x 6784 1.55, many rows 1.41, both
+// parts 1.0).  Such products wait for the weights, the added rows cost little; more rows would double the products.
+int dz_parts(const vita_gated_args* a) { return a->dtype == VITA_DT_BF16 && a->M <= kFewRows && !wide_product(a) ? 2 : 1; }
 
-struct Ws { float* sk; float* z; void* dz; float* dw32; void* wt; float* db_part; float* cs; size_t bytes; };
+struct Ws { float* sk; float* z; void* dz; float* dx32; void* xx; float* dw32; void* wt; float* db_part; float* cs; size_t bytes; };
 Ws carve(const vita_gated_args* a, bool bwd, void* ws) {
     Carver c(ws);
     Ws r{};
@@ -399,8 +407,10 @@ Ws carve(const vita_gated_args* a, bool bwd, void* ws) {
     if (bwd) {
         const size_t es = a->dtype == VITA_DT_F32 ? 4 : 2, parts = dz_parts(a);
         r.dz = c.take((M * F2 * parts * es + 3) / 4);
-        if (a->dtype == VITA_DT_BF16 && a->dw != nullptr && !wide_fills(F2, K)) r.dw32 = c.take(parts * F2 * K);
-        if (a->dtype == VITA_DT_BF16 && a->dx != nullptr && !wide_fills(M, K)) r.wt = c.take((parts * F2 * K * es + 3) / 4);
+        if (a->dtype == VITA_DT_BF16 && a->dw != nullptr && !wide_fills(F2, K)) r.dw32 = c.take(F2 * K);
+        if (a->dtype == VITA_DT_BF16 && a->dx != nullptr && (parts == 2 || !wide_fills(M, K))) r.wt = c.take((F2 * K * es + 3) / 4);
+        if (parts == 2 && a->dx != nullptr) r.dx32 = c.take(parts * M * K);
+        if (parts == 2 && a->dw != nullptr) r.xx = c.take((parts * M * K * es + 3) / 4);
         // fp32 dx: W transposed once lets the product take the row-operand GEMM (2176 x 512 x 4096: 162 us on W as it lies), from as many
         // rows as the training step does so; the transpose wants W without gaps
         if (a->dtype == VITA_DT_F32 && a->dx != nullptr && a->M >= kWtMinRows && a->ldw == a->K) r.wt = c.take(F2 * K);
@@ -440,7 +450,7 @@ int preact(const vita_gated_args* a, float* z, int64_t ldz, const Ws& ws, hipStr
 
 int run_bwd(const vita_gated_args* a, void* workspace, hipStream_t s) {
     const Ws ws = carve(a, true, workspace);
-    const int M = a->M, F = a->F, F2 = 2 * a->F, K = a->K, parts = dz_parts(a), FZ = parts * F2;      // FZ: columns of dz
+    const int M = a->M, F = a->F, F2 = 2 * a->F, K = a->K, parts = dz_parts(a);
     const float* z = a->z;
     int64_t ldz = a->ldz;
     const bool wide = wide_product(a);
@@ -462,7 +472,7 @@ int run_bwd(const vita_gated_args* a, void* workspace, hipStream_t s) {
     } else if (a->dtype == VITA_DT_F32)
         hipLaunchKernelGGL(gated_dz_kernel<float>, grid, dim3(256), 0, s, z, ldz, (const float*)a->dh, a->ld_dh, (float*)ws.dz, F2, part, M, F, a->act, (int64_t)segs, false);
     else
-        hipLaunchKernelGGL(gated_dz_kernel<bf16>, grid, dim3(256), 0, s, z, ldz, (const bf16*)a->dh, a->ld_dh, (bf16*)ws.dz, FZ, part, M, F, a->act, (int64_t)segs, parts == 2);
+        hipLaunchKernelGGL(gated_dz_kernel<bf16>, grid, dim3(256), 0, s, z, ldz, (const bf16*)a->dh, a->ld_dh, (bf16*)ws.dz, F2, part, M, F, a->act, (int64_t)segs, parts == 2);
     VITA_CHECK_HIP(hipGetLastError());
     if (a->db != nullptr) VITA_TRY(vita_colsum_f32(part, F2, segs, F2, ws.cs, a->db, 0, s));
     SplitkScope sk(ws.sk, kSplitkBytes);
@@ -477,28 +487,42 @@ int run_bwd(const vita_gated_args* a, void* workspace, hipStream_t s) {
         if (a->dw != nullptr) VITA_TRY(gemm_f32(wgrad((const float*)ws.dz, F2, (const float*)a->x, a->ldx, (float*)a->dw, a->ld_dw, M, K, F2), s));
         return VITA_OK;
     }
-    if (a->dx != nullptr && wide_fills(M, K)) {
+    if (a->dx != nullptr && parts == 1 && wide_fills(M, K)) {
         WideOut o{};
         o.c = (bf16*)a->dx; o.ldc = a->ld_dx;
         VITA_TRY((launch_wide<false, true, WIDE_C>((const bf16*)ws.dz, F2, (const bf16*)a->w, a->ldw, M, K, F2, 0, o, s)));
     } else if (a->dx != nullptr) {
-        hipLaunchKernelGGL(transpose16_kernel, dim3((K + 63) / 64, (F2 + 63) / 64), dim3(256), 0, s, (const uint16_t*)a->w, a->ldw, (uint16_t*)ws.wt, (int64_t)FZ, F2, K,
-                           parts);
+        hipLaunchKernelGGL(transpose16_kernel, dim3((K + 63) / 64, (F2 + 63) / 64), dim3(256), 0, s, (const uint16_t*)a->w, a->ldw, (uint16_t*)ws.wt, (int64_t)F2, F2, K);
         VITA_CHECK_HIP(hipGetLastError());
         vita_linear_args l{};
-        l.X = (const float*)ws.dz; l.ldx = FZ; l.W = (const float*)ws.wt; l.ldw = FZ; l.M = M; l.N = K; l.K = FZ; l.ldy = K;
-        VITA_TRY(gemm_bf16_dma(l, (uint16_t*)a->dx, a->ld_dx, s));
+        l.X = (const float*)ws.dz; l.ldx = F2; l.W = (const float*)ws.wt; l.ldw = F2; l.M = parts * M; l.N = K; l.K = F2; l.ldy = K;
+        if (parts == 1) {
+            VITA_TRY(gemm_bf16_dma(l, (uint16_t*)a->dx, a->ld_dx, s));
+        } else {
+            l.Y = ws.dx32;
+            VITA_TRY(gemm_bf16_dma(l, nullptr, 0, s));
+            hipLaunchKernelGGL(to_bf16_kernel, dim3((unsigned)(((int64_t)M * K + 255) / 256)), dim3(256), 0, s, ws.dx32, (bf16*)a->dx, a->ld_dx, M, K, parts);
+            VITA_CHECK_HIP(hipGetLastError());
+        }
+    }
+    const bf16* x = (const bf16*)a->x;
+    int64_t ldx = a->ldx;
+    if (a->dw != nullptr && parts == 2) {
+        hipLaunchKernelGGL(rows_twice_kernel, dim3((unsigned)(((int64_t)M * (K / 8) + 255) / 256)), dim3(256), 0, s, x, ldx, (bf16*)ws.xx, M, K);
+        VITA_CHECK_HIP(hipGetLastError());
+        x = (const bf16*)ws.xx;
+        ldx = K;
     }
     if (a->dw != nullptr && wide_fills(F2, K)) {
         WideOut o{};
         o.c = (bf16*)a->dw; o.ldc = a->ld_dw;
-        VITA_TRY((launch_wide<true, true, WIDE_C>((const bf16*)ws.dz, F2, (const bf16*)a->x, a->ldx, F2, K, M, 0, o, s)));
+        VITA_TRY((launch_wide<true, true, WIDE_C>((const bf16*)ws.dz, F2, x, ldx, F2, K, parts * M, 0, o, s)));
     } else if (a->dw != nullptr) {
         vita_linear_args l{};
-        l.Y = ws.dw32; l.ldy = K; l.M = FZ; l.N = K; l.K = M; l.splitk_ws = ws.sk; l.splitk_ws_bytes = kSplitkBytes;
-        VITA_TRY(gemm_bf16_wgrad_tn((const uint16_t*)ws.dz, FZ, (const uint16_t*)a->x, a->ldx, l, s));
+        l.Y = ws.dw32; l.ldy = K; l.M = F2; l.N = K; l.K = parts * M; l.splitk_ws = ws.sk; l.splitk_ws_bytes = kSplitkBytes;
+        VITA_TRY(gemm_bf16_wgrad_tn((const uint16_t*)ws.dz, F2, (const uint16_t*)x, ldx, l, s));
         const int64_t n = (int64_t)F2 * K;
-        hipLaunchKernelGGL(to_bf16_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, ws.dw32, (bf16*)a->dw, a->ld_dw, F2, K, parts);
+        hipLaunchKernelGGL(to_bf16_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, ws.dw32, (bf16*)a->dw, a->ld_dw, F2, K, 1);
         VITA_CHECK_HIP(hipGetLastError());
     }
     return VITA_OK;

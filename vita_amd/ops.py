@@ -1427,9 +1427,42 @@ def _out(t: Optional[Tensor], what: str, shape, like: Tensor) -> Tensor:
         return torch.empty(shape, dtype=like.dtype, device=like.device)
     if tuple(t.shape) != tuple(shape) or t.dtype != like.dtype or t.device != like.device:
         raise L.VitaHipError(f"{what}: {t.dtype} {tuple(t.shape)} on {t.device}, expected {like.dtype} {tuple(shape)} on {like.device}")
-    if t.numel() and (t.stride(-1) != 1 or any(n > 1 and s < t.shape[-1] for n, s in zip(t.shape[:-1], t.stride()[:-1]))):
-        raise L.VitaHipError(f"{what}: needs contiguous rows that do not overlap, got strides {t.stride()}")
+    if t.numel():
+        room = 1 if t.stride(-1) == 1 else math.inf                   # elements that the smaller strides walk over
+        for s, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+            if s < room:
+                raise L.VitaHipError(f"{what}: needs contiguous rows that do not overlap, got strides {t.stride()}")
+            room = s * (n - 1) + room
     return t
+
+
+def _apart(what: str, out: Tensor, *others: Optional[Tensor], but: tuple = ()) -> None:
+    """Refuses an output that shares memory with a tensor the call reads or writes besides (`but`: which it may be, element for element)."""
+    def extent(t):
+        return t.data_ptr(), t.data_ptr() + (sum(s * (n - 1) for s, n in zip(t.stride(), t.shape)) + 1) * t.element_size()
+
+    def rows(t, d):                                                   # pitch of the rows that the dimensions from d on make, and their extent
+        lead = [s for s, n in zip(t.stride()[:d], t.shape) if n > 1]
+        pitch = min(lead, default=0)
+        inner = sum(s * (n - 1) for s, n in zip(t.stride()[d:], t.shape[d:])) + 1
+        return pitch, inner, pitch > 0 and all(s % pitch == 0 for s in lead)
+
+    def side_by_side(t, d):
+        (pa, wa, ra), (pb, wb, rb) = rows(out, d), rows(t, d)
+        gap = (t.data_ptr() - out.data_ptr()) // t.element_size()
+        return ra and rb and pa == pb and gap % pa >= wa and gap % pa + wb <= pa
+
+    if out.numel() == 0:
+        return
+    for t in others:
+        if t is None or t.numel() == 0 or t.untyped_storage().data_ptr() != out.untyped_storage().data_ptr():
+            continue
+        a, b = extent(out), extent(t)
+        if a[1] <= b[0] or b[1] <= a[0] or any(t is x and t.data_ptr() == out.data_ptr() and t.stride() == out.stride() for x in but):
+            continue
+        if t.dtype == out.dtype and t.dim() == out.dim() and any(side_by_side(t, d) for d in range(1, t.dim())):
+            continue
+        raise L.VitaHipError(f"{what}: shares memory with a tensor of the call")
 
 
 def _scratch(nbytes: int, device) -> Optional[Tensor]:
@@ -1495,6 +1528,9 @@ def _qk_norm_rope(q, k, rope, q_weight, q_bias, k_weight, k_bias, norm, eps, pos
     head, sides, keep = _norm_rope_args(q, k, rope, q_weight, q_bias, k_weight, k_bias, norm, eps, positions, "qk_norm_rope")
     qo, ko = out if out is not None else (None, None)
     qo, ko = _out(qo, "qk_norm_rope: out[0]", q.shape, q), _out(ko, "qk_norm_rope: out[1]", k.shape, k)
+    if out is not None:
+        _apart("qk_norm_rope: out[0]", qo, q, k, ko, rope, but=(q,))
+        _apart("qk_norm_rope: out[1]", ko, q, k, rope, but=(k,))
     if q.numel():
         a = L.NormRopeArgs(*head, *(L.NormRopeSide(*_bshd(x), *_bshd(y), *_NO_TENSOR, _ptr(w), _ptr(b), None, None, x.shape[2])
                                     for (x, w, b), y in zip(sides, (qo, ko))))
@@ -1507,7 +1543,8 @@ def qk_norm_rope_bwd(dq: Tensor, dk: Tensor, q: Tensor, k: Tensor, rope: Tensor,
                      k_weight: Optional[Tensor] = None, k_bias: Optional[Tensor] = None, norm: str = "layer", eps: float = 1e-5,
                      positions: Optional[Tensor] = None, out=None):
     """Backward of qk_norm_rope from the gradients of its results: (dq, dk, dq_weight, dq_bias, dk_weight, dk_bias) with respect to its
-    inputs, None for a parameter that was not given.  out: a pair of tensors for the first two (may be the gradients passed in)."""
+    inputs, None for a parameter that was not given.  out: a pair of tensors for the first two (each may be its own side's gradient or input,
+    and shares no memory with anything else)."""
     head, sides, keep = _norm_rope_args(q, k, rope, q_weight, q_bias, k_weight, k_bias, norm, eps, positions, "qk_norm_rope_bwd")
     qo, ko = out if out is not None else (None, None)
     qo, ko = _out(qo, "qk_norm_rope_bwd: out[0]", q.shape, q), _out(ko, "qk_norm_rope_bwd: out[1]", k.shape, k)
@@ -1516,6 +1553,9 @@ def qk_norm_rope_bwd(dq: Tensor, dk: Tensor, q: Tensor, k: Tensor, rope: Tensor,
         if d.shape != x.shape:
             raise L.VitaHipError(f"qk_norm_rope_bwd: {name} {tuple(d.shape)}, expected {tuple(x.shape)}")
         _act(d, f"qk_norm_rope_bwd: {name}", 4, q)
+    if out is not None:
+        _apart("qk_norm_rope_bwd: out[0]", qo, dq, dk, q, k, ko, rope, but=(dq, q))
+        _apart("qk_norm_rope_bwd: out[1]", ko, dq, dk, q, k, rope, but=(dk, k))
     dq, dk = (d if d.stride(3) == 1 else d.contiguous() for d in (dq, dk))
     if q.numel() == 0:
         for t in grads:
@@ -1554,7 +1594,7 @@ def qk_norm_rope(q: Tensor, k: Tensor, rope: Tensor, *, q_weight: Optional[Tenso
     q (B, S, H, D), k (B, S, Hk, D) of any strides with contiguous rows (the halves of a packed projection as they lie), fp32 or bf16,
     D even and at most 256.  rope (P, D / 2, 2) = (cos, sin) of every position for all heads, or (P, H * D / 2, 2) as
     RotaryPosEmbed.cache has it (frequencies dealt to the heads in order; then Hk = H).  positions: int64 (S,) or (B, S), by default
-    0 .. S - 1; a position outside the table makes its row NaN.  out: a pair of tensors for the results (may be q and k themselves).
+    0 .. S - 1; a position outside the table makes its row NaN.  out: a pair of tensors for the results (may be q and k themselves, and share no other memory).
     Differentiable in q, k and the parameters."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, q_bias, k_weight, k_bias)):
         if out is not None:
@@ -1623,8 +1663,10 @@ def _attention(q, k, v, scale, causal, key_pad, table, buckets, need_lse, out):
     o = _out(out, "attention: out", q.shape, q)
     stats = torch.empty(_stats_shape(q), dtype=torch.float32, device=q.device) if need_lse else None
     if o.numel():
-        if out is not None and not _aligned(o):
-            raise L.VitaHipError("attention: out needs 16-byte aligned rows")
+        if out is not None:
+            _apart("attention: out", o, q, k, v, key_pad, table)
+            if not _aligned(o):
+                raise L.VitaHipError("attention: out needs 16-byte aligned rows")
         a = L.AttentionArgs(*head, *_bshd(o), _ptr(stats), *tail)
         lib = L.load()
         with _On(q.device):
@@ -1636,7 +1678,7 @@ def _attention(q, k, v, scale, causal, key_pad, table, buckets, need_lse, out):
 def attention_bwd(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, o: Tensor, stats: Tensor, *, scale: Optional[float] = None, causal: bool = False,
                   key_pad: Optional[Tensor] = None, table: Optional[Tensor] = None, buckets: Optional[Tensor] = None, need_dtable: bool = True, out=None):
     """Backward of attention from the gradient of its result, the result and its row statistics (need_lse=True): (dq, dk, dv, dtable), dtable None
-    without a table.  out: tensors for the first three."""
+    without a table.  out: tensors for the first three, which share no memory with each other or what is read."""
     head, tail, keep = _attention_args(q, k, v, scale, causal, key_pad, table, buckets, "attention_bwd")
     for name, t in (("dout", dout), ("o", o)):
         _act(t, f"attention_bwd: {name}", 4, q)
@@ -1650,8 +1692,11 @@ def attention_bwd(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, o: Tensor, stat
     dq, dk, dv = out if out is not None else (None, None, None)
     dq, dk, dv = (_out(t, f"attention_bwd: out[{i}]", x.shape, q) for i, (t, x) in enumerate(((dq, q), (dk, k), (dv, v))))
     dtable = torch.empty(table.shape, dtype=table.dtype, device=table.device) if table is not None and need_dtable else None
-    if out is not None and not all(t.numel() == 0 or _aligned(t) for t in (dq, dk, dv)):
-        raise L.VitaHipError("attention_bwd: out needs 16-byte aligned rows")
+    if out is not None:
+        for i, t in enumerate((dq, dk, dv)):
+            _apart(f"attention_bwd: out[{i}]", t, q, k, v, o, dout, stats, key_pad, table, *(dq, dk, dv)[i + 1:])
+            if t.numel() and not _aligned(t):
+                raise L.VitaHipError("attention_bwd: out needs 16-byte aligned rows")
     if q.numel() == 0 or k.numel() == 0:
         for t in (dq, dk, dv, dtable):
             if t is not None:
@@ -1693,7 +1738,7 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, scale: Optional[float] = None,
     need_lse: also the row statistics that attention_bwd takes, (B, H, Sq, n) fp32: [..., 0] a maximum m of the row's scores times log2 e,
     [..., 1] r = 1 / sum 2 ** (score log2 e - m), so that log sum exp = m ln 2 - ln r, (0, 0) for a query without keys; bf16: behind them
     what the result lost when it was rounded (probabilities are then multiplied in two bf16 parts: the result is nearer than without).
-    out: the result's tensor.  Differentiable in q, k, v and table."""
+    out: the result's tensor, which shares no memory with the others.  Differentiable in q, k, v and table."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, table)):
         if out is not None:
             raise L.VitaHipError("attention: out= cannot be used where a gradient is wanted")
@@ -1730,8 +1775,10 @@ def _gated_linear(x, w, b, act, need_saved, out):
     # fp32 calls keep the pre-activations; bf16 calls form them again in the backward pass (vita_gated.hip)
     z = torch.empty((x.shape[0], 2 * F), dtype=torch.float32, device=x.device) if need_saved and x.dtype == torch.float32 else None
     if h.numel():
-        if out is not None and not _aligned(h):
-            raise L.VitaHipError("gated_linear: out needs 16-byte aligned rows")
+        if out is not None:
+            _apart("gated_linear: out", h, x, w, b)
+            if not _aligned(h):
+                raise L.VitaHipError("gated_linear: out needs 16-byte aligned rows")
         a.h, a.ldh = h.data_ptr(), _ld(h)
         if z is not None:
             a.z, a.ldz = z.data_ptr(), 2 * F
@@ -1796,7 +1843,7 @@ class _GatedLinear(torch.autograd.Function):
 def gated_linear(x: Tensor, w: Tensor, b: Optional[Tensor] = None, act: str = "silu", *, need_saved: bool = False, out: Optional[Tensor] = None):
     """act(x @ w[:F].T + b[:F]) * (x @ w[F:].T + b[F:]): both projections of a gated feed-forward block, the activation and the product.
     x (M, K), w (2 F, K), fp32 or bf16, K and F multiples of 8; b (2 F) fp32 or None; act: relu, gelu, gelu_tanh, silu or mish.
-    need_saved: also what gated_linear_bwd takes (None where it needs nothing).  out: the result's tensor.  Differentiable in x, w and b."""
+    need_saved: also what gated_linear_bwd takes (None where it needs nothing).  out: the result's tensor, apart from x and w.  Differentiable in x, w and b."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, b)):
         if out is not None or need_saved:
             raise L.VitaHipError("gated_linear: out= and need_saved= cannot be used where a gradient is wanted")

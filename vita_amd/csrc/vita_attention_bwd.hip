@@ -6,6 +6,8 @@
 // Two kernels, each owning what it sums, so nothing is added by atomics and the bits do not depend on the run:
 //   dq:  a wave owns 32 query rows and walks the keys (scores transposed as in the forward pass; also delta and the bias gradient);
 //   dkv: a wave owns 32 keys and walks the query rows of every query head of its key head (scores untransposed, a lane owns one key).
+// With few such workgroups the 4 waves of one share 32 rows (keys) and take a part of the other axis each; their sums are joined in LDS
+// in wave order (attention_narrow in vita_attention.h).  Where one tile has all the keys, delta is sum P dP.
 // Each forms S and dP again: 7 products of Sq x Sk x D against 5 for one kernel that would have to add dQ or dK, dV across workgroups.
 // In both the second operand of the next product is the score tile's own registers (vita_attention.h), so P and dS never touch LDS.
 //
@@ -35,6 +37,9 @@ __global__ __launch_bounds__(64 * NQ * NK, (sizeof(T) == 4 && DP >= 64) || (NK >
     constexpr bool AHEAD = NW > 1 && !(NK > 1 && sizeof(T) == 4 && DP > 96);
     constexpr bool EXACT = sizeof(T) == 2 && NQ == 1;      // few rows or keys: roundings do not average out, and there is time to multiply them too
     static_assert(NK == 1 || KT == NK * 32, "a wave has one block of 32 keys of a tile");
+    // fp32: a row's dS has to sum to zero; what it does sum to is delta's rounding, which the far keys' bias gradient (P of it a row) and the
+    // dkv kernel's delta are rid of afterwards (96 x 52 x 239 keys, 3 heads, radius 16: the table's gradient 1.8e-6 -> 0.4e-6 off)
+    constexpr bool FIX = sizeof(T) == 4 && NW > 1;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* kt = reinterpret_cast<T*>(smem);
     T* vt = kt + KT * KS;
@@ -80,7 +85,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (sizeof(T) == 4 && DP >= 64) || (NK >
     }
     if constexpr (NW > 1) {
         delta += __shfl_xor(delta, 32, 64);
-        if (valid && half == 0 && wk == 0) p.delta[rec] = delta;
+        if (!FIX && valid && half == 0 && wk == 0) p.delta[rec] = delta;
     }
     const float2 st = *reinterpret_cast<const float2*>(p.stats + rec * p.stats_row);
     [[maybe_unused]] const float top = st.x, inv = valid ? st.y : 0.f, dinv = delta * inv;      // dS = 2^(s - top) (dP inv - delta inv)
@@ -89,7 +94,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (sizeof(T) == 4 && DP >= 64) || (NK >
     const int R = p.R, nb = 2 * R + 1;
     float* diag = bias + (has_bias ? ((nb + 3) & ~3) : 0) + wave * (want ? 32 * kDiag + ((dist_slots(R) + 3) & ~3) : 0);
     float* dist = diag + 32 * kDiag;
-    float far_lo = 0.f, far_hi = 0.f;
+    float far_lo = 0.f, far_hi = 0.f, left = 0.f, p_lo = 0.f, p_hi = 0.f;      // left: what the row's dS sums to; p: sums of P / inv over far keys
     if (has_bias) load_bias<T>(p, bias, h, 1, tid, NT);
     if (want)
         for (int i = lane; i < dist_slots(R); i += 64) dist[i] = 0.f;
@@ -145,6 +150,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (sizeof(T) == 4 && DP >= 64) || (NK >
             const int dmax = key0 + 31 - pos_lo, dmin = key0 - pos_hi;
             const bool far = dmax <= -R || dmin >= R, full = bits == 0xffffffffu && !(p.causal && key0 + 31 > pos_lo);
             const float add = has_bias ? bias[dmax <= -R ? 0 : 2 * R] : 0.f;
+            float psum = 0.f, ssum = 0.f;
             if constexpr (NW == 1) {
                 // one tile has every key of a row: delta = sum P dP from the same P and dP, so that dS sums to zero over the row as it has to
                 // (dO . O, rounded by itself, left dq and dk of 3 causal keys 1.3e-6 off where P and dP put them 0.2e-6)
@@ -167,7 +173,11 @@ __global__ __launch_bounds__(64 * NQ * NK, (sizeof(T) == 4 && DP >= 64) || (NK >
             } else if (full && (!has_bias || (far && __builtin_fabsf(add) < kFoldBias))) {
                 const float shift = add - top;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale_log2, shift)) * fmaf(dp[r], inv, -dinv);
+                for (int r = 0; r < 16; ++r) {
+                    const float e = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale_log2, shift));
+                    s[r] = e * fmaf(dp[r], inv, -dinv);
+                    if constexpr (FIX) psum += e;
+                }
             } else {
                 const uint32_t mine = bits >> (half * 4);
                 const int see = p.causal ? qpos - key0 - half * 4 : 1 << 30;
@@ -175,9 +185,16 @@ __global__ __launch_bounds__(64 * NQ * NK, (sizeof(T) == 4 && DP >= 64) || (NK >
                 for (int r = 0; r < 16; ++r) {
                     const int k = acc_row(r, 0);
                     const float bv = has_bias ? bias[max(-R, min(R, key0 + half * 4 + k - qpos)) + R] : 0.f;
-                    const float v = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale_log2, bv) - top) * fmaf(dp[r], inv, -dinv);
-                    s[r] = ((mine >> k) & 1) != 0 && k <= see ? v : 0.f;
+                    const bool on = ((mine >> k) & 1) != 0 && k <= see;
+                    const float e = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale_log2, bv) - top);
+                    s[r] = on ? e * fmaf(dp[r], inv, -dinv) : 0.f;
+                    if constexpr (FIX) psum += on ? e : 0.f;
                 }
+            }
+            if (FIX || (want && far)) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) ssum += s[r];
+                left += ssum;
             }
             {
                 const Frag<T> df[2] = {pack8<T>(s, 0), pack8<T>(s, 1)};
@@ -191,11 +208,8 @@ __global__ __launch_bounds__(64 * NQ * NK, (sizeof(T) == 4 && DP >= 64) || (NK >
             }
             if (want) {
                 if (far) {
-                    float a = 0.f;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) a += s[r];
-                    if (dmax <= -R) far_lo += a;
-                    else far_hi += a;
+                    if (dmax <= -R) { far_lo += ssum; p_lo += psum; }
+                    else { far_hi += ssum; p_hi += psum; }
                 } else {
                     // rows are queries here: lane t sums the elements (i, i + t - 31)
 #pragma unroll
@@ -216,7 +230,21 @@ __global__ __launch_bounds__(64 * NQ * NK, (sizeof(T) == 4 && DP >= 64) || (NK >
         }
         t = tn;
     }
-    if (NW == 1 && valid && half == 0) p.delta[rec] = delta;
+    if constexpr (FIX) {
+        left += __shfl_xor(left, 32, 64);
+        if constexpr (NK > 1) {
+            float* red = reinterpret_cast<float*>(smem);              // (NK, 32)
+            __syncthreads();
+            if (half == 0) red[wk * 32 + col] = left;
+            __syncthreads();
+            left = 0.f;
+#pragma unroll
+            for (int w = 0; w < NK; ++w) left += red[w * 32 + col];
+        }
+        far_lo -= p_lo * inv * left;
+        far_hi -= p_hi * inv * left;
+    }
+    if ((NW == 1 || FIX) && valid && half == 0 && wk == 0) p.delta[rec] = delta + left;
     if constexpr (NK > 1) {
         // the waves' sums are added in wave order
         static_assert(NK * DP * 32 * 4 <= 2 * KT * KS * (int)sizeof(T), "the join must fit the tiles' room");

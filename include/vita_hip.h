@@ -698,7 +698,8 @@ size_t vita_qk_norm_rope_bwd_workspace_bytes(const vita_norm_rope_args* args);
 int vita_qk_norm_rope_bwd(const vita_norm_rope_args* args, void* workspace, size_t workspace_bytes, vita_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------
- * vita_attention — softmax attention (F.scaled_dot_product_attention, attention.py:58) with a learned relative position bias:
+ * vita_attention — softmax attention (F.scaled_dot_product_attention, attention.py:58) with a learned relative position bias (results share no memory with what is
+ * read):
  *   s[i, j] = scale * q_i . k_j + table[buckets[clamp(j - (i + Sk - Sq), -radius, radius) + radius], h],   o_i = sum_j softmax_j(s) v_j
  *   q, o (B, Sq, H, D), k, v (B, Sk, Hk, D): head h reads key head h / (H / Hk).  The queries are the LAST Sq of the Sk positions.
  *   causal: key j is seen by query i when j <= i + Sk - Sq.  key_pad (B, Sk) bytes, row stride ld_pad: nonzero = the key does not
@@ -710,8 +711,8 @@ int vita_qk_norm_rope_bwd(const vita_norm_rope_args* args, void* workspace, size
  *   its scores times log2 e and 1 / sum 2^(score log2 e - M), so that log sum exp = M ln 2 - ln(second), (0, 0) for a query without keys
  *   (two numbers, because their log sum exp would lose the sum where a mask of the type's lowest value makes every score of a row
  *   huge); behind them, in bf16 calls, what o lost when it was rounded.
- * Backward: dq, dk, dv (written), dtable (num_buckets, H) of the call's dtype (NULL = not wanted), from dout, o and stats; every sum
- * in a fixed order.
+ * Backward: dq, dk, dv (written), dtable (num_buckets, H) of the call's dtype (NULL = not wanted), from dout, o and stats, none of which they
+ * share memory with; every sum in a fixed order.
  * --------------------------------------------------------------------------------------- */
 typedef struct vita_attention_args {
     int32_t dtype, B, H, Hk, Sq, Sk, D, causal;
@@ -738,7 +739,7 @@ int vita_attention_bwd(const vita_attention_args* args, void* workspace, size_t 
 /* ---------------------------------------------------------------------------------------
  * vita_gated_linear — the gated feed-forward product: z = x . w^T + b, h = act(z[:, :F]) * z[:, F:]
  *   x (M, K), w (2F, K): rows 0 .. F - 1 the gate, F .. 2F - 1 the up projection, b (2F) fp32 or NULL, h (M, F); act VITA_ACT_RELU ..
- *   VITA_ACT_MISH.  K and F multiples of 8; rows 16-byte aligned.
+ *   VITA_ACT_MISH.  K and F multiples of 8 up to 2^20; rows 16-byte aligned; results share no memory with what is read.
  *   z: NULL, or (M, 2F) fp32 that receives the pre-activations.
  * Backward from dh (M, F):  dz = [dh * z_up * act'(z_gate) | dh * act(z_gate)],  dx = dz . w,  dw = dz^T . x,  db = column sums of dz
  *   (dx (M, K) and dw (2F, K) of the call's dtype, db fp32; each may be NULL).  z: the forward call's, or NULL = formed again from x and w.

@@ -8,15 +8,22 @@
 // the previous one is multiplied).  With few rows the key axis is also split over workgroups, whose (O, m, l) a second launch joins in
 // split order.  Query heads that share a key head share a row tile there (row = query * G + head), so the cache is read once.
 // Tiles whose keys are all padded, or all ahead of a causal row, are skipped without being read.
+//
+// Measured: bf16, 2 x 4095 tokens, 16 heads of 128, causal 205 us (137 GFLOP, 0.67 PFLOP/s: the matrix unit is busy half of the time, the
+// exponentials of a wave run beside the products of its SIMD's other one); fp32, 16 x 1000 of 8 heads of 64 291 us (113 TFLOP/s, 0.74 of
+// a large product's); one new token, 32 over 8 heads of 128, 25 rows of up to 4097 bf16 keys: 46 us for 210 MB (4.6 TB/s) and 4 us for the join.
 // P is rounded to bf16 for the second product of bf16 calls (the matrix unit's operand type); sums, maxima and O stay fp32.  EXACT: what
 // the rounding lost is multiplied too, and O's own rounding is kept beside the row statistics: the backward pass's sum dO . O needs O
 // nearer than bf16 where a row has few keys (dq, dk and the bias gradient came out 1.5 - 1.8 times as far off as their own rounding puts
-// them, with it 1.4).  The few-row kernels always do it (they wait for memory), the long one in training only (205 against 247 us,
-// 2 x 4095 rows, 16 heads of 128, causal).
+// them, with it 1.4).  The few-row kernels always do it (they wait for memory), the long one in training only and for the first 256 keys
+// that a row meets: among more keys the roundings average out (2 x 4095 rows, 16 heads of 128, causal: 205 us without, 227 with, 247 for
+// all keys).
 #include "vita_attention.h"
 
 namespace vita {
 namespace {
+
+constexpr int kExactTiles = 4;      // ... of 64 keys
 
 template <class T, int DP, int NQ, int NK, int KW, bool EXACT>
 __global__ __launch_bounds__(64 * NQ * NK, sizeof(T) == 4 && DP >= 96 ? 1 : 2) void attention_fwd_kernel(AttnParams p) {
@@ -89,6 +96,7 @@ __global__ __launch_bounds__(64 * NQ * NK, sizeof(T) == 4 && DP >= 96 ? 1 : 2) v
 
     int t = next(t0);
     if (AHEAD && t < t1) fetch(t);
+    [[maybe_unused]] int seen = 0;
     while (t < t1) {
         const uint64_t c0 = m0, c1 = m1;
         __syncthreads();           // the previous tile has been read by every wave
@@ -165,6 +173,7 @@ __global__ __launch_bounds__(64 * NQ * NK, sizeof(T) == 4 && DP >= 96 ? 1 : 2) v
             }
             // probabilities of 16 keys at a time, so that a step's exponentials run beside the previous step's products
             Frag<T> pf, rest;
+            const bool near = NQ == 1 || seen++ < kExactTiles;
             pipelined<T, 2 * NS, ND>(
                 [&](int i, int d) { return col_frag<T, DP>(vt, wk * KW + i * 16, d * 32, lane); },
                 [&](int i, int d, const Frag<T>& a) {
@@ -178,10 +187,12 @@ __global__ __launch_bounds__(64 * NQ * NK, sizeof(T) == 4 && DP >= 96 ? 1 : 2) v
                         }
                         l += sum;
                         pf = pack8<T>(sn, i & 1);
-                        if constexpr (EXACT) rest = pack8_rest(sn, i & 1, pf);
+                        if constexpr (EXACT)
+                            if (near) rest = pack8_rest(sn, i & 1, pf);
                     }
                     mma(to[d], a, pf);
-                    if constexpr (EXACT) mma(to[d], a, rest);
+                    if constexpr (EXACT)
+                        if (near) mma(to[d], a, rest);
                 });
             if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -315,7 +326,7 @@ Plan plan(const vita_attention_args* a) {
     const int G = a->H / a->Hk;
     // few rows of a head over many keys: the key axis is what there is to share out
     const bool few = (int64_t)a->Sq * G <= 64 && a->Sk > 128;
-    const bool narrow = a->Sk > 128 && attention_narrow(a, (int64_t)(a->Sq + 127) / 128 * a->H * a->B);
+    const bool narrow = a->Sk > 128 && attention_narrow(a, (int64_t)(a->Sq + 127) / 128 * a->H * a->B, false);
     f.mode = few || narrow ? FWD_KEYS4 : (a->Sq <= 32 ? FWD_ROWS1 : FWD_ROWS4);
     f.pack = few ? G : 1;
     f.rows = a->Sq * f.pack;

@@ -14,6 +14,9 @@
 // are.  A lane keeps its columns' weight and bias in registers over the rows that its group walks.  The weight gradients: a lane sums
 // its columns over its rows, a workgroup joins its groups through LDS and writes one partial row, a second launch adds the partial
 // rows in index order: no atomics, the same bits every time.
+//
+// 2 x 8191 tokens, 32 + 8 heads of 128, bf16: forward 82 us (335 MB, 4.1 TB/s), backward 126 us (503 MB,
+// 4.0 TB/s) and 5 us for the weights' partial rows; a copy of that size reaches 4.7 TB/s.  128 x 17 tokens of 16 heads of 64: launches.
 #include "vita_host.h"
 
 namespace vita {

@@ -294,17 +294,28 @@ __global__ __launch_bounds__(64 * NQ * NK, (sizeof(T) == 4 && DP >= 64) || (NK >
         const int stride = 32 * kDiag + ((dist_slots(R) + 3) & ~3);
         const float* all = dist - wave * stride;
         float* out = p.dist_part + ((int64_t)(b * p.tiles + qt) * p.H + h) * nb;
+        float lo = 0.f, hi = 0.f;                 // what lies beyond the radius belongs to its ends: 62 slots on either side
+        if (wave == 0) {
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                lo += lane < 62 ? all[w * stride + lane] : 0.f;
+                hi += lane < 62 ? all[w * stride + 2 * R + 63 + lane] : 0.f;
+            }
+            lo = wave_sum(lo);
+            hi = wave_sum(hi);
+        }
         for (int i = tid; i < nb; i += NT) {
             float a = 0.f;
-            for (int w = 0; w < NW; ++w) {
-                const float* s = all + w * stride;
-                a += s[i + 62];
-                if (i == 0)
-                    for (int e = 0; e < 62; ++e) a += s[e];
-                if (i == 2 * R)
-                    for (int e = 2 * R + 63; e < dist_slots(R); ++e) a += s[e];
-            }
-            out[i] = a;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) a += all[w * stride + i + 62];
+            if (i == 0) a += R > 0 ? lo : lo + hi;
+            if (i != 2 * R || R == 0) out[i] = a;
+        }
+        if (tid == 0 && R > 0) {
+            float a = hi;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) a += all[w * stride + 2 * R + 62];
+            out[2 * R] = a;
         }
     }
 }

@@ -308,11 +308,10 @@ __device__ __forceinline__ bool pair_order(int id, int pairs, int tiles, int by_
 // 46 / 147 -> 20 / 54 us; 1 x 1000 of 128 (64) fp32 155 / 519 -> 60 / 203, bf16 29 / 102 -> 22 / 64; 2 x 2048 of 64 causal (256) fp32
 // 168 / 578 -> 105 / 386; all rows alike (1 x 4095 of 64, 256) 334 / 1186 -> 333 / 1321; one tile long (32 x 100 causal, 256) 19 / 53 ->
 // 19 / 89; of 128 causal (2 x 2000 x 16 heads, 512) 340 / 1127 -> 447 / 1640.
-inline bool attention_narrow(const vita_attention_args* a, int64_t wide, bool dq) {
+inline bool attention_narrow(const vita_attention_args* a, int64_t wide) {
     if (a->dtype == VITA_DT_F32 && a->D > 96 && a->radius > 240) return false;                // its tiles and the bias gradient's rows fill the LDS
-    // (bf16 tiles are short of delivery sooner: 4 x 1000 padded tokens of 64, 256: 28 / 84 -> 36 / 111; the dq kernel of padded rows, whose
-    // wide form has the shortest run of the three: 148 -> 171, where dkv goes from 188 to 132)
-    const bool uneven = a->dtype == VITA_DT_F32 && (a->causal || (a->key_pad != nullptr && !dq));
+    // (bf16 tiles are short of delivery sooner: 4 x 1000 padded tokens of 64, 256: 28 / 84 -> 36 / 111)
+    const bool uneven = a->dtype == VITA_DT_F32 && (a->causal || a->key_pad != nullptr);
     return wide < 256 || (wide < 512 && uneven && a->D <= 64 && a->Sq >= 512 && a->Sk >= 512);
 }
 

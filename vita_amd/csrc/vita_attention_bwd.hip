@@ -11,7 +11,7 @@
 // Each forms S and dP again: 7 products of Sq x Sk x D against 5 for one kernel that would have to add dQ or dK, dV across workgroups.
 // In both the second operand of the next product is the score tile's own registers (vita_attention.h), so P and dS never touch LDS.
 //
-// Measured: bf16, 2 x 4095 tokens, 16 heads of 128, causal: dq 325 us (206 GFLOP, 0.63 PFLOP/s), dkv 525 us (275 GFLOP, 0.52 PFLOP/s: its
+// Measured: bf16, 2 x 4095 tokens, 16 heads of 128, causal: dq 309 us (206 GFLOP, 0.67 PFLOP/s), dkv 525 us (275 GFLOP, 0.52 PFLOP/s: its
 // accumulators and k, v fragments leave one wave a SIMD, and the LDS serves 44 KB a wave and 32 x 32 scores, 1400 cycles of a CU for 4 waves
 // against 1024 of the matrix units); fp32, 16 x 1000 of 8 heads of 64: both 1200 us (115 GFLOP, 96 TFLOP/s, 0.63 of a large product's).
 //
@@ -636,9 +636,9 @@ BPlan plan(const vita_attention_args* a) {
     BPlan f{};
     const int64_t qwide = (int64_t)(a->Sq + 127) / 128 * a->H * a->B, kwide = (int64_t)(a->Sk + 127) / 128 * a->Hk * a->B;
     const int64_t rows = (int64_t)a->Sq * (a->H / a->Hk);
-    f.q = a->Sq <= 32 || (a->Sk > 32 && attention_narrow(a, qwide, true)) ? 1 : 4;
+    f.q = a->Sq <= 32 || (a->Sk > 32 && attention_narrow(a, qwide)) ? 1 : 4;
     f.qk = f.q == 1 && a->Sk > 32 ? 4 : 1;
-    f.k = a->Sk <= 32 || (rows > 32 && attention_narrow(a, kwide, false)) ? 1 : 4;
+    f.k = a->Sk <= 32 || (rows > 32 && attention_narrow(a, kwide)) ? 1 : 4;
     f.kr = f.k == 1 && rows > 32 ? 4 : 1;
     f.qtiles = (a->Sq + 32 * f.q - 1) / (32 * f.q);
     f.ktiles = (a->Sk + 32 * f.k - 1) / (32 * f.k);

@@ -326,7 +326,7 @@ Plan plan(const vita_attention_args* a) {
     const int G = a->H / a->Hk;
     // few rows of a head over many keys: the key axis is what there is to share out
     const bool few = (int64_t)a->Sq * G <= 64 && a->Sk > 128;
-    const bool narrow = a->Sk > 128 && attention_narrow(a, (int64_t)(a->Sq + 127) / 128 * a->H * a->B, false);
+    const bool narrow = a->Sk > 128 && attention_narrow(a, (int64_t)(a->Sq + 127) / 128 * a->H * a->B);
     f.mode = few || narrow ? FWD_KEYS4 : (a->Sq <= 32 ? FWD_ROWS1 : FWD_ROWS4);
     f.pack = few ? G : 1;
     f.rows = a->Sq * f.pack;

@@ -7,7 +7,7 @@
 //   dq:  a wave owns 32 query rows and walks the keys (scores transposed as in the forward pass; also delta and the bias gradient);
 //   dkv: a wave owns 32 keys and walks the query rows of every query head of its key head (scores untransposed, a lane owns one key).
 // With few such workgroups the 4 waves of one share 32 rows (keys) and take a part of the other axis each; their sums are joined in LDS
-// in wave order (attention_narrow in vita_attention.h).  Where one tile has all the keys, delta is sum P dP.
+// in wave order (attention_narrow in vita_attention.h).  Where 32 keys are all that the rows have, delta is sum P dP.
 // Each forms S and dP again: 7 products of Sq x Sk x D against 5 for one kernel that would have to add dQ or dK, dV across workgroups.
 // In both the second operand of the next product is the score tile's own registers (vita_attention.h), so P and dS never touch LDS.
 //
@@ -89,7 +89,6 @@ __global__ __launch_bounds__(64 * NQ * NK, (sizeof(T) == 4 && DP >= 64) || (NK >
     }
     if constexpr (NW > 1) {
         delta += __shfl_xor(delta, 32, 64);
-        if (!FIX && valid && half == 0 && wk == 0) p.delta[rec] = delta;
     }
     const float2 st = *reinterpret_cast<const float2*>(p.stats + rec * p.stats_row);
     [[maybe_unused]] const float top = st.x, inv = valid ? st.y : 0.f, dinv = delta * inv;      // dS = 2^(s - top) (dP inv - delta inv)
@@ -132,6 +131,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (sizeof(T) == 4 && DP >= 64) || (NK >
     };
     int t = next(0);
     if (AHEAD && t < t1) fetch(t);
+    [[maybe_unused]] bool first = true;
     while (t < t1) {
         const uint64_t c0 = m0, c1 = m1;
         __syncthreads();
@@ -141,6 +141,9 @@ __global__ __launch_bounds__(64 * NQ * NK, (sizeof(T) == 4 && DP >= 64) || (NK >
         __syncthreads();
         const int tn = next(t + 1);
         if (AHEAD && tn < t1) fetch(tn);
+        // all the keys that these rows have lie in this tile's first 32 (bf16: one-wave kernels only, its long one has no registers to spare)
+        const bool single = NW == 1 || (FIX && first && tn >= t1 && (c0 >> 32) == 0 && c1 == 0);
+        first = false;
 #pragma unroll
         for (int j = 0; j < KT / 32 / NK; ++j) {
             const int n = NK > 1 ? wk : j, key0 = t * KT + n * 32;
@@ -155,8 +158,8 @@ __global__ __launch_bounds__(64 * NQ * NK, (sizeof(T) == 4 && DP >= 64) || (NK >
             const bool far = dmax <= -R || dmin >= R, full = bits == 0xffffffffu && !(p.causal && key0 + 31 > pos_lo);
             const float add = has_bias ? bias[dmax <= -R ? 0 : 2 * R] : 0.f;
             float psum = 0.f, ssum = 0.f;
-            if constexpr (NW == 1) {
-                // one tile has every key of a row: delta = sum P dP from the same P and dP, so that dS sums to zero over the row as it has to
+            if (single) {
+                // delta = sum P dP from the same P and dP, so that dS sums to zero over the row as it has to
                 // (dO . O, rounded by itself, left dq and dk of 3 causal keys 1.3e-6 off where P and dP put them 0.2e-6)
                 const uint32_t mine = bits >> (half * 4);
                 const int see = p.causal ? qpos - key0 - half * 4 : 1 << 30;
@@ -198,7 +201,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (sizeof(T) == 4 && DP >= 64) || (NK >
             if (FIX || (want && far)) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) ssum += s[r];
-                left += ssum;
+                if constexpr (FIX) left += ssum;
             }
             {
                 const Frag<T> df[2] = {pack8<T>(s, 0), pack8<T>(s, 1)};
@@ -248,7 +251,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (sizeof(T) == 4 && DP >= 64) || (NK >
         far_lo -= p_lo * inv * left;
         far_hi -= p_hi * inv * left;
     }
-    if ((NW == 1 || FIX) && valid && half == 0 && wk == 0) p.delta[rec] = delta + left;
+    if (valid && half == 0 && wk == 0) p.delta[rec] = delta + left;
     if constexpr (NK > 1) {
         // the waves' sums are added in wave order
         static_assert(NK * DP * 32 * 4 <= 2 * KT * KS * (int)sizeof(T), "the join must fit the tiles' room");

@@ -41,9 +41,9 @@ __global__ __launch_bounds__(64 * NQ * NK, (sizeof(T) == 4 && DP >= 64) || (NK >
     constexpr bool AHEAD = NW > 1 && !(NK > 1 && sizeof(T) == 4 && DP > 96);
     constexpr bool EXACT = sizeof(T) == 2 && NQ == 1;      // few rows or keys: roundings do not average out, and there is time to multiply them too
     static_assert(NK == 1 || KT == NK * 32, "a wave has one block of 32 keys of a tile");
-    // fp32: a row's dS has to sum to zero; what it does sum to is delta's rounding, which the far keys' bias gradient (P of it a row) and the
+    // a row's dS has to sum to zero (not in bf16 of 128, which has no registers for it); what it does sum to is delta's rounding, which the far keys' bias gradient (P of it a row) and the
     // dkv kernel's delta are rid of afterwards (96 x 52 x 239 keys, 3 heads, radius 16: the table's gradient 1.8e-6 -> 0.4e-6 off)
-    constexpr bool FIX = sizeof(T) == 4 && NW > 1;
+    constexpr bool FIX = (sizeof(T) == 4 || DP < 128) && NW > 1;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* kt = reinterpret_cast<T*>(smem);
     T* vt = kt + KT * KS;

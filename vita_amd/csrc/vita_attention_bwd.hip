@@ -116,7 +116,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (sizeof(T) == 4 && DP >= 64) || (NK >
     auto next = [&](int t) {
         for (; t < t1; ++t) {
             mask.tile<KT>(t, m0, m1);
-            if (m0 != 0) break;
+            if ((m0 | m1) != 0) break;               // tiles of 128 keys: two words
         }
         return t;
     };

@@ -385,7 +385,8 @@ __global__ __launch_bounds__(64 * NB * NR, DP >= 64 ? 1 : 2) void attention_dkv_
         sg.load(at<T>(p.dout, b, row0, h), m0, m1, p.D, tid);
         if (tid < QT) {
             const int64_t rec = ((int64_t)b * p.H + h) * p.Sq + row0 + tid;
-            st = tid < left ? *reinterpret_cast<const float2*>(p.stats + rec * p.stats_row) : make_float2(0.f, 0.f);
+            // rows behind the last: 2^(anything - inf) = 0, whatever the bias
+            st = tid < left ? *reinterpret_cast<const float2*>(p.stats + rec * p.stats_row) : make_float2(kInf, 0.f);
             st_d = tid < left ? p.delta[rec] : 0.f;
         }
     };
@@ -503,7 +504,8 @@ __global__ __launch_bounds__(64 * NB * NR, DP >= 64 ? 1 : 2) void attention_dkv_
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             const float bv = has_bias ? bias[max(-R, min(R, key - pos0 - acc_row(r + j, half))) + R] : 0.f;
-                            const bool on = valid && acc_row(r + j, 0) >= see;
+                            // (rows without keys and behind the last: their distance's bias may be infinite or NaN)
+                            const bool on = valid && acc_row(r + j, 0) >= see && i4[j] != 0.f;
                             const float pr = __builtin_amdgcn_exp2f(fmaf(s[r + j], p.scale_log2, bv) - m4[j]) * i4[j];
                             s[r + j] = on ? pr : 0.f;
                             dp[r + j] = on ? pr * (dp[r + j] - d4[j]) : 0.f;

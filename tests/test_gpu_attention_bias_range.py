@@ -1,5 +1,5 @@
-"""ops.attention's learned bias over its whole range: large entries and entries that no pair of tokens meets, against the 64-bit forms and
-bounds of tests/block_ops_reference.py."""
+"""ops.attention's learned bias over its whole range: large entries, entries that no pair of tokens meets, and every radius up to the largest,
+against the 64-bit forms and bounds of tests/block_ops_reference.py."""
 import pytest
 import torch
 
@@ -62,3 +62,21 @@ def test_entries_of_distances_that_no_pair_has(dtype, entry, Sq, Sk):
     far = torch.arange(-R, R + 1)
     buckets[(far <= -Sk) | (far > Sq - 1)] = 9 if entry == "outside" else 3
     _check(q, k, v, g, table=table, buckets=buckets.to(DEV))
+
+
+# ---- the radius -------------------------------------------------------------------------------------------------------------------
+def _radius(dtype, R, Sq, Sk, H, Hk, D):
+    g = torch.Generator().manual_seed(R + Sq)
+    q, k, v = _randn(g, 2, Sq, H, D, dtype=dtype), _randn(g, 2, Sk, Hk, D, dtype=dtype), _randn(g, 2, Sk, Hk, D, dtype=dtype)
+    bias = dict(table=_randn(g, 32, H, dtype=dtype), buckets=torch.randint(0, 32, (2 * R + 1,), generator=g, dtype=torch.int32).to(DEV))
+    pad = torch.zeros(2, Sk, dtype=torch.bool)
+    pad[1, Sk // 3:] = True
+    _check(q, k, v, g, causal=R % 2 == 0, key_pad=pad.to(DEV), **bias)
+
+
+@pytest.mark.parametrize("R", [240, 241, 243, 244, 256, 1024])
+@pytest.mark.parametrize("Sq", [1, 17, 32, 70])
+@pytest.mark.parametrize("Sk", [64, 300])
+@pytest.mark.parametrize("D", [96, 128])
+def test_backward_at_every_radius(R, Sq, Sk, D):
+    _radius(torch.float32, R, min(Sq, Sk), Sk, 2, 2, D)

@@ -58,8 +58,13 @@ __device__ __forceinline__ int acc_row(int r, int half) { return (r >> 2) * 8 + 
 // the stride is an odd number of 16 bytes.  The transposed reads of bf16 take 4 rows x 64 bytes at a time, which share no more than two
 // to a bank where the stride is 48, 80, 176 or 208 bytes beyond a multiple of 256.  (XORed pieces in place of padding free both of
 // conflicts, but want an address register for every piece: the dq kernel spilled and went from 340 to 374 us, 2 x 4096 x 16 heads of 128.)
-template <class T, int DP> constexpr int lds_stride() {
-    return DP + (sizeof(T) == 2 && DP % 64 == 0 ? 24 : 16 / (int)sizeof(T));
+constexpr int lds_stride_of(int element, int DP) { return DP + (element == 2 && DP % 64 == 0 ? 24 : 16 / element); }
+template <class T, int DP> constexpr int lds_stride() { return lds_stride_of((int)sizeof(T), DP); }
+constexpr size_t kLds = 160 * 1024;                                                     // of a workgroup
+// bytes of `tiles` tiles of 128 rows of D elements, as the kernels whose waves share out an axis keep them
+inline size_t tiles128_bytes(int dtype, int D, int tiles) {
+    const int es = dtype == VITA_DT_F32 ? 4 : 2;
+    return (size_t)tiles * 128 * lds_stride_of(es, (D + 31) / 32 * 32) * es;
 }
 // the 16-byte piece `piece` of a row
 template <class T, int DP>

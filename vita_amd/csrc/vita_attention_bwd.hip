@@ -635,13 +635,20 @@ __global__ __launch_bounds__(256) void attention_zero_rows_kernel(AttnTensor t, 
     at_mut<T>(t, b, tok - (int64_t)b * S, h)[d] = (T)0.f;
 }
 
+// LDS of a dq workgroup beside its tiles: the bias by distance, and each wave's score tile and sums by distance
+size_t dq_bias_bytes(bool table, bool want, int R, int waves) {
+    return (table ? (size_t)((2 * R + 1 + 3) & ~3) * 4 : 0) + (want ? (size_t)waves * (32 * kDiag + ((dist_slots(R) + 3) & ~3)) * 4 : 0);
+}
+
 // q: query rows of a workgroup by 32, qk: waves that share them, a part of the keys each; k, kr: the same of keys and query rows
 struct BPlan { int q, qk, k, kr, qtiles, ktiles; };
 BPlan plan(const vita_attention_args* a) {
     BPlan f{};
     const int64_t qwide = (int64_t)(a->Sq + 127) / 128 * a->H * a->B, kwide = (int64_t)(a->Sk + 127) / 128 * a->Hk * a->B;
     const int64_t rows = (int64_t)a->Sq * (a->H / a->Hk);
-    f.q = a->Sq <= 32 || (a->Sk > 32 && attention_narrow(a, qwide)) ? 1 : 4;
+    // (fp32 heads above 96 with the bias gradient of a radius from 244 on do not fit that form)
+    const bool fits = tiles128_bytes(a->dtype, a->D, 2) + dq_bias_bytes(a->table != nullptr, a->dtable != nullptr, a->radius, 4) <= kLds;
+    f.q = (a->Sk <= 32 ? a->Sq <= 32 : fits && (a->Sq <= 32 || attention_narrow(a, qwide))) ? 1 : 4;
     f.qk = f.q == 1 && a->Sk > 32 ? 4 : 1;
     f.k = a->Sk <= 32 || (rows > 32 && attention_narrow(a, kwide)) ? 1 : 4;
     f.kr = f.k == 1 && rows > 32 ? 4 : 1;
@@ -665,10 +672,9 @@ size_t carve(const vita_attention_args* a, void* ws, float** delta, float** part
 template <class T, int DP, int NQ, int NK, int KT>
 int launch_dq(const AttnParams& p, int64_t blocks, hipStream_t s) {
     constexpr int NW = NQ * NK;
-    const size_t lds = (size_t)2 * KT * lds_stride<T, DP>() * sizeof(T) + (p.table != nullptr ? (size_t)((2 * p.R + 1 + 3) & ~3) * 4 : 0) +
-                       (p.want_dtable ? (size_t)NW * (32 * kDiag + ((dist_slots(p.R) + 3) & ~3)) * 4 : 0);
+    const size_t lds = (size_t)2 * KT * lds_stride<T, DP>() * sizeof(T) + dq_bias_bytes(p.table != nullptr, p.want_dtable != 0, p.R, NW);
     auto kernel = attention_dq_kernel<T, DP, NQ, NK, KT>;
-    VITA_REQUIRE(lds <= 160 * 1024, "vita_attention_bwd: %zu bytes of LDS", lds);
+    VITA_REQUIRE(lds <= kLds, "vita_attention_bwd: %zu bytes of LDS", lds);
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * NW), lds, s, p);
     VITA_CHECK_HIP(hipGetLastError());
     return VITA_OK;
@@ -677,7 +683,7 @@ template <class T, int DP, int NB, int NR, int QT>
 int launch_dkv(const AttnParams& p, int64_t blocks, hipStream_t s) {
     constexpr int NW = NB * NR, tiles = NR > 1 ? 1 : 2;
     const size_t lds = (size_t)2 * tiles * QT * lds_stride<T, DP>() * sizeof(T) + 3 * tiles * QT * 4 + (p.table != nullptr ? (size_t)(2 * p.R + 1) * 8 : 0);
-    VITA_REQUIRE(lds <= 160 * 1024, "vita_attention_bwd: %zu bytes of LDS", lds);
+    VITA_REQUIRE(lds <= kLds, "vita_attention_bwd: %zu bytes of LDS", lds);
     auto kernel = attention_dkv_kernel<T, DP, NB, NR, QT>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * NW), lds, s, p);
     VITA_CHECK_HIP(hipGetLastError());

@@ -1,5 +1,5 @@
-"""ops.attention's learned bias over its whole range: large entries, entries that no pair of tokens meets, and every radius up to the largest,
-against the 64-bit forms and bounds of tests/block_ops_reference.py."""
+"""ops.attention's learned bias over its whole range: large entries, entries that no pair of tokens meets, and every radius up to the largest
+with many query heads to a key head, against the 64-bit forms and bounds of tests/block_ops_reference.py."""
 import pytest
 import torch
 
@@ -80,3 +80,12 @@ def _radius(dtype, R, Sq, Sk, H, Hk, D):
 @pytest.mark.parametrize("D", [96, 128])
 def test_backward_at_every_radius(R, Sq, Sk, D):
     _radius(torch.float32, R, min(Sq, Sk), Sk, 2, 2, D)
+
+
+@pytest.mark.parametrize("dtype,G", [(torch.float32, 4), (torch.float32, 8), (torch.float32, 12), (torch.float32, 32), (torch.bfloat16, 16), (torch.bfloat16, 64)])
+@pytest.mark.parametrize("R", [128, 432, 664, 1024])
+@pytest.mark.parametrize("D", [64, 128])
+def test_packed_heads_at_every_radius(dtype, G, R, D):
+    """Few rows of many query heads to a key head: one of 300 and of 129 keys."""
+    _radius(dtype, R, 1, 300, G, 1, D)
+    _radius(dtype, R, max(1, 64 // G), 129, 2 * G, 2, D)

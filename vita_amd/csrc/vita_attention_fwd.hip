@@ -318,6 +318,9 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p) {
     }
 }
 
+// LDS of the form whose 4 waves share out the keys, with the bias of `pack` heads
+size_t keys4_bytes(int dtype, int D, int pack, int R) { return tiles128_bytes(dtype, D, 2) + 4 * 64 * 4 + (size_t)pack * (2 * R + 1) * 4; }
+
 enum { FWD_ROWS4 = 0, FWD_ROWS1 = 1, FWD_KEYS4 = 2 };
 struct Plan { int mode, pack, rows, tiles, splits, tiles_per_split; int64_t blocks; };
 
@@ -328,7 +331,10 @@ Plan plan(const vita_attention_args* a) {
     const bool few = (int64_t)a->Sq * G <= 64 && a->Sk > 128;
     const bool narrow = a->Sk > 128 && attention_narrow(a, (int64_t)(a->Sq + 127) / 128 * a->H * a->B);
     f.mode = few || narrow ? FWD_KEYS4 : (a->Sq <= 32 ? FWD_ROWS1 : FWD_ROWS4);
+    // as many heads to a row tile as leave their biases room beside the tiles (fp32 heads of 128, a radius of 1024: 3)
     f.pack = few ? G : 1;
+    if (a->table != nullptr)
+        while (f.pack > 1 && (G % f.pack != 0 || keys4_bytes(a->dtype, a->D, f.pack, a->radius) > kLds)) --f.pack;
     f.rows = a->Sq * f.pack;
     const int per = f.mode == FWD_ROWS4 ? 128 : 32;
     f.tiles = (f.rows + per - 1) / per;
@@ -350,7 +356,7 @@ template <class T, int DP, int NQ, int NK, int KW, bool EXACT>
 int launch(const AttnParams& p, int64_t blocks, hipStream_t s) {
     const size_t lds = (size_t)2 * KW * NK * lds_stride<T, DP>() * sizeof(T) + (NK > 1 ? NK * 64 * 4 : 0) +
                        (p.table != nullptr ? (size_t)p.pack * (2 * p.R + 1) * 4 : 0);
-    VITA_REQUIRE(lds <= 160 * 1024, "vita_attention: radius %d with %d heads to a key head needs %zu bytes of LDS", p.R, p.pack, lds);
+    VITA_REQUIRE(lds <= kLds, "vita_attention: %zu bytes of LDS", lds);
     auto kernel = attention_fwd_kernel<T, DP, NQ, NK, KW, EXACT>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * NQ * NK), lds, s, p);
     VITA_CHECK_HIP(hipGetLastError());

@@ -349,6 +349,7 @@ __device__ __forceinline__ void store_stats(float* stats, float m, float r) {
 }
 
 int attention_check(const vita_attention_args* a, bool bwd, const char* who);
+bool attention_sizes_ok(const vita_attention_args* a);      // whether a size query's sizes are ones that a call would take
 void attention_fill(const vita_attention_args* a, AttnParams& p);
 
 }  // namespace vita

@@ -751,7 +751,7 @@ using namespace vita;
 extern "C" {
 
 size_t vita_attention_bwd_workspace_bytes(const vita_attention_args* a) {
-    if (a == nullptr || a->B <= 0 || a->Sq <= 0 || a->Sk <= 0 || a->H < 1) return 0;
+    if (!attention_sizes_ok(a) || a->Sk == 0) return 0;
     float *d, *p, *s;
     return carve(a, nullptr, &d, &p, &s);
 }

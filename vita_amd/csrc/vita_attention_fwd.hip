@@ -389,6 +389,12 @@ int launch_type(const AttnParams& p, const Plan& f, hipStream_t s) {
 
 }  // namespace
 
+bool attention_sizes_ok(const vita_attention_args* a) {
+    return a != nullptr && a->B > 0 && a->Sq > 0 && a->Sk >= 0 && a->Sq <= (1 << 28) && a->Sk <= (1 << 28) && a->Hk >= 1 && a->H >= a->Hk &&
+           a->H % a->Hk == 0 && (int64_t)a->Sq * (a->H / a->Hk) <= (1 << 28) && a->D >= 8 && a->D <= 128 && a->D % 8 == 0 &&
+           ((a->table == nullptr && a->dtable == nullptr) || (a->radius >= 0 && a->radius <= kMaxRadius));
+}
+
 int attention_check(const vita_attention_args* a, bool bwd, const char* who) {
     VITA_REQUIRE(a != nullptr, "%s: null args", who);
     VITA_REQUIRE(a->dtype == VITA_DT_F32 || a->dtype == VITA_DT_BF16, "%s: unknown dtype %d", who, a->dtype);
@@ -444,7 +450,7 @@ extern "C" {
 int32_t vita_attention_stats_row(int32_t dtype, int32_t D) { return stats_row(dtype == VITA_DT_BF16, D); }
 
 size_t vita_attention_workspace_bytes(const vita_attention_args* a) {
-    if (a == nullptr || a->B <= 0 || a->Sq <= 0 || a->Hk <= 0 || a->H < a->Hk || a->H % a->Hk != 0 || a->Sk < 0) return 0;
+    if (!attention_sizes_ok(a)) return 0;
     const Plan f = plan(a);
     if (f.splits == 1) return 0;
     Carver c(nullptr);

@@ -205,37 +205,26 @@ __global__ __launch_bounds__(64 * NQ * NK, sizeof(T) == 4 && DP >= 96 ? 1 : 2) v
     }
     l += __shfl_xor(l, 32, 64);
 
-    const int64_t rec = ((int64_t)b * p.H + head0 + g) * p.Sq + qi, nrec = (int64_t)p.B * p.H * p.Sq;
-    if constexpr (NK == 1) {
+    const int64_t rec = ((int64_t)b * p.H + head0 + g) * p.Sq + qi;
+    if constexpr (NK == 1) {                                    // (the keys are never split here)
         const float inv = l == 0.f ? 0.f : 1.0f / l;
         if (valid) {
             T* dst = at_mut<T>(p.o, b, qi, head0 + g);
-            float* part = p.splits > 1 ? p.part_o + (split * nrec + rec) * p.D : nullptr;
 #pragma unroll
             for (int d = 0; d < ND; ++d)
 #pragma unroll
                 for (int r = 0; r < 16; r += 4) {
                     const int c = d * 32 + acc_row(r, half);
                     if (c < p.D) {
-                        if (part != nullptr) {
-                            store4<float>(part + c, o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]);
-                        } else {
-                            const float v0 = o[d][r] * inv, v1 = o[d][r + 1] * inv, v2 = o[d][r + 2] * inv, v3 = o[d][r + 3] * inv;
-                            store4<T>(dst + c, v0, v1, v2, v3);
-                            if (sizeof(T) == 2 && p.stats != nullptr) store_rest4(p.stats + rec * p.stats_row, c, v0, v1, v2, v3);
-                        }
+                        const float v0 = o[d][r] * inv, v1 = o[d][r + 1] * inv, v2 = o[d][r + 2] * inv, v3 = o[d][r + 3] * inv;
+                        store4<T>(dst + c, v0, v1, v2, v3);
+                        if (sizeof(T) == 2 && p.stats != nullptr) store_rest4(p.stats + rec * p.stats_row, c, v0, v1, v2, v3);
                     }
                 }
-            if (half == 0) {
-                if (part != nullptr) {
-                    p.part_ml[(split * nrec + rec) * 2] = m;
-                    p.part_ml[(split * nrec + rec) * 2 + 1] = l;
-                } else if (p.stats != nullptr) {
-                    store_stats<T>(p.stats + rec * p.stats_row, m == -kInf ? 0.f : m, inv);
-                }
-            }
+            if (half == 0 && p.stats != nullptr) store_stats<T>(p.stats + rec * p.stats_row, m == -kInf ? 0.f : m, inv);
         }
     } else {
+        const int64_t nrec = (int64_t)p.B * p.H * p.Sq;
         // join the waves: every wave scales its O to the common maximum, the four are added in wave order
         if (half == 0) {
             ml[(wk * 32 + col) * 2] = m;

@@ -1505,6 +1505,8 @@ def _norm_rope_args(q, k, rope, q_weight, q_bias, k_weight, k_bias, norm, eps, p
     Hk = k.shape[2]
     if k.shape[0] != B or k.shape[1] != S or k.shape[3] != D:
         raise L.VitaHipError(f"{who}: q {tuple(q.shape)} and k {tuple(k.shape)} differ in more than their heads")
+    if H < 1 or Hk < 1:
+        raise L.VitaHipError(f"{who}: q {tuple(q.shape)} and k {tuple(k.shape)}: each needs a head")
     if norm not in _NORMS:
         raise L.VitaHipError(f"{who}: norm {norm!r}, expected one of {sorted(_NORMS)}")
     _f32(rope, f"{who}: rope")

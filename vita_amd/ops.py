@@ -1415,6 +1415,12 @@ def _aligned(t: Tensor) -> bool:
     return True
 
 
+def _on_border(t: Tensor, nbytes: int = 16) -> Tensor:
+    """A contiguous tensor that starts on a border of so many bytes (a slice of a flat buffer need not: it is copied)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % nbytes == 0 else t.clone()
+
+
 def _aligned_rows(t: Tensor) -> Tensor:
     if _aligned(t) and (t.shape[1] <= 1 or t.stride(1) < 1 << 23):
         return t
@@ -1512,7 +1518,7 @@ def _norm_rope_args(q, k, rope, q_weight, q_bias, k_weight, k_bias, norm, eps, p
     _f32(rope, f"{who}: rope")
     if rope.dim() != 3 or rope.shape[2] != 2 or rope.device != dev or D % 2 or rope.shape[1] not in (D // 2, H * D // 2):
         raise L.VitaHipError(f"{who}: rope {tuple(rope.shape)} on {rope.device}, expected (positions, {D // 2} or {H * D // 2}, 2) on {dev}")
-    rope = rope.contiguous()
+    rope = _on_border(rope, 8)
     ld = 0
     if positions is not None:
         if positions.dtype != torch.int64 or positions.device != dev or tuple(positions.shape) not in ((S,), (1, S), (B, S)):
@@ -1690,7 +1696,7 @@ def attention_bwd(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, o: Tensor, stat
     rows = _stats_shape(q)
     if tuple(stats.shape) != rows or stats.device != q.device:
         raise L.VitaHipError(f"attention_bwd: stats {tuple(stats.shape)} on {stats.device}, expected {rows} on {q.device}")
-    dout, o, stats = _aligned_rows(dout), _aligned_rows(o), stats.contiguous()
+    dout, o, stats = _aligned_rows(dout), _aligned_rows(o), _on_border(stats)
     dq, dk, dv = out if out is not None else (None, None, None)
     dq, dk, dv = (_out(t, f"attention_bwd: out[{i}]", x.shape, q) for i, (t, x) in enumerate(((dq, q), (dk, k), (dv, v))))
     dtable = torch.empty(table.shape, dtype=table.dtype, device=table.device) if table is not None and need_dtable else None
@@ -1762,6 +1768,7 @@ def _gated_args(x, w, b, act, who):
     if act not in _ACTS:
         raise L.VitaHipError(f"{who}: activation {act!r}, expected one of {sorted(_ACTS)}")
     b = _param(b, f"{who}: b", (2 * F,), x.device)
+    b = _on_border(b) if b is not None else None
     x, w = _gated_rows(x), _gated_rows(w)
     a = L.GatedArgs(_DT[x.dtype], _ACTS[act], M, F, K, x.data_ptr(), _ld(x), w.data_ptr(), _ld(w), _ptr(b))
     return a, (x, w, b), F
@@ -1813,6 +1820,7 @@ def gated_linear_bwd(dh: Tensor, x: Tensor, w: Tensor, b: Optional[Tensor], act:
         _f32(saved, "gated_linear_bwd: saved")
         if tuple(saved.shape) != (M, 2 * F) or saved.device != x.device or not saved.is_contiguous():
             raise L.VitaHipError(f"gated_linear_bwd: saved {tuple(saved.shape)} on {saved.device}, expected contiguous {(M, 2 * F)} on {x.device}")
+        saved = _on_border(saved)
         a.z, a.ldz = saved.data_ptr(), 2 * F
     a.dh, a.ld_dh = dh.data_ptr(), _ld(dh)
     a.dx, a.ld_dx = (dx.data_ptr() if dx is not None else None), K

@@ -122,6 +122,8 @@ class _GatedMlp(nn.Module):
 
     def forward(self, x):
         if self.kernels and x.is_cuda:
+            if torch.is_autocast_enabled("cuda") and x.dtype != torch.float64:          # what autocast does to an nn.Linear's input
+                x = x.to(torch.get_autocast_dtype("cuda"))
             h = ops.gated_linear(x.reshape(-1, x.shape[-1]), self.fc1.weight.to(x.dtype), self.fc1.bias.float(), "gelu_tanh")
             return self.fc2(h.view(*x.shape[:-1], -1))
         gate, up = self.fc1(x).chunk(2, dim=-1)

@@ -660,7 +660,9 @@ int vita_compute_loss_meanflow_f32(const vita_meanflow_policy_weights* w, const 
 /* ---------------------------------------------------------------------------------------
  * Operators of the transformer blocks (flare/models/attention.py, models/transformer/blocks.py; the modules are
  * vita_amd/encoders.py).  dtype is that of the activations (and, where said, of a table or weight); strides are in elements; the last
- * dimension of every tensor is contiguous.  Statistics, softmax and sums are fp32, each result is rounded once.
+ * dimension of every tensor is contiguous.  Statistics, softmax and sums are fp32.  fp32 calls round each result once and nothing before
+ * it.  bf16 calls round each result once, and besides what the matrix unit takes as bf16 operands of a later product: the attention's
+ * probabilities P and dS, the gated product's dz (which of them keep a second bf16 part is said below).
  * --------------------------------------------------------------------------------------- */
 enum { VITA_DT_F32 = 0, VITA_DT_BF16 = 1 };
 enum { VITA_NORM_LAYER = 0, /* (x - mean) / sqrt(var + eps): nn.LayerNorm(head_dim), attention.py:38-39 */
@@ -711,6 +713,10 @@ int vita_qk_norm_rope_bwd(const vita_norm_rope_args* args, void* workspace, size
  *   its scores times log2 e and 1 / sum 2^(score log2 e - M), so that log sum exp = M ln 2 - ln(second), (0, 0) for a query without keys
  *   (two numbers, because their log sum exp would lose the sum where a mask of the type's lowest value makes every score of a row
  *   huge); behind them, in bf16 calls, what o lost when it was rounded.
+ *   bf16: with Sq <= 32, and where there are too few rows for the CUs, P goes into the product with V as two bf16 parts; else as two for
+ *   the first 256 keys that a row meets in calls with stats, as one behind them and in calls without (whose o can differ in the last bit).
+ *   dS goes into dq in the same way as P in calls without stats, P and dS into dv and dk as one part (two where Sk and the rows of a key
+ *   head are at most 32).  Gradients are up to 1.4 times as far off as their own rounding puts them.
  * Backward: dq, dk, dv (written), dtable (num_buckets, H) of the call's dtype (NULL = not wanted), from dout, o and stats, none of which they
  * share memory with; every sum in a fixed order.
  * --------------------------------------------------------------------------------------- */
@@ -743,7 +749,7 @@ int vita_attention_bwd(const vita_attention_args* args, void* workspace, size_t 
  *   z: NULL, or (M, 2F) fp32 that receives the pre-activations.
  * Backward from dh (M, F):  dz = [dh * z_up * act'(z_gate) | dh * act(z_gate)],  dx = dz . w,  dw = dz^T . x,  db = column sums of dz
  *   (dx (M, K) and dw (2F, K) of the call's dtype, db fp32; each may be NULL).  z: the forward call's, or NULL = formed again from x and w.
- *   Every sum is in a fixed order.
+ *   Every sum is in a fixed order.  bf16: dz is rounded to bf16 for dx and dw (two parts up to 64 rows), db is summed before that.
  * --------------------------------------------------------------------------------------- */
 typedef struct vita_gated_args {
     int32_t dtype, act, M, F, K;

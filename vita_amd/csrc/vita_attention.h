@@ -312,7 +312,8 @@ __device__ __forceinline__ bool pair_order(int id, int pairs, int tiles, int by_
 // longest rows twice the mean, all share it.  Forward / backward, 8 heads, wide -> narrow: 1 x 512 tokens of 64 (32 workgroups) fp32
 // 46 / 147 -> 20 / 54 us; 1 x 1000 of 128 (64) fp32 155 / 519 -> 60 / 203, bf16 29 / 102 -> 22 / 64; 2 x 2048 of 64 causal (256) fp32
 // 168 / 578 -> 105 / 386; all rows alike (1 x 4095 of 64, 256) 334 / 1186 -> 333 / 1321; one tile long (32 x 100 causal, 256) 19 / 53 ->
-// 19 / 89; of 128 causal (2 x 2000 x 16 heads, 512) 340 / 1127 -> 447 / 1640.
+// 19 / 89; of 128 causal (2 x 2000 x 16 heads, 512) 340 / 1127 -> 447 / 1640.  (The second clause's edges lie somewhere between these
+// points: 100 and 512 tokens, heads of 64 and 128, 256 and 512 workgroups.)
 inline bool attention_narrow(const vita_attention_args* a, int64_t wide) {
     if (a->dtype == VITA_DT_F32 && a->D > 96 && a->radius > 240) return false;                // its tiles and the bias gradient's rows fill the LDS
     // (bf16 tiles are short of delivery sooner: 4 x 1000 padded tokens of 64, 256: 28 / 84 -> 36 / 111)

@@ -11,7 +11,7 @@
 // Each forms S and dP again: 7 products of Sq x Sk x D against 5 for one kernel that would have to add dQ or dK, dV across workgroups.
 // In both the second operand of the next product is the score tile's own registers (vita_attention.h), so P and dS never touch LDS.
 //
-// Measured: bf16, 2 x 4095 tokens, 16 heads of 128, causal: dq 309 us (206 GFLOP, 0.67 PFLOP/s), dkv 525 us (275 GFLOP, 0.52 PFLOP/s: its
+// Measured: bf16, 2 x 4095 tokens, 16 heads of 128, causal: dq 317 us (206 GFLOP, 0.65 PFLOP/s), dkv 531 us (275 GFLOP, 0.52 PFLOP/s: its
 // accumulators and k, v fragments leave one wave a SIMD, and the LDS serves 44 KB a wave and 32 x 32 scores, 1400 cycles of a CU for 4 waves
 // against 1024 of the matrix units); fp32, 16 x 1000 of 8 heads of 64: both 1200 us (115 GFLOP, 96 TFLOP/s, 0.63 of a large product's).
 //
@@ -42,7 +42,9 @@ __global__ __launch_bounds__(64 * NQ * NK, (sizeof(T) == 4 && DP >= 64) || (NK >
     constexpr bool EXACT = sizeof(T) == 2 && NQ == 1;      // few rows or keys: roundings do not average out, and there is time to multiply them too
     static_assert(NK == 1 || KT == NK * 32, "a wave has one block of 32 keys of a tile");
     // a row's dS has to sum to zero (not in bf16 of 128, which has no registers for it); what it does sum to is delta's rounding, which the far keys' bias gradient (P of it a row) and the
-    // dkv kernel's delta are rid of afterwards (96 x 52 x 239 keys, 3 heads, radius 16: the table's gradient 1.8e-6 -> 0.4e-6 off)
+    // dkv kernel's delta are rid of afterwards (96 x 52 x 239 keys, 3 heads, radius 16: the table's gradient 1.8e-6 -> 0.4e-6 off).
+    // dq and the near diagonals keep it, for that would take a product more: fp32 rows whose only two keys lie in different tiles come out
+    // up to 1.1e-6 off, three keys 0.9e-6 (formed from P dP 0.3e-6)
     constexpr bool FIX = (sizeof(T) == 4 || DP < 128) && NW > 1;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* kt = reinterpret_cast<T*>(smem);

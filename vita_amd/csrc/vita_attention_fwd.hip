@@ -16,7 +16,7 @@
 // the rounding lost is multiplied too, and O's own rounding is kept beside the row statistics: the backward pass's sum dO . O needs O
 // nearer than bf16 where a row has few keys (dq, dk and the bias gradient came out 1.5 - 1.8 times as far off as their own rounding puts
 // them, with it 1.4).  The few-row kernels always do it (they wait for memory), the long one in training only and for the first 256 keys
-// that a row meets: among more keys the roundings average out (2 x 4095 rows, 16 heads of 128, causal: 205 us without, 227 with, 247 for
+// that a row meets: among more keys the roundings average out (2 x 4095 rows, 16 heads of 128, causal: 205 us without, 223 with, 247 for
 // all keys).
 #include "vita_attention.h"
 

@@ -3,15 +3,17 @@
 // bf16 products that fill the chip run on the 256 x 256 tile of vita_gemm_bf16_wide.h: a tile's columns are 128 features' gate and up
 // projections, a wave's two column blocks the same 32 features, so both are in one lane's registers and the epilogue writes h alone.
 // Backward: the same product again with another epilogue (reads dh, writes dz = [dg | du] in bf16 and fp32 partial sums for db), then
-// dx = dz W and dw = dz^T x on the operands as they lie.  Forming z again costs 2 of 8 products but keeps nothing between the passes:
-// saved in bf16 it would round the slopes' arguments, saved in fp32 it would move 4 M F bytes twice.  dz is rounded to bf16 because the
-// matrix unit takes bf16 operands; db is summed before that rounding.
+// dx = dz W and dw = dz^T x on the operands as they lie.  Forming z again trades time for memory: 8191 x 2048 x 8192 takes 647 us for it
+// where z in fp32, written and read once, would move 1.07 GB (228 us at a copy's rate), but nothing is kept between the passes (z is 8 M F
+// bytes, 0.54 GB there, four times h; in bf16 it would round the slopes' arguments).  dz is rounded to bf16 because the matrix unit takes
+// bf16 operands; db is summed before that rounding.
 // Up to 64 bf16 rows: a kernel of its own, bound by reading the weights once.
 // Everything else goes over z (M, 2F) in fp32 with the library's GEMMs and one elementwise pass: fp32 (where the product runs at a
 // sixteenth of the rate and saving z is the cheap choice) and small bf16 calls.
 //
-// Measured: bf16 8191 x 2048 x 8192 541 us forward, 612 dz, 484 dx, 500 dw (550 GFLOP each, 0.9 - 1.14 PFLOP/s); fp32 2176 x 512 x 2048
-// 115 us z (80 TFLOP/s), 12 us h, 20 us dz, 5 us db, 6 + 115 us dx, 103 us dw; few rows 25 x 2048 x 8192 bf16 18 us (67 MB, 3.7 TB/s).
+// Measured, median (best) of ten: bf16 8191 x 2048 x 8192 577 (533) us forward, 647 (600) dz, 511 (467) dx, 559 (511) dw (550 GFLOP each,
+// 0.85 - 1.08 PFLOP/s); fp32 2176 x 512 x 2048 116 us z (79 TFLOP/s), 11 us h, 20 us dz, 5 us db, 6 + 107 + 7 us dx, 94 + 8 us dw; few
+// rows 25 x 2048 x 8192 bf16 18 us (67 MB, 3.7 TB/s).
 #include <type_traits>
 
 #include "vita_gemm_bf16_wide.h"

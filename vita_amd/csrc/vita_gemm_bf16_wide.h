@@ -9,8 +9,9 @@
 // One wait and one barrier a k-tile: when tile t is multiplied, t + 1 has landed or is about to, and the requests run 3 (two COL
 // operands: 4) tiles ahead: what bounds the loop is the latency of lines that no workgroup of the XCD has touched yet, and the clock that
 // the power limit leaves (1.8 - 2.1 GHz in a run of such products).  A wave's k-step is 8 MFMAs (256 cycles) on 6 KB of LDS reads.
-// Measured, 550 GFLOP each: X W^T 8191 x 16384 x 2048 with the activation's epilogue 541 us, dY W 484 us (1.14 PFLOP/s), dY^T X 16384 x
-// 2048 x 8191 485 - 531 us; k tiles of 64 in two stages: 547 / 495 / 590 us; 5 stages of ROW tiles were slower, 4 of COL tiles 550 us.
+// Measured, 550 GFLOP each, median (best) of ten: X W^T 8191 x 16384 x 2048 with the activation's epilogue 577 (533) us, dY W 511 (467) us
+// (1.08 PFLOP/s), dY^T X 16384 x 2048 x 8191 559 (511) us; the best with k tiles of 64 in two stages: 547 / 495 / 590 us, with 4 stages of
+// COL tiles 550 us; 5 stages of ROW tiles were slower.
 #pragma once
 #include <type_traits>
 

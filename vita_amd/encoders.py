@@ -10,9 +10,10 @@ same parameter / buffer names (so the reference's checkpoints load), same arithm
 17-token attention are torch-ROCm ops (rocBLAS / ATen) by default: the encoder is 4 % of a training step's FLOPs and off the sampler
 path.  kernels=True runs the head norms with the rotation, the attention and the gated feed-forward product of its blocks as the
 library's kernels instead (ops.qk_norm_rope, ops.attention, ops.gated_linear; same formulas, other rounding; forward and backward of 128 x
-17 tokens, 512 wide, 4 layers, fp32: 4.2 ms against 5.6, with both options below 3.9 ms against 7.6); on the CPU such a module computes
-them in torch.  Two options of a block that the reference has not: gated=True (act(gate) * up in the feed-forward, fc1 twice as
-wide) and rel_buckets > 0 (a learned bias per head and bucket of the relative position, added to the scores beside the rotation).
+17 tokens, 512 wide, 4 layers, fp32: 4.1 ms against 5.5, with both options below 3.9 ms against 7.5).  They take heads of a multiple of 8
+up to 128 in fp32 or bf16, also under autocast; others raise in the first forward call on the GPU.  On the CPU such a module computes the
+same in torch.  Two options of a block that the reference has not: gated=True (act(gate) * up in the feed-forward, fc1 twice as wide) and
+rel_buckets > 0 (a learned bias per head and bucket of the relative position, added to the scores beside the rotation).
 Dropout > 0 is not built (vita.yaml ships 0.0)."""
 from __future__ import annotations
 

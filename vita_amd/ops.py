@@ -1745,7 +1745,8 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, scale: Optional[float] = None,
     (2 R + 1,), the bucket of each distance -R .. R (relative_buckets): adds table[bucket of (key - query position), h] to the scores.
     need_lse: also the row statistics that attention_bwd takes, (B, H, Sq, n) fp32: [..., 0] a maximum m of the row's scores times log2 e,
     [..., 1] r = 1 / sum 2 ** (score log2 e - m), so that log sum exp = m ln 2 - ln r, (0, 0) for a query without keys; bf16: behind them
-    what the result lost when it was rounded (probabilities are then multiplied in two bf16 parts: the result is nearer than without).
+    what the result lost when it was rounded (the probabilities of a row's first 256 keys are then multiplied in two bf16 parts: the result
+    is nearer than without and can differ from it in the last bit).
     out: the result's tensor, which shares no memory with the others.  Differentiable in q, k, v and table."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, table)):
         if out is not None:

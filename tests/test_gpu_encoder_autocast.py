@@ -32,3 +32,15 @@ def test_gated_product_takes_autocast_type(monkeypatch):
         assert (got.double().cpu() - ref).abs().max().item() <= 0.05 * ref.abs().max().item()
     blk(a)
     assert seen[1:] == [(torch.float32,) * 3]
+
+
+def test_gated_product_keeps_its_type_under_float16():
+    torch.manual_seed(7)
+    mlp = encoders._GatedMlp(32, 48, kernels=True).to(DEV)
+    x = torch.randn(3, 5, 32, device=DEV)
+    with torch.autocast("cuda", dtype=torch.float16):
+        y = mlp(x)
+    want = mlp(x)
+    assert ops.gated_linear(x.view(15, 32), mlp.fc1.weight, mlp.fc1.bias, "gelu_tanh").abs().max().item() <= 4
+    # fc2 alone runs in float16: its operands' and its result's roundings of 2^-11, on values of at most 4
+    assert y.dtype == torch.float16 and (y.float() - want).abs().max().item() <= 3 * 2.0 ** -11 * (mlp.fc2.weight.abs().sum(1).max() * 4).item()

@@ -123,8 +123,9 @@ class _GatedMlp(nn.Module):
 
     def forward(self, x):
         if self.kernels and x.is_cuda:
-            if torch.is_autocast_enabled("cuda") and x.dtype != torch.float64:          # what autocast does to an nn.Linear's input
-                x = x.to(torch.get_autocast_dtype("cuda"))
+            # what autocast does to an nn.Linear's input (float16 is no type of the kernels: the product stays in the input's)
+            if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16 and x.dtype != torch.float64:
+                x = x.bfloat16()
             h = ops.gated_linear(x.reshape(-1, x.shape[-1]), self.fc1.weight.to(x.dtype), self.fc1.bias.float(), "gelu_tanh")
             return self.fc2(h.view(*x.shape[:-1], -1))
         gate, up = self.fc1(x).chunk(2, dim=-1)
